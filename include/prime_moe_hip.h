@@ -170,11 +170,59 @@ int pmoe_quantize_mx(const void *src_bf16, void *q, void *scales, int64_t rows, 
  */
 #define PMOE_DTYPE_F32 0
 #define PMOE_DTYPE_BF16 1
+#define PMOE_DTYPE_F16 2 /* the ragged products and quantize_int8 only */
 int pmoe_route(const void *logits, int logits_dtype, const float *bias, int32_t *topk_ids,
                float *topk_weights, int32_t *sorted_token_ids, int32_t *expert_ids,
                int32_t *num_tokens_post_padded, int n_tokens, int num_experts, int top_k,
                int block_m, int pad_to, int max_padded, int max_blocks, void *workspace,
                size_t workspace_bytes, void *stream);
+
+/*
+ * Ragged expert products: the experts' matrices on their own, for layers that the fused calls do not cover (other
+ * activations, training, 8-bit integers).  No counterpart in the reference.  Rows are sorted by expert: group g holds rows
+ * offsets[g-1] .. offsets[g]-1 (from 0 for g == 0), offsets (n_groups) int32 on the device, non-decreasing and within
+ * 0 .. M, at most 1024 groups.  Offsets that are not leave the outputs unspecified, but no access leaves the arguments.
+ * Strides are in elements; the dimension without a stride is contiguous.  Nothing is allocated, no call needs a workspace,
+ * the outputs do not depend on anything but the inputs (no atomics), and no call synchronises the host.
+ *
+ * expert_offsets -- the ends of the groups of a schedule of pmoe_moe_align with block_m == pad_to == 1 (a sorted
+ *   permutation): expert_ids (n) int32, the first num_tokens_post_padded[0] of them sorted.
+ */
+int pmoe_expert_offsets(const int32_t *expert_ids, const int32_t *num_tokens_post_padded, int32_t *offsets, int n,
+                        int n_groups, void *stream);
+
+/*
+ * grouped_mm -- out (M,N) = x (M,K) times w[g]^T of each row's group; zero for rows >= offsets[n_groups-1].
+ *   bf16 or fp16, fp32 sums, rounded once.  w: n_groups matrices w_group_stride apart; w_across == 0: (N,K), rows
+ *   w_stride apart; w_across != 0: the same matrices stored (K,N).  With w_across it is the gradient with respect to x of
+ *   the product without, and the other way round.  N, K and strides multiples of 8 (x and w 16-byte aligned).
+ */
+int pmoe_grouped_mm(const void *x, const void *w, void *out, const int32_t *offsets, int n_groups, int64_t M, int N, int K,
+                    int64_t x_stride, int64_t w_stride, int64_t w_group_stride, int w_across, int dtype, void *stream);
+
+/*
+ * grouped_mm_wgrad -- dw (n_groups,N,K), contiguous: the sum over a group's rows of dy[r]^T x[r]; zero for an empty group.
+ *   dy (M,N), x (M,K) bf16 or fp16, fp32 sums, rounded once.
+ */
+int pmoe_grouped_mm_wgrad(const void *dy, const void *x, void *dw, const int32_t *offsets, int n_groups, int64_t M, int N,
+                          int K, int64_t dy_stride, int64_t x_stride, int dtype, void *stream);
+
+/*
+ * grouped_mm_int8 -- out[r][n] = (sum over k of x[r][k] w[g][n][k]) x_scale[r] w_scale[g][n]; int8 values, exact 32-bit sums
+ *   (K < 131072), fp32 scales, out bf16, fp16 or fp32 (out_dtype); zero for rows behind the last group.  offsets == NULL:
+ *   one group of all rows (a dense product).  N a multiple of 8, K and strides multiples of 16 (x and w 16-byte aligned).
+ */
+int pmoe_grouped_mm_int8(const void *x, const void *w, const float *x_scale, const float *w_scale, void *out,
+                         const int32_t *offsets, int n_groups, int64_t M, int N, int K, int64_t x_stride, int64_t w_stride,
+                         int64_t w_group_stride, int out_dtype, void *stream);
+
+/*
+ * quantize_int8 -- the step in front of grouped_mm_int8: scales[r] = max(amax(row) c, 2^-126) with c = 1 / 127, all in fp32, q =
+ *   the integer nearest to the exact quotient of value and scale, ties to even.  A row with an infinity or a NaN gets the scale NaN and
+ *   zeros.  src (rows, cols) bf16, fp16 or fp32, rows `stride` elements apart; cols and stride multiples of 8.
+ */
+int pmoe_quantize_int8(const void *src, int dtype, void *q, float *scales, int64_t rows, int cols, int64_t stride,
+                       void *stream);
 
 #ifdef __cplusplus
 }

@@ -9,6 +9,7 @@
 // call, which the device spends less than on a single token.
 #include <limits>
 
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 #include <torch/library.h>
 #include <ATen/ATen.h>
@@ -246,6 +247,263 @@ void fused_moe_mxfp8(const Tensor &x, const Tensor &x_scales, const Tensor &w, c
         (int)bpc, split, ws.data_ptr(), (size_t)ws.numel(), stream_of(dev)));
 }
 
+// ------------------------------------------------------------------------------- ragged expert products
+
+// What the checks below find out about a matrix, or a stack of them, whose rows are `stride` elements apart.
+struct Rows {
+    int64_t stride = 0;        // between rows
+    int64_t group_stride = 0;  // between matrices
+    bool across = false;       // stored transposed
+};
+// A stride that no access uses (a single row) may be anything: it is taken as the least that the kernels accept.
+int64_t stride_of(const Tensor &t, int64_t dim, int64_t least) {
+    return t.size(dim) > 1 ? t.stride(dim) : (least + 15) / 16 * 16;
+}
+void require_rows(const char *op, const char *name, const Tensor &t, int64_t unit, int64_t stride, int64_t width) {
+    REQUIRE(stride >= width && stride % unit == 0 && stride <= (8 << 20) / t.element_size(), op, ": the rows of ", name, " are ", stride,
+            " elements apart; supported are multiples of ", unit, " from ", width, " to ", (8 << 20) / t.element_size());
+}
+Rows rows_of(const char *op, const char *name, const Tensor &t, int64_t unit) {
+    Rows r;
+    REQUIRE(t.size(1) == 1 || t.stride(1) == 1, op, ": the last dimension of ", name, " must be contiguous");
+    r.stride = stride_of(t, 0, t.size(1));
+    if (t.numel() > 0) require_rows(op, name, t, unit, r.stride, t.size(1));
+    return r;
+}
+// `w` (E, N, K): K contiguous, or (`transposed`) N.
+Rows stack_of(const char *op, const Tensor &w, int64_t unit, bool transposed) {
+    Rows r;
+    r.across = transposed && w.stride(2) != 1 && w.stride(1) == 1;
+    REQUIRE(r.across || w.stride(2) == 1, op, ": ", transposed ? "one of the last two dimensions" : "the last dimension", " of w must be contiguous");
+    const int64_t along = r.across ? 1 : 2;
+    r.stride = stride_of(w, 3 - along, w.size(along));
+    require_rows(op, "w", w, unit, r.stride, w.size(along));
+    r.group_stride = w.size(0) > 1 ? w.stride(0) : 0;
+    REQUIRE(r.group_stride % unit == 0, op, ": the matrices of w are ", r.group_stride, " elements apart, which is not a multiple of ", unit);
+    return r;
+}
+int dtype_code(at::ScalarType t) {
+    return t == at::kFloat ? PMOE_DTYPE_F32 : t == at::kBFloat16 ? PMOE_DTYPE_BF16 : t == at::kHalf ? PMOE_DTYPE_F16 : -1;
+}
+void require_16bit(const char *op, const char *name, const Tensor &t) {
+    REQUIRE(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, op, ": ", name, " must be bfloat16 or float16");
+}
+constexpr int64_t kMostGroups = 1024, kMostRows = std::numeric_limits<int32_t>::max() - 512, kMostSide = 1 << 28;
+void require_groups(const char *op, const Tensor &offsets, int64_t groups) {
+    REQUIRE(offsets.dim() == 1 && offsets.is_contiguous() && offsets.scalar_type() == at::kInt, op, ": offsets must be a contiguous int32 (E,) tensor");
+    REQUIRE(groups < 0 || offsets.size(0) == groups, op, ": offsets must have one entry per matrix of w (", groups, "), got ", offsets.size(0));
+    REQUIRE(offsets.size(0) > 0 && offsets.size(0) <= kMostGroups, op, " supports 1..", kMostGroups, " experts, got ", offsets.size(0));
+}
+void require_side(const char *op, const char *name, int64_t n, int64_t unit) {
+    REQUIRE(n > 0 && n % unit == 0 && n <= kMostSide, op, ": ", name, " must be a positive multiple of ", unit, " up to 2^28, got ", n);
+}
+
+struct MmPlan {
+    Rows x, w;
+};
+MmPlan check_grouped_mm(const Tensor &x, const Tensor &w, const Tensor &offsets, bool placement) {
+    const char *op = "grouped_mm";
+    REQUIRE(x.dim() == 2 && w.dim() == 3, op, ": x must be 2-D (M, K), w 3-D (E, N, K)");
+    REQUIRE(x.size(1) == w.size(2), op, ": x.size(1) must equal w.size(2), got ", x.size(1), " and ", w.size(2));
+    require_16bit(op, "x", x);
+    REQUIRE(w.scalar_type() == x.scalar_type(), op, ": x and w must have the same dtype");
+    REQUIRE(x.size(0) <= kMostRows, op, ": too many rows");
+    require_side(op, "N", w.size(1), 8);
+    require_side(op, "K", w.size(2), 8);
+    require_groups(op, offsets, w.size(0));
+    const MmPlan p{rows_of(op, "x", x, 8), stack_of(op, w, 8, true)};
+    if (placement) {
+        require_same_device(op, {{"x", &x}, {"w", &w}, {"offsets", &offsets}});
+        require_aligned(op, {{"x", &x}, {"w", &w}}, 16);
+    }
+    return p;
+}
+Tensor grouped_mm(const Tensor &x, const Tensor &w, const Tensor &offsets) {
+    const MmPlan p = check_grouped_mm(x, w, offsets, true);
+    const c10::Device dev = x.device();
+    const c10::DeviceGuard guard(dev);
+    Tensor out = empty({x.size(0), w.size(1)}, x.scalar_type(), dev);
+    check_status(pmoe_grouped_mm(x.const_data_ptr(), w.const_data_ptr(), out.data_ptr(), offsets.const_data_ptr<int32_t>(), (int)w.size(0),
+                                 x.size(0), (int)w.size(1), (int)w.size(2), p.x.stride, p.w.stride, p.w.group_stride, p.w.across,
+                                 dtype_code(x.scalar_type()), stream_of(dev)));
+    return out;
+}
+
+MmPlan check_grouped_mm_wgrad(const Tensor &dy, const Tensor &x, const Tensor &offsets, bool placement) {
+    const char *op = "grouped_mm_wgrad";
+    REQUIRE(dy.dim() == 2 && x.dim() == 2 && dy.size(0) == x.size(0), op, ": dy (M, N) and x (M, K) must be 2-D with the same number of rows");
+    require_16bit(op, "x", x);
+    REQUIRE(dy.scalar_type() == x.scalar_type(), op, ": dy and x must have the same dtype");
+    REQUIRE(x.size(0) <= kMostRows, op, ": too many rows");
+    require_side(op, "N", dy.size(1), 8);
+    require_side(op, "K", x.size(1), 8);
+    require_groups(op, offsets, -1);
+    const MmPlan p{rows_of(op, "dy", dy, 8), rows_of(op, "x", x, 8)};
+    if (placement) {
+        require_same_device(op, {{"dy", &dy}, {"x", &x}, {"offsets", &offsets}});
+        require_aligned(op, {{"dy", &dy}, {"x", &x}}, 16);
+    }
+    return p;
+}
+Tensor grouped_mm_wgrad(const Tensor &dy, const Tensor &x, const Tensor &offsets) {
+    const MmPlan p = check_grouped_mm_wgrad(dy, x, offsets, true);
+    const c10::Device dev = x.device();
+    const c10::DeviceGuard guard(dev);
+    Tensor dw = empty({offsets.size(0), dy.size(1), x.size(1)}, x.scalar_type(), dev);
+    check_status(pmoe_grouped_mm_wgrad(dy.const_data_ptr(), x.const_data_ptr(), dw.data_ptr(), offsets.const_data_ptr<int32_t>(),
+                                       (int)offsets.size(0), x.size(0), (int)dy.size(1), (int)x.size(1), p.x.stride, p.w.stride,
+                                       dtype_code(x.scalar_type()), stream_of(dev)));
+    return dw;
+}
+
+// Gradients.  Each of the two operators has its gradients in terms of both, so gradients of gradients exist too.  What
+// comes back from a loss may have any strides (an expanded scalar): it is laid out first where the kernels need it.
+using Product = Tensor(const Tensor &, const Tensor &, const Tensor &);
+Tensor call_mm(const Tensor &x, const Tensor &w, const Tensor &offsets) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("prime_moe::grouped_mm", "").typed<Product>();
+    return op.call(x, w, offsets);
+}
+Tensor call_wgrad(const Tensor &dy, const Tensor &x, const Tensor &offsets) {
+    static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("prime_moe::grouped_mm_wgrad", "").typed<Product>();
+    return op.call(dy, x, offsets);
+}
+
+Tensor laid_out(const Tensor &t) {
+    const bool fine = (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) % 8 == 0 && t.stride(0) <= 4 << 20)) &&
+                      t.storage_offset() % 8 == 0;
+    return fine ? t : t.contiguous();
+}
+
+struct GroupedMm : torch::autograd::Function<GroupedMm> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &x, const Tensor &w, const Tensor &offsets) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({x, w, offsets});
+        return call_mm(x, w, offsets);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        Tensor dx, dw;
+        if (grads[0].defined()) {
+            const Tensor dy = laid_out(grads[0]);
+            if (ctx->needs_input_grad(0)) dx = call_mm(dy, saved[1].transpose(1, 2), saved[2]);
+            if (ctx->needs_input_grad(1)) dw = call_wgrad(dy, saved[0], saved[2]);
+        }
+        return {dx, dw, Tensor()};
+    }
+};
+struct GroupedMmWgrad : torch::autograd::Function<GroupedMmWgrad> {
+    static Tensor forward(torch::autograd::AutogradContext *ctx, const Tensor &dy, const Tensor &x, const Tensor &offsets) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        ctx->save_for_backward({dy, x, offsets});
+        return call_wgrad(dy, x, offsets);
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        Tensor ddy, dx;
+        if (grads[0].defined()) {
+            const Tensor g = grads[0].contiguous();  // (E, N, K)
+            if (ctx->needs_input_grad(0)) ddy = call_mm(saved[1], g, saved[2]);
+            if (ctx->needs_input_grad(1)) dx = call_mm(saved[0], g.transpose(1, 2), saved[2]);
+        }
+        return {ddy, dx, Tensor()};
+    }
+};
+bool differentiated(const Tensor &a, const Tensor &b) { return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad()); }
+Tensor grouped_mm_autograd(const Tensor &x, const Tensor &w, const Tensor &offsets) {
+    if (differentiated(x, w)) return GroupedMm::apply(x, w, offsets);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_mm(x, w, offsets);
+}
+Tensor grouped_mm_wgrad_autograd(const Tensor &dy, const Tensor &x, const Tensor &offsets) {
+    if (differentiated(dy, x)) return GroupedMmWgrad::apply(dy, x, offsets);
+    at::AutoDispatchBelowADInplaceOrView below;
+    return call_wgrad(dy, x, offsets);
+}
+
+MmPlan check_grouped_mm_int8(const Tensor &x, const Tensor &w, const Tensor &x_scale, const Tensor &w_scale, const std::optional<Tensor> &offsets,
+                             at::ScalarType out_dtype, bool placement) {
+    const char *op = "grouped_mm_int8";
+    const bool dense = !offsets.has_value();
+    REQUIRE(x.dim() == 2 && w.dim() == (dense ? 2 : 3), op, ": x must be 2-D (M, K), w 3-D (E, N, K) with offsets and 2-D (N, K) without");
+    REQUIRE(x.size(1) == w.size(-1), op, ": x.size(1) must equal w.size(-1), got ", x.size(1), " and ", w.size(-1));
+    REQUIRE(x.scalar_type() == at::kChar && w.scalar_type() == at::kChar, op, ": x and w must be int8");
+    REQUIRE(dtype_code(out_dtype) >= 0, op, ": out_dtype must be bfloat16, float16 or float32");
+    REQUIRE(x.size(0) <= kMostRows, op, ": too many rows");
+    require_side(op, "N", w.size(-2), 8);
+    require_side(op, "K", w.size(-1), 16);
+    REQUIRE(x.size(1) < 131072, op, ": K must be below 131072 (exact sums in 32 bits), got ", x.size(1));
+    if (!dense) require_groups(op, *offsets, w.size(0));
+    REQUIRE(x_scale.scalar_type() == at::kFloat && x_scale.is_contiguous() && x_scale.dim() == 1 && x_scale.size(0) == x.size(0), op,
+            ": x_scale must be a contiguous float32 (M,) tensor");
+    REQUIRE(w_scale.scalar_type() == at::kFloat && w_scale.is_contiguous() && w_scale.sizes() == w.sizes().slice(0, w.dim() - 1), op,
+            ": w_scale must be a contiguous float32 tensor of shape ", dense ? "(N,)" : "(E, N)");
+    const MmPlan p{rows_of(op, "x", x, 16), dense ? rows_of(op, "w", w, 16) : stack_of(op, w, 16, false)};
+    if (placement) {
+        require_same_device(op, {{"x", &x}, {"w", &w}, {"x_scale", &x_scale}, {"w_scale", &w_scale}});
+        if (!dense) require_same_device(op, {{"x", &x}, {"offsets", &*offsets}});
+        require_aligned(op, {{"x", &x}, {"w", &w}}, 16);
+    }
+    return p;
+}
+Tensor grouped_mm_int8(const Tensor &x, const Tensor &w, const Tensor &x_scale, const Tensor &w_scale, const std::optional<Tensor> &offsets,
+                       at::ScalarType out_dtype) {
+    const MmPlan p = check_grouped_mm_int8(x, w, x_scale, w_scale, offsets, out_dtype, true);
+    const c10::Device dev = x.device();
+    const c10::DeviceGuard guard(dev);
+    Tensor out = empty({x.size(0), w.size(-2)}, out_dtype, dev);
+    check_status(pmoe_grouped_mm_int8(x.const_data_ptr(), w.const_data_ptr(), x_scale.const_data_ptr<float>(), w_scale.const_data_ptr<float>(),
+                                      out.data_ptr(), offsets.has_value() ? offsets->const_data_ptr<int32_t>() : nullptr,
+                                      offsets.has_value() ? (int)w.size(0) : 1, x.size(0), (int)w.size(-2), (int)x.size(1), p.x.stride,
+                                      p.w.stride, p.w.group_stride, dtype_code(out_dtype), stream_of(dev)));
+    return out;
+}
+
+// `x` (..., K): rows of the last dimension; a 2-D view may have rows any multiple of 8 elements apart.
+int64_t check_quantize_int8(const Tensor &x, bool placement) {
+    const char *op = "quantize_int8";
+    REQUIRE(dtype_code(x.scalar_type()) >= 0, op, ": x must be bfloat16, float16 or float32");
+    REQUIRE(x.dim() > 0, op, ": x must have a dimension");
+    const int64_t cols = x.size(-1);
+    require_side(op, "the last dimension", cols, 8);
+    REQUIRE(x.is_contiguous() || (x.dim() == 2 && x.stride(1) == 1), op, ": x must be contiguous, or 2-D with a contiguous last dimension");
+    const int64_t stride = x.is_contiguous() || x.size(0) <= 1 ? cols : x.stride(0);
+    REQUIRE(stride >= cols && stride % 8 == 0, op, ": the rows of x are ", stride, " elements apart; supported are multiples of 8 from ", cols, " on");
+    if (placement) {
+        require_same_device(op, {{"x", &x}});
+        require_aligned(op, {{"x", &x}}, 16);
+    }
+    return stride;
+}
+std::tuple<Tensor, Tensor> quantize_int8(const Tensor &x) {
+    const int64_t stride = check_quantize_int8(x, true);
+    const c10::Device dev = x.device();
+    const c10::DeviceGuard guard(dev);
+    Tensor q = empty(x.sizes(), at::kChar, dev), scale = empty(x.sizes().slice(0, x.dim() - 1), at::kFloat, dev);
+    check_status(pmoe_quantize_int8(x.const_data_ptr(), dtype_code(x.scalar_type()), q.data_ptr(), scale.data_ptr<float>(),
+                                    x.numel() / x.size(-1), (int)x.size(-1), stride, stream_of(dev)));
+    return {q, scale};
+}
+
+void check_expert_offsets(const Tensor &expert_ids, const Tensor &total, int64_t num_experts, bool placement) {
+    const char *op = "expert_offsets";
+    const Arg ae{"expert_ids", &expert_ids}, at_{"num_tokens_post_padded", &total};
+    require_dtype(op, {ae, at_}, at::kInt, "int32");
+    require_contiguous(op, {ae, at_});
+    REQUIRE(num_experts > 0 && num_experts <= kMostGroups, op, " supports 1..", kMostGroups, " experts, got ", num_experts);
+    REQUIRE(expert_ids.numel() <= kMostRows, op, ": too many rows");
+    REQUIRE(total.numel() >= 1, op, ": num_tokens_post_padded is empty");
+    if (placement) require_same_device(op, {ae, at_});
+}
+Tensor expert_offsets(const Tensor &expert_ids, const Tensor &total, int64_t num_experts) {
+    check_expert_offsets(expert_ids, total, num_experts, true);
+    const c10::Device dev = expert_ids.device();
+    const c10::DeviceGuard guard(dev);
+    Tensor offsets = empty({num_experts}, at::kInt, dev);
+    check_status(pmoe_expert_offsets(expert_ids.const_data_ptr<int32_t>(), total.const_data_ptr<int32_t>(), offsets.data_ptr<int32_t>(),
+                                     (int)expert_ids.numel(), (int)num_experts, stream_of(dev)));
+    return offsets;
+}
+
 // ------------------------------------------------------------------------------- helpers that are not ops
 
 std::tuple<Tensor, Tensor> quantize_mx(const Tensor &t) {
@@ -298,6 +556,16 @@ TORCH_LIBRARY_IMPL(prime_moe, CUDA, m) {
     m.impl("moe_align", &moe_align);
     m.impl("fused_moe_bf16", &fused_moe_bf16);
     m.impl("fused_moe_mxfp8", &fused_moe_mxfp8);
+    m.impl("grouped_mm", &grouped_mm);
+    m.impl("grouped_mm_wgrad", &grouped_mm_wgrad);
+    m.impl("grouped_mm_int8", &grouped_mm_int8);
+    m.impl("quantize_int8", &quantize_int8);
+    m.impl("expert_offsets", &expert_offsets);
+}
+
+TORCH_LIBRARY_IMPL(prime_moe, AutogradCUDA, m) {
+    m.impl("grouped_mm", &grouped_mm_autograd);
+    m.impl("grouped_mm_wgrad", &grouped_mm_wgrad_autograd);
 }
 
 PYBIND11_MODULE(_torch_ops, m) {
@@ -306,6 +574,12 @@ PYBIND11_MODULE(_torch_ops, m) {
     m.def("validate_align", &validate_align, nogil);
     m.def("validate_bf16", &validate_bf16, nogil);
     m.def("validate_mxfp8", &validate_mxfp8, nogil);
+    m.def("validate_grouped_mm", [](const Tensor &x, const Tensor &w, const Tensor &o) { check_grouped_mm(x, w, o, false); }, nogil);
+    m.def("validate_grouped_mm_wgrad", [](const Tensor &dy, const Tensor &x, const Tensor &o) { check_grouped_mm_wgrad(dy, x, o, false); }, nogil);
+    m.def("validate_grouped_mm_int8", [](const Tensor &x, const Tensor &w, const Tensor &xs, const Tensor &ws, const std::optional<Tensor> &o,
+                                         at::ScalarType t) { check_grouped_mm_int8(x, w, xs, ws, o, t, false); }, nogil);
+    m.def("validate_quantize_int8", [](const Tensor &x) { check_quantize_int8(x, false); }, nogil);
+    m.def("validate_expert_offsets", [](const Tensor &e, const Tensor &n, int64_t k) { check_expert_offsets(e, n, k, false); }, nogil);
     m.def("quantize_mx", &quantize_mx, nogil);
     m.def("route", &route, nogil);
 }

@@ -32,6 +32,11 @@ _LIB.define(
     "int stages, int bpc, bool split=True) -> ()"
 )
 _LIB.define("moe_align(Tensor topk_ids, int num_experts, int block_m, int bpc) -> (Tensor, Tensor, Tensor)")
+_LIB.define("expert_offsets(Tensor expert_ids, Tensor num_tokens_post_padded, int num_experts) -> Tensor")
+_LIB.define("grouped_mm(Tensor x, Tensor w, Tensor offsets) -> Tensor")
+_LIB.define("grouped_mm_wgrad(Tensor dy, Tensor x, Tensor offsets) -> Tensor")
+_LIB.define("grouped_mm_int8(Tensor x, Tensor w, Tensor x_scale, Tensor w_scale, Tensor? offsets, ScalarType out_dtype) -> Tensor")
+_LIB.define("quantize_int8(Tensor x) -> (Tensor, Tensor)")
 
 
 try:
@@ -52,7 +57,8 @@ except ImportError as _err:
             return self._raise
 
     _torch_ops = _Unavailable(str(_err))
-    for _op in ("moe_align", "fused_moe_bf16", "fused_moe_mxfp8"):
+    for _op in ("moe_align", "fused_moe_bf16", "fused_moe_mxfp8", "expert_offsets", "grouped_mm", "grouped_mm_wgrad",
+                "grouped_mm_int8", "quantize_int8"):
         _LIB.impl(_op, _torch_ops._raise, "CUDA")
 
 
@@ -108,9 +114,36 @@ def _fused_moe_mxfp8_fake(x, x_scales, w, w_scales, w2, w2_scales, sorted_token_
     return None
 
 
+# ------------------------------------------------------------------------------- ragged expert products
+
+def _expert_offsets_fake(expert_ids, num_tokens_post_padded, num_experts):
+    return expert_ids.new_empty((num_experts,))
+
+
+def _grouped_mm_fake(x, w, offsets):
+    return x.new_empty((x.shape[0], w.shape[1]))
+
+
+def _grouped_mm_wgrad_fake(dy, x, offsets):
+    return x.new_empty((offsets.shape[0], dy.shape[1], x.shape[1]))
+
+
+def _grouped_mm_int8_fake(x, w, x_scale, w_scale, offsets, out_dtype):
+    return x.new_empty((x.shape[0], w.shape[-2]), dtype=out_dtype)
+
+
+def _quantize_int8_fake(x):
+    return x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
+
+
 torch.library.register_fake("prime_moe::moe_align", _moe_align_fake, lib=_LIB)
 torch.library.register_fake("prime_moe::fused_moe_bf16", _fused_moe_bf16_fake, lib=_LIB)
 torch.library.register_fake("prime_moe::fused_moe_mxfp8", _fused_moe_mxfp8_fake, lib=_LIB)
+torch.library.register_fake("prime_moe::expert_offsets", _expert_offsets_fake, lib=_LIB)
+torch.library.register_fake("prime_moe::grouped_mm", _grouped_mm_fake, lib=_LIB)
+torch.library.register_fake("prime_moe::grouped_mm_wgrad", _grouped_mm_wgrad_fake, lib=_LIB)
+torch.library.register_fake("prime_moe::grouped_mm_int8", _grouped_mm_int8_fake, lib=_LIB)
+torch.library.register_fake("prime_moe::quantize_int8", _quantize_int8_fake, lib=_LIB)
 
 
 # ------------------------------------------------------------------------------- public wrappers
@@ -177,7 +210,66 @@ def route(logits: torch.Tensor, top_k: int, block_m: int = 128, bpc: int = 1, bi
     return _torch_ops.route(logits, top_k, block_m, bpc, bias)
 
 
+def expert_offsets(expert_ids: torch.Tensor, num_tokens_post_padded: torch.Tensor, num_experts: int) -> torch.Tensor:
+    """``offsets`` of the ragged products below, from a schedule of ``moe_align`` / :func:`route` with ``block_m=1``.
+
+    Such a schedule is the permutation that sorts the pairs by expert without padding: ``sorted_token_ids`` holds the pair of
+    every row, ``expert_ids`` its expert.  Returns the end of every expert's rows, ``(num_experts,)`` int32; pairs that the
+    schedule drops (ids outside the experts) lie behind the last end.
+    """
+    return torch.ops.prime_moe.expert_offsets(expert_ids, num_tokens_post_padded, num_experts)
+
+
+def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """Rows by their expert's matrix: ``out[r] = w[g] @ x[r]`` for the rows ``offsets[g-1] <= r < offsets[g]`` of expert ``g``.
+
+    ``x`` (M, K), ``w`` (E, N, K), both bfloat16 or float16; ``offsets`` (E,) int32 on the same GPU, non-decreasing, at most
+    1024 experts.  Rows from ``offsets[-1]`` on come out as zeros.  Sums in fp32, rounded once.  ``x`` needs a contiguous last
+    dimension; ``w`` may be stored either way (``w.transpose(1, 2)`` of an (E, K, N) tensor).  K, N and the strides are
+    multiples of 8, tensors start 16-byte aligned.  Differentiable in ``x`` and ``w`` (any number of times).  Offsets are
+    read on the device and not checked: with other values the output is unspecified, but nothing outside the arguments is read
+    or written.
+    """
+    return torch.ops.prime_moe.grouped_mm(x, w, offsets)
+
+
+def grouped_mm_wgrad(dy: torch.Tensor, x: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
+    """Gradient of :func:`grouped_mm` with respect to ``w``: ``dw[g]`` is the sum of ``dy[r] x[r]^T`` over expert g's rows.
+
+    ``dy`` (M, N), ``x`` (M, K); returns (E, N, K), zeros for an expert without rows.  What the backward pass of
+    ``grouped_mm`` calls; for programs that accumulate weight gradients themselves.
+    """
+    return torch.ops.prime_moe.grouped_mm_wgrad(dy, x, offsets)
+
+
+def grouped_mm_int8(x: torch.Tensor, w: torch.Tensor, x_scale: torch.Tensor, w_scale: torch.Tensor,
+                    offsets: torch.Tensor = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """:func:`grouped_mm` of 8-bit integers: ``out[r, n] = (x[r] . w[g, n]) * x_scale[r] * w_scale[g, n]``.
+
+    ``x`` (M, K) and ``w`` (E, N, K) int8, ``x_scale`` (M,) and ``w_scale`` (E, N) float32.  Without ``offsets`` it is a dense
+    product with ``w`` (N, K) and ``w_scale`` (N,), such as a shared expert's.  Sums are exact (K < 131072); ``out_dtype``
+    bfloat16, float16 or float32.  N is a multiple of 8, K and the strides are multiples of 16.  No gradients.
+    """
+    return torch.ops.prime_moe.grouped_mm_int8(x, w, x_scale, w_scale, offsets, out_dtype)
+
+
+def quantize_int8(x: torch.Tensor):
+    """``(q, scale)`` of every row of the last dimension: ``scale = max(amax * (1 / 127), 2**-126)`` in float32, ``q`` the
+    integer nearest to ``x / scale`` (exactly, ties to even).
+
+    ``x`` (..., K) bfloat16, float16 or float32, K a multiple of 8; ``q`` int8 of the same shape, ``scale`` float32 of
+    ``x.shape[:-1]``: what :func:`grouped_mm_int8` takes for rows and, applied to (E, N, K) weights, for ``w``.  A row that
+    holds an infinity or a NaN gets the scale NaN and zeros.
+    """
+    return torch.ops.prime_moe.quantize_int8(x)
+
+
 __all__ = [
+    "expert_offsets",
+    "grouped_mm",
+    "grouped_mm_int8",
+    "grouped_mm_wgrad",
+    "quantize_int8",
     "route",
     "fused_moe_bf16",
     "fused_moe_mxfp8",

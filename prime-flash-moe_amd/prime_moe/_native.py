@@ -30,6 +30,11 @@ SIGNATURES = {
     "pmoe_fused_moe_mxfp8": (_c_int, [_c_void_p] * 11 + [_c_int] * 12 + [_c_void_p, _c_size_t, _c_void_p]),
     "pmoe_quantize_mx": (_c_int, [_c_void_p] * 3 + [ctypes.c_int64, _c_int, _c_void_p]),
     "pmoe_route": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 6 + [_c_int] * 7 + [_c_void_p, _c_size_t, _c_void_p]),
+    "pmoe_expert_offsets": (_c_int, [_c_void_p] * 3 + [_c_int] * 2 + [_c_void_p]),
+    "pmoe_grouped_mm": (_c_int, [_c_void_p] * 4 + [_c_int, ctypes.c_int64] + [_c_int] * 2 + [ctypes.c_int64] * 3 + [_c_int] * 2 + [_c_void_p]),
+    "pmoe_grouped_mm_wgrad": (_c_int, [_c_void_p] * 4 + [_c_int, ctypes.c_int64] + [_c_int] * 2 + [ctypes.c_int64] * 2 + [_c_int, _c_void_p]),
+    "pmoe_grouped_mm_int8": (_c_int, [_c_void_p] * 6 + [_c_int, ctypes.c_int64] + [_c_int] * 2 + [ctypes.c_int64] * 3 + [_c_int, _c_void_p]),
+    "pmoe_quantize_int8": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 2 + [ctypes.c_int64, _c_int, ctypes.c_int64, _c_void_p]),
     "pmoe_set_phase_mask": (None, [_c_int]),
     "pmoe_set_tiles_per_workgroup": (None, [_c_int]),
     "pmoe_set_compute_units": (None, [_c_int]),

@@ -18,7 +18,8 @@ CSRC = os.path.join(os.path.dirname(HERE), "csrc")
 OBJ_DIR = os.path.join(CSRC, "build")
 LIB_NAME = "libprime_moe_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
-SOURCES = ["api.hip", "moe_align.hip", "route.hip", "quantize_mx.hip", "fused_moe.hip", "fused_moe_bf16.hip"]
+SOURCES = ["api.hip", "moe_align.hip", "route.hip", "quantize_mx.hip", "fused_moe.hip", "fused_moe_bf16.hip",
+           "grouped_mm.hip", "grouped_int8.hip", "quantize_int8.hip"]
 ARCH = "gfx950"
 EXT_SOURCE = "torch_ops.cpp"
 EXT_PATH = os.path.join(HERE, "_torch_ops.so")
@@ -85,7 +86,7 @@ def _link_extension(obj: str, verbose: bool) -> None:
 
 def build(verbose: bool = True) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
-    with ThreadPoolExecutor(max_workers=7) as pool:
+    with ThreadPoolExecutor(max_workers=8) as pool:
         ext = pool.submit(_compile_extension, verbose)
         objs = list(pool.map(lambda s: _compile(s, verbose), SOURCES))
         ext_obj = ext.result()
