@@ -267,6 +267,7 @@ __device__ __forceinline__ void rows_feed(Feed<FM, false, QX> &feed, const RowsA
     feed.p.setup(tid, a.x + tile.row0 * a.x_pitch, a.x_pitch, tile.live);
     feed.q.setup(tid, a.w + tile.group * a.w_group + tile.col0 * (QX ? (int64_t)T::kBytes : a.w_pitch), a.w_pitch, min(kCols, a.cols - tile.col0));
     feed.set_length(tile.zero ? 0 : a.depth, T::kBytes);
+    feed.set_ahead(tid, a.x_pitch, tile.live, a.w_pitch, min(kCols, a.cols - tile.col0));
 }
 template <class T, bool QX>
 __device__ __forceinline__ void rows_start(const RowsArgs &a, const Tile &tile, char *lds, int tid) {
@@ -352,6 +353,7 @@ __global__ __launch_bounds__(kThreads, 1) void grouped_mm_wgrad_kernel(WgradArgs
         feed.p.setup(tid, a.dy + begin * a.dy_pitch + p.row0 * T::kBytes, a.dy_pitch, min(64 * FM, a.out_rows - p.row0));
         feed.q.setup(tid, a.x + begin * a.x_pitch + p.col0 * T::kBytes, a.x_pitch, min(kCols, a.cols - p.col0));
         feed.set_length(uniform(end - begin), T::kBytes);
+        feed.set_ahead(tid, a.dy_pitch, min(64 * FM, a.out_rows - p.row0), a.x_pitch, min(kCols, a.cols - p.col0));
     };
     int i = 0, t = walk_place(0);
     if (t >= total) return;

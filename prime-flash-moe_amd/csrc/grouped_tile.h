@@ -80,8 +80,27 @@ struct Geo {
 // What lies behind the end of a contraction.
 __device__ const uint4 g_zeros = {0, 0, 0, 0};
 
-__device__ __forceinline__ void copy16_at(const char *src, const char *lds_dst) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(ring::lds_addr(lds_dst)) : "memory");
+// Copies to `lds` (wave-uniform byte address) + OFF.  One scalar instruction in front of each: what stands between two matrix
+// instructions of the only wave of a SIMD has 32 cycles, and a longer chain of dependent scalar instructions (a wave number
+// read, shifted and added for every copy) cost 50 cycles a copy.
+template <int OFF>
+__device__ __forceinline__ void copy16(const char *base, uint32_t voff, uint32_t lds) {
+    asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(base), "s"(lds), "n"(OFF) : "memory", "scc");
+}
+template <int OFF>
+__device__ __forceinline__ void copy16_at(const char *src, uint32_t lds) {
+    asm volatile("s_add_u32 m0, %1, %2\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds), "n"(OFF) : "memory", "scc");
+}
+__device__ __forceinline__ void copy4_at(const char *src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" : : "v"(src), "s"(lds) : "memory");
+}
+// Calls f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>).
+template <int N, class F>
+__device__ __forceinline__ void unrolled(F f) {
+    if constexpr (N > 0) {
+        unrolled<N - 1>(f);
+        f(std::integral_constant<int, N - 1>());
+    }
 }
 
 // An operand of a tile.  ROWS: its rows (64 FM or 256) in a stage.
@@ -112,60 +131,65 @@ struct Operand {
             }
         }
     }
-    // Copy `i` of this wave's share of a slab.  END: the contraction may end inside the slab; `left` of it remains from the slab
-    // on, in bytes (along) or k rows (across).
-    template <bool END>
-    __device__ __forceinline__ void issue(int i, int tid, char *at, int64_t slab_off, int left) const {
-        const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        char *dst = at + (wave + kWaves * i) * 1024;
-        if constexpr (!END) {
-            ring::copy16(base + slab_off, off[i], dst);
-        } else {
-            const int lane = tid & 63, row = (wave + kWaves * i) * kPerPiece + lane / kLanes;
-            const int k = ACROSS ? row : ((lane % kLanes) ^ ((row >> 1) & 7)) * 16;
-            uint32_t o = off[i];
-            asm volatile("" : "+v"(o));  // (the 64-bit addresses of all pieces, kept through the whole contraction otherwise)
-            copy16_at(k < left ? base + slab_off + o : reinterpret_cast<const char *>(&g_zeros), dst);
-        }
+    // Byte offset of line `i` of a slab (ROWS lines of 128 B).
+    static __device__ __forceinline__ uint32_t line(int i, int64_t pitch, int live) {
+        if constexpr (ACROSS) return (uint32_t)(i / (ROWS / 64)) * (uint32_t)pitch + (uint32_t)min(i % (ROWS / 64) * 128, live * 2 - 4);
+        return (uint32_t)min(i, live - 1) * (uint32_t)pitch;
+    }
+    // Copy I of this wave's share of a slab to `at` (the wave's first piece) + AT.  END: the contraction may end inside the slab;
+    // `left` of it remains from the slab on, in bytes (along) or k rows (across).
+    template <int I, int AT>
+    __device__ __forceinline__ void issue(const char *slab, uint32_t at) const {
+        copy16<AT + I * kWaves * 1024>(slab, off[I], at);
+    }
+    template <int I, int AT>
+    __device__ __forceinline__ void issue_end(int tid, const char *slab, uint32_t at, int left) const {
+        const int wave = tid >> 6, lane = tid & 63, row = (wave + kWaves * I) * kPerPiece + lane / kLanes;
+        const int k = ACROSS ? row : ((lane % kLanes) ^ ((row >> 1) & 7)) * 16;
+        uint32_t o = off[I];
+        asm volatile("" : "+v"(o));  // (the 64-bit addresses of all pieces, kept through the whole contraction otherwise)
+        copy16_at<AT + I * kWaves * 1024>(k < left ? slab + o : reinterpret_cast<const char *>(&g_zeros), at);
     }
 };
 
-// Where this lane reads its fragments: `at[j]` for an operand along (step j of a slab, fragment f at f * 4 KB), `at[f & 3]`
-// for one across (step j at 16 j rows).
+// Where this lane reads its fragments, as LDS byte addresses in the current stage: `at[j]` for an operand along (step j of a
+// slab, fragment f 4 KB f behind), `at[f]` for one across (step j 16 j rows behind).
 template <int ROWS, bool ACROSS>
 struct Reader {
-    int at[4];
-    // `first`: the wave's first fragment in the operand
-    __device__ __forceinline__ void setup(int lane, int first) {
+    uint32_t at[4];
+    // `first`: the wave's first fragment in the operand, `lds`: the operand in the first stage
+    __device__ __forceinline__ void setup(int lane, int first, uint32_t lds) {
         if constexpr (ACROSS) {
             const int q = lane >> 4, i = lane & 15, k = 8 * (q >> 1) + (i >> 2);
 #pragma unroll
             for (int f = 0; f < 4; ++f) {
                 const int group = ((first + f) * 2 + (q & 1)) ^ ((k & 3) << 1);
-                at[f] = k * (ROWS * 2) + group * 32 + (i & 3) * 8;
+                at[f] = lds + k * (ROWS * 2) + group * 32 + (i & 3) * 8;
             }
         } else {
             const int r = lane & 31, half = lane >> 5, sx = (lane >> 1) & 7;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) at[j] = (first * 32 + r) * kSlab + (((2 * j + half) ^ sx) << 4);
+            for (int j = 0; j < 4; ++j) at[j] = lds + (first * 32 + r) * kSlab + (((2 * j + half) ^ sx) << 4);
         }
     }
-    __device__ __forceinline__ i32x4 read(const char *stage, int f, int j) const {
+    __device__ __forceinline__ i32x4 read(int f, int j) const {
         if constexpr (ACROSS) {
             typedef __attribute__((address_space(3))) s16x4 *lds4;
-            char *p = const_cast<char *>(stage) + at[f] + j * 16 * (ROWS * 2);
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)p);
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(p + 4 * (ROWS * 2)));
             typedef short s16x8 __attribute__((ext_vector_type(8)));
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at[f] + j * 16 * (ROWS * 2)));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at[f] + j * 16 * (ROWS * 2) + 4 * (ROWS * 2)));
             return __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
-            return *reinterpret_cast<const i32x4 *>(stage + at[j] + f * 32 * kSlab);
+            typedef const __attribute__((address_space(3))) i32x4 *lds16;
+            return *(lds16)(uintptr_t)(at[j] + f * 32 * kSlab);
         }
     }
 };
 
 // Nothing crosses this point in the instruction schedule.
 #define PMOE_GMM_FENCE() __builtin_amdgcn_sched_barrier(0)
+
+constexpr int kAhead = 1;  // slabs that lines are asked for in front of their copies (0, 2 and 3 are slower by 0.5 - 1 %)
 
 // A tile's operands and its place in the contraction.
 template <int FM, bool PX, bool QX>
@@ -175,100 +199,176 @@ struct Feed {
     Operand<kCols, QX> q;
     int n_slabs, full;  // slabs, and how many of them are whole
     int len_p, len_q;   // contraction in bytes (along) or elements (across)
+    // Lines of a slab that this workgroup asks the L2 for, kAhead slabs in front of its copies: of the row tile that its eight
+    // neighbours on the XCD share an eighth, of the column tile that four share a quarter, 24 lines per wave.  (The barrier
+    // of a slab waits for the slowest of 512 lines: without this, nearly always for one that missed the L2.)
+    const char *ahead;
+    int64_t ahead_step;
+    int ahead_slab;
 
+    __device__ __forceinline__ void set_ahead(int tid, int64_t p_pitch, int p_live, int64_t q_pitch, int q_live) {
+        const int slot = blockIdx.x / 8, wave = tid >> 6, lane = min(tid & 63, 23);
+        const bool is_p = lane < 8;
+        ahead = is_p ? p.base + Operand<G::kRows, PX>::line((slot & 7) * 8 * FM + wave * 2 * FM + min(lane, 2 * FM - 1), p_pitch, p_live)
+                     : q.base + Operand<kCols, QX>::line(((slot >> 3) & 3) * 64 + wave * 16 + lane - 8, q_pitch, q_live);
+        ahead_step = is_p ? p.step : q.step;
+        ahead_slab = min(G::kStages + kAhead, full - 1);
+        ahead += ahead_slab * ahead_step;
+        if (full == 0) ahead = reinterpret_cast<const char *>(&g_zeros);
+    }
+    // Behind the copies of a slab: one more copy, into the wave's scratch, which is free during a contraction.
+    __device__ __forceinline__ void ask_ahead(uint32_t sink) {
+        copy4_at(ahead, sink);
+        if (++ahead_slab < full) ahead += ahead_step;
+    }
     __device__ __forceinline__ void set_length(int elements, int bytes_per) {
         len_p = PX ? elements : elements * bytes_per;
         len_q = QX ? elements : elements * bytes_per;
         full = elements * bytes_per / kSlab;
         n_slabs = (elements * bytes_per + kSlab - 1) / kSlab;
     }
-    template <bool END>
-    __device__ __forceinline__ void issue(int c, int tid, char *stage, int slab) const {
-        if (c < G::kQPieces) q.template issue<END>(c, tid, stage + G::kPBytes, slab * q.step, len_q - slab * (QX ? 64 : kSlab));
-        else p.template issue<END>(c - G::kQPieces, tid, stage, slab * p.step, len_p - slab * (PX ? 64 : kSlab));
+    // `at`: the wave's first piece in the stage.
+    template <int C>
+    __device__ __forceinline__ void issue(uint32_t at, const char *p_slab, const char *q_slab) const {
+        if constexpr (C < G::kQPieces) q.template issue<C, G::kPBytes>(q_slab, at);
+        else p.template issue<C - G::kQPieces, 0>(p_slab, at);
     }
-    template <bool END>
-    __device__ __forceinline__ void issue_all(int tid, char *stage, int slab) const {
-#pragma unroll
-        for (int c = 0; c < G::kCopies; ++c) issue<END>(c, tid, stage, slab);
+    __device__ __forceinline__ void issue_all(int tid, uint32_t at, int slab) const {
+        const char *p_slab = p.base + slab * p.step, *q_slab = q.base + slab * q.step;
+        if (slab < full) {
+            unrolled<G::kCopies>([&](auto c) { issue<c.value>(at, p_slab, q_slab); });
+        } else {
+            unrolled<G::kQPieces>([&](auto c) { q.template issue_end<c.value, G::kPBytes>(tid, q_slab, at, len_q - slab * (QX ? 64 : kSlab)); });
+            unrolled<G::kPPieces>([&](auto c) { p.template issue_end<c.value, 0>(tid, p_slab, at, len_p - slab * (PX ? 64 : kSlab)); });
+        }
     }
     // The first slabs, up to all stages.
-    __device__ __forceinline__ void start(int tid, char *lds) const {
+    __device__ __forceinline__ void start(int tid, const char *lds) {
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), at = ring::lds_addr(lds);
 #pragma unroll 1
-        for (int s = 0; s < G::kStages; ++s) {
-            if (s < full) issue_all<false>(tid, lds + s * G::kStageBytes, s);
-            else if (s < n_slabs) issue_all<true>(tid, lds + s * G::kStageBytes, s);
+        for (int s = 0; s < min(G::kStages, n_slabs); ++s) {
+            issue_all(tid, at + s * G::kStageBytes + wave * 1024, s);
         }
     }
 };
 
-// Waits until at most `slabs` (wave-uniform, <= 3) slabs of copies are in flight and this wave's LDS reads have returned,
-// then joins the barrier.
+// Waits until at most `slabs` (wave-uniform, <= 2) slabs of copies are in flight and this wave's LDS reads have returned, then joins
+// the barrier.
 template <int COPIES>
 __device__ __forceinline__ void landed(int slabs) {
     if (slabs <= 0) ring::wait_and_barrier<0>();
     else if (slabs == 1) ring::wait_and_barrier<COPIES>();
-    else if (slabs == 2) ring::wait_and_barrier<2 * COPIES>();
-    else ring::wait_and_barrier<3 * COPIES>();
+    else ring::wait_and_barrier<2 * COPIES>();
 }
 
 // The contraction of one tile whose first slabs are on their way (Feed::start).  acc[f][t]: column fragment 4 wn + f
-// against row fragment FM wm + t.  Every wave is past the reads
-// of the last slab when one returns (n_slabs > 0): the stages may be filled again.
+// against row fragment FM wm + t.  Every wave is past the reads of the last slab when one returns (n_slabs > 0): the stages
+// may be filled again.
 template <class T, int FM, bool PX, bool QX>
-__device__ __forceinline__ void contract(typename T::Acc (&acc)[4][FM], const Feed<FM, PX, QX> &feed, char *lds, int tid) {
+__device__ __forceinline__ void contract(typename T::Acc (&acc)[4][FM], Feed<FM, PX, QX> &feed, const char *lds, int tid) {
     using G = Geo<FM>;
     constexpr int S = G::kStages, READS = 4 + FM, MM = 4 * FM;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), base = ring::lds_addr(lds);
+    const int lane = tid & 63, n = feed.n_slabs;
+    if (n == 0) {
+        ring::wait_and_barrier<0>();
+        return;
+    }
     Reader<G::kRows, PX> rp;
     Reader<kCols, QX> rq;
-    rp.setup(lane, (wave >> 1) * FM);
-    rq.setup(lane, (wave & 1) * 4);
-    const int n = feed.n_slabs;
+    rp.setup(lane, (wave >> 1) * FM, base);
+    rq.setup(lane, (wave & 1) * 4, base + G::kPBytes);
     landed<G::kCopies>(min(S, n) - 1);
 
     i32x4 a[2][4], b[2][FM];
-    auto read = [&](int r, int set, const char *stage, int j) {
-        if (r < 4) a[set][r] = rq.read(stage + G::kPBytes, r, j);
-        else b[set][r - 4] = rp.read(stage, r - 4, j);
+    auto read = [&](int r, int set, int j) {
+        if (r < 4) a[set][r] = rq.read(r, j);
+        else b[set][r - 4] = rp.read(r - 4, j);
     };
 #pragma unroll
-    for (int r = 0; r < READS; ++r) read(r, 0, lds, 0);
+    for (int r = 0; r < READS; ++r) read(r, 0, 0);
 
-    // Straight-line code for a slab, with branches around copies only: with the matrix instructions themselves in
-    // branches the compiler keeps a second set of accumulators and spills.
-    int cur = 0;
-    for (int k = 0; k < n; ++k) {
-        char *stage = lds + cur * G::kStageBytes;
-        cur = cur + 1 == S ? 0 : cur + 1;
-        const char *next = lds + cur * G::kStageBytes;
-        const bool fill = k + S < feed.full;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int set = j & 1;
-            if (j == 3) {
-                landed<G::kCopies>(min(S - 2, n - 2 - k));
-                if (k + S < n && !fill) feed.template issue_all<true>(tid, stage, k + S);
-            }
-            PMOE_GMM_FENCE();
-#pragma unroll
-            for (int m = 0; m < MM; ++m) {
-                const int t = m >> 2, f = m & 3;
-                acc[f][t] = T::mfma(a[set][f], b[set][t], acc[f][t]);
-                // the next step's fragments behind the first half of this step's instructions (behind the last slab:
-                // whatever the stage holds, which nobody uses)
+    // Where the next copies go: the wave's first piece in the stage of slab k, and slab k + S of the operands.
+    uint32_t into = base + wave * 1024;
+    const char *p_slab = feed.p.base + S * feed.p.step, *q_slab = feed.q.base + S * feed.q.step;
+    uint32_t stage = 0, by = 0;  // of slab k; to the next one
+    // Step J of a slab: its matrix instructions, the reads of the next step's fragments behind the first half of them, and
+    // copies FROM .. TO - 1 of a slab spread over all of them.  `more(m)` runs behind instruction m.
+    auto step = [&](auto J, auto read_next, auto from, auto to, auto more) {
+        constexpr int j = J.value, set = j & 1, FROM = from.value, COUNT = to.value - from.value;
+        unrolled<MM>([&](auto M) {
+            constexpr int m = M.value, t = m >> 2, f = m & 3;
+            acc[f][t] = T::mfma(a[set][f], b[set][t], acc[f][t]);
+            if constexpr (read_next.value) {
 #pragma unroll
                 for (int r = 0; r < READS; ++r)
-                    if (r * MM / (2 * READS) == m) read(r, set ^ 1, j < 3 ? stage : next, (j + 1) & 3);
-                if (j == 3 && m % 2 == 1 && fill) {
-#pragma unroll
-                    for (int c = 0; c < G::kCopies; ++c)
-                        if (c * (MM / 2) / G::kCopies == m / 2) feed.template issue<false>(c, tid, stage, k + S);
-                }
-                PMOE_GMM_FENCE();
+                    if (r * MM / (2 * READS) == m) read(r, set ^ 1, (j + 1) & 3);
             }
+            unrolled<COUNT>([&](auto c) {
+                if constexpr ((c.value * MM + MM / 2) / COUNT == m) feed.template issue<FROM + c.value>(into, p_slab, q_slab);
+            });
+            more(M);
+            PMOE_GMM_FENCE();
+        });
+    };
+    using Yes = std::integral_constant<bool, true>;
+    using No = std::integral_constant<bool, false>;
+#define PMOE_INT(v) std::integral_constant<int, (v)>()
+    // Copies are spread over two steps: in one, the four waves ask the address path of the CU for more than it takes (16 cycles
+    // a copy) and stand still; in three, the last ones have too little time to land.
+    constexpr int C1 = G::kCopies / 2, C2 = G::kCopies;
+
+    auto nothing = [](auto) {};
+    // The readers on to the next stage, among the last instructions of step 2, whose reads are the stage's last.
+    auto move = [&](auto M) {
+        constexpr int m = M.value;
+        if constexpr (m == MM / 2) {
+            by = stage + 1 == S ? 0u - (S - 1) * G::kStageBytes : G::kStageBytes;
+            stage = stage + 1 == S ? 0 : stage + 1;
+        } else if constexpr (m > MM / 2) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (MM / 2 + 1 + i * (MM / 2 - 1) / 8 == m) (i < 4 ? rp.at[i & 3] : rq.at[i & 3]) += by;
         }
+    };
+    // The slabs of the loops begin with step 3 of slab k and end with step 2 of slab k + 1.  No branch stands between matrix
+    // instructions: with them in branches the compiler keeps a second set of accumulators and spills.
+    step(PMOE_INT(0), Yes(), PMOE_INT(0), PMOE_INT(0), nothing);
+    step(PMOE_INT(1), Yes(), PMOE_INT(0), PMOE_INT(0), nothing);
+    step(PMOE_INT(2), Yes(), PMOE_INT(0), PMOE_INT(0), move);
+    int k = 0;
+    for (; k + S < feed.full; ++k) {
+        // slab k + 1 has landed; behind it are the line asked for ahead and the slabs up to k + S - 1 (the first S slabs
+        // have no line behind them)
+        if (k >= S) ring::wait_and_barrier<1 + (S - 2) * (G::kCopies + 1)>();
+        else ring::wait_and_barrier<(S - 2) * G::kCopies>();
+        PMOE_GMM_FENCE();
+        step(PMOE_INT(3), Yes(), PMOE_INT(0), PMOE_INT(C1), nothing);
+        step(PMOE_INT(0), Yes(), PMOE_INT(C1), PMOE_INT(C2), nothing);
+        step(PMOE_INT(1), Yes(), PMOE_INT(0), PMOE_INT(0), [&](auto M) {  // (no copy of the slab may follow)
+            if constexpr (M.value == MM / 2) feed.ask_ahead(base + kScratchOff + wave * kScratchBytes);
+            if constexpr (M.value == MM / 2 + 1) {
+                p_slab += feed.p.step;
+                q_slab += feed.q.step;
+                into = base + wave * 1024 + stage * G::kStageBytes;
+            }
+        });
+        step(PMOE_INT(2), Yes(), PMOE_INT(0), PMOE_INT(0), move);
     }
+    for (; k + 1 < n; ++k) {
+        landed<G::kCopies>(min(S - 2, n - 2 - k));
+        if (k + S < n) feed.issue_all(tid, into, k + S);
+        into = base + wave * 1024 + stage * G::kStageBytes;
+        PMOE_GMM_FENCE();
+        step(PMOE_INT(3), Yes(), PMOE_INT(0), PMOE_INT(0), nothing);
+        step(PMOE_INT(0), Yes(), PMOE_INT(0), PMOE_INT(0), nothing);
+        step(PMOE_INT(1), Yes(), PMOE_INT(0), PMOE_INT(0), nothing);
+        step(PMOE_INT(2), Yes(), PMOE_INT(0), PMOE_INT(0), move);
+    }
+    ring::wait_and_barrier<0>();
+    PMOE_GMM_FENCE();
+    step(PMOE_INT(3), No(), PMOE_INT(0), PMOE_INT(0), nothing);
+#undef PMOE_INT
 }
 
 }  // namespace gmm
