@@ -2,6 +2,7 @@
 // Sums are exact in 32 bits (the depth is limited to what cannot overflow); scales are applied in fp32 on the way out.
 #include <algorithm>
 
+#include "grouped_few.h"
 #include "grouped_host.h"
 #include "grouped_kernel.h"
 
@@ -12,6 +13,7 @@ using namespace pmoe::gmm;
 
 template <class OUT>
 void launch(const RowsArgs &a, int grid, hipStream_t stream) {
+    if (few::takes(a)) return few::launch<I8, OUT>(a, stream);
     hipLaunchKernelGGL((grouped_mm_kernel<I8, false, OUT>), dim3(grid), dim3(kThreads), 0, stream, a);
 }
 

@@ -1,6 +1,7 @@
 // Ragged expert products in bf16 and fp16: rows by their expert's weights, and the gradient of the weights.
 #include <algorithm>
 
+#include "grouped_few.h"
 #include "grouped_host.h"
 #include "grouped_kernel.h"
 
@@ -11,6 +12,8 @@ using namespace pmoe::gmm;
 
 template <class T, bool QX>
 void launch_rows(const RowsArgs &a, int grid, hipStream_t stream) {
+    if constexpr (!QX)
+        if (few::takes(a)) return few::launch<T, T>(a, stream);
     hipLaunchKernelGGL((grouped_mm_kernel<T, QX, T>), dim3(grid), dim3(kThreads), 0, stream, a);
 }
 

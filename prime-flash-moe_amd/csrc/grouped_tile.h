@@ -87,6 +87,11 @@ template <int OFF>
 __device__ __forceinline__ void copy16(const char *base, uint32_t voff, uint32_t lds) {
     asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(base), "s"(lds), "n"(OFF) : "memory", "scc");
 }
+// The same with the non-temporal hint, for what no other workgroup reads.
+template <int OFF>
+__device__ __forceinline__ void copy16_once(const char *base, uint32_t voff, uint32_t lds) {
+    asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1 nt" : : "v"(voff), "s"(base), "s"(lds), "n"(OFF) : "memory", "scc");
+}
 template <int OFF>
 __device__ __forceinline__ void copy16_at(const char *src, uint32_t lds) {
     asm volatile("s_add_u32 m0, %1, %2\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds), "n"(OFF) : "memory", "scc");
