@@ -47,14 +47,18 @@ struct Tile {
     bool zero;       // rows behind the last group: their outputs are zero
 };
 
-// Walk over the tiles of a launch.  A group's rows are cut into as few tiles as there can be, of even height (in
-// steps of 64 rows); tile number t runs through [group][8 column tiles][row tile][column tile], and the rows behind the
-// last group follow.  Thread i holds groups 4 i .. 4 i + 3 in registers.
+// Walk over the tiles of a launch.  A group's rows are cut into as few tiles as there can be, of even height (in steps of
+// 64 rows).  The walk takes the tallest tiles first: tile number t runs through [height, 4 to 1][group][8 column tiles][row
+// tile][column tile], and the rows behind the last group follow.  The workgroups, which take every grid-th tile, then have
+// equal shares of every height (in the order of the groups: the largest share 16 % above the mean with 128 groups of 512
+// rows on average), and a tile is nearly always followed by one of its own height.  Thread i holds groups 4 i .. 4 i + 3.
 struct Walk {
     int begin[5];   // first rows of the thread's groups, and the end of the last one
-    int before[5];  // row tiles in front of them
+    int before[4];  // row tiles in front of each
     int row_tiles, col_tiles, live_rows, total;
 
+    static __device__ __forceinline__ int tiles_of(int rows) { return (rows + 255) / 256; }
+    static __device__ __forceinline__ int height_of(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 63) & ~63; }
     __device__ __forceinline__ void setup(const RowsArgs &a, int tid, int *words) {
         const int g0 = 4 * tid, lane = tid & 63, wave = tid >> 6;
         // A group begins where the furthest end in front of it is (its predecessor's, if the ends are in order), so that
@@ -78,62 +82,75 @@ struct Walk {
             live_rows = max(live_rows, words[w]);
         }
         live_rows = uniform(live_rows);
-        int sum = 0, count[4];
+        int count[4], fm[4], sum[4] = {}, incl[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             begin[i + 1] = max(begin[i + 1], begin[i]);
-            count[i] = (begin[i + 1] - begin[i] + 255) / 256;
-            sum += count[i];
-        }
-        int incl = sum;
+            const int rows = begin[i + 1] - begin[i];
+            count[i] = tiles_of(rows);
+            fm[i] = rows > 0 ? height_of(rows, count[i]) / 64 : 0;
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const int v = __shfl_up(incl, d, 64);
-            if (lane >= d) incl += v;
+            for (int c = 0; c < 4; ++c) sum[c] += fm[i] == c + 1 ? count[i] : 0;
         }
-        if (lane == 63) words[kWaves + wave] = incl;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) incl[c] = sum[c];
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int v = __shfl_up(incl[c], d, 64);
+                if (lane >= d) incl[c] += v;
+            }
+        if (lane == 63)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) words[kWaves + 4 * wave + c] = incl[c];
         ring::all_read();
-        int lower = 0;
         row_tiles = 0;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-            if (w < wave) lower += words[kWaves + w];
-            row_tiles += words[kWaves + w];
+        for (int c = 3; c >= 0; --c) {
+            int at = row_tiles + incl[c] - sum[c];
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) {
+                const int v = words[kWaves + 4 * w + c];
+                if (w < wave) at += v;
+                row_tiles += v;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (fm[i] == c + 1) {
+                    before[i] = at;
+                    at += count[i];
+                }
         }
         ring::all_read();  // the words may be written again
-        before[0] = lower + incl - sum;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) before[i + 1] = before[i] + count[i];
         row_tiles = uniform(row_tiles);
         col_tiles = (a.cols + kCols - 1) / kCols;
         total = (row_tiles + (a.rows - live_rows + 255) / 256) * col_tiles;
     }
 
-    // Tile t < total, through five words of LDS that nobody else uses meanwhile.  Two barriers.
-    __device__ __forceinline__ Tile find(const RowsArgs &a, int t, int tid, int *words) const {
+    // Tile t < total, through four words of LDS: post(), a barrier, get().
+    __device__ __forceinline__ void post(int t, int tid, int *words) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int rows = begin[i + 1] - begin[i], rt = tiles_of(rows), local = t - before[i] * col_tiles;
+            if (rows > 0 && local >= 0 && local < rt * col_tiles) {
+                const int band = local / (rt * kWalkCols), width = min(kWalkCols, col_tiles - band * kWalkCols);
+                const int rem = local - band * rt * kWalkCols, m = rem / width, height = height_of(rows, rt);
+                words[0] = 4 * tid + i;
+                words[1] = begin[i] + m * height;
+                words[2] = min(height, rows - m * height);
+                words[3] = band * kWalkCols + rem - m * width;
+            }
+        }
+    }
+    __device__ __forceinline__ Tile get(const RowsArgs &a, int t, const int *words) const {
         Tile r;
         if (t < row_tiles * col_tiles) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int rt = before[i + 1] - before[i], local = t - before[i] * col_tiles;
-                if (local >= 0 && local < rt * col_tiles) {
-                    const int band = local / (rt * kWalkCols), width = min(kWalkCols, col_tiles - band * kWalkCols);
-                    const int rem = local - band * rt * kWalkCols, m = rem / width;
-                    const int rows = begin[i + 1] - begin[i];
-                    const int height = ((rows + rt - 1) / rt + 63) & ~63;
-                    words[0] = 4 * tid + i;
-                    words[1] = begin[i] + m * height;
-                    words[2] = min(height, rows - m * height);
-                    words[3] = band * kWalkCols + rem - m * width;
-                }
-            }
-            ring::all_read();
             r.group = uniform(words[0]);
             r.row0 = uniform(words[1]);
             r.live = uniform(words[2]);
             r.col0 = uniform(words[3]) * kCols;
             r.zero = false;
-            ring::all_read();
         } else {
             const int local = t - row_tiles * col_tiles, m = local / col_tiles;
             r.group = 0;
@@ -188,6 +205,7 @@ template <class T, int FM>
 struct Scales {
     static constexpr int kRowBytes = 256;  // of a row in scratch
     __device__ __forceinline__ void load(const RowsArgs &, const Tile &, int) {}
+    __device__ __forceinline__ void pin() {}
     __device__ __forceinline__ void keep(char *, int) const {}
     __device__ __forceinline__ float4 apply(const typename T::Acc &acc, int, int, int i4, const char *, int) const {
         return make_float4(acc[4 * i4], acc[4 * i4 + 1], acc[4 * i4 + 2], acc[4 * i4 + 3]);
@@ -209,6 +227,12 @@ struct Scales<I8, FM> {
             for (int t = 0; t < FM; ++t) x[t] = 0.f;
             w = make_float2(0.f, 0.f);
         }
+    }
+    // Waits for them here, where few copies are under way, and not in front of their first use.
+    __device__ __forceinline__ void pin() {
+#pragma unroll
+        for (int t = 0; t < FM; ++t) asm volatile("" : "+v"(x[t]));
+        asm volatile("" : "+v"(w.x), "+v"(w.y));
     }
     __device__ __forceinline__ void keep(char *scratch, int lane) const {
         *reinterpret_cast<float2 *>(scratch + kScratchBytes / 2 + lane * 8) = w;
@@ -269,39 +293,69 @@ __device__ __forceinline__ void rows_feed(Feed<FM, false, QX> &feed, const RowsA
     feed.set_length(tile.zero ? 0 : a.depth, T::kBytes);
     feed.set_ahead(tid, a.x_pitch, tile.live, a.w_pitch, min(kCols, a.cols - tile.col0));
 }
+// Copies of slab 0 or 1 of a tile of any height, all at once.
 template <class T, bool QX>
-__device__ __forceinline__ void rows_start(const RowsArgs &a, const Tile &tile, char *lds, int tid) {
-    auto start = [&](auto &feed) {
+__device__ __forceinline__ void rows_issue(const RowsArgs &a, const Tile &tile, int slab, uint32_t at, int tid) {
+    auto issue = [&](auto &feed) {
         rows_feed<T>(feed, a, tile, tid);
-        feed.start(tid, lds);
+        feed.issue_all(tid, at, slab);
     };
     switch (tile.fm) {
-        case 1: { Feed<1, false, QX> feed; start(feed); break; }
-        case 2: { Feed<2, false, QX> feed; start(feed); break; }
-        case 3: { Feed<3, false, QX> feed; start(feed); break; }
-        default: { Feed<4, false, QX> feed; start(feed); break; }
+        case 1: { Feed<1, false, QX> feed; issue(feed); break; }
+        case 2: { Feed<2, false, QX> feed; issue(feed); break; }
+        case 3: { Feed<3, false, QX> feed; issue(feed); break; }
+        default: { Feed<4, false, QX> feed; issue(feed); break; }
     }
 }
+
+// The walk of a workgroup.
+struct RowsState {
+    Tile tile;
+    int turn;        // of the tile, in this workgroup's list
+    uint32_t stage;  // of its slab 0
+};
+
 template <class T, bool QX, class OUT, int FM>
-__device__ __forceinline__ bool rows_tile(const RowsArgs &a, const Walk &walk, Tile &tile, int next, char *lds, int tid) {
-    typename T::Acc acc[4][FM] = {};
-    {
-        Feed<FM, false, QX> feed;
+struct RowsNext {
+    const RowsArgs &a;
+    const Walk &walk;
+    Scales<T, FM> &scales;
+    int *words;
+    int tid, place;
+    Tile tile;  // the next one, behind take()
+
+    __device__ __forceinline__ void post() const {
+        if (place < walk.total) walk.post(place, tid, words);
+    }
+    __device__ __forceinline__ void pin() { scales.pin(); }
+    __device__ __forceinline__ int take(Feed<FM, false, QX> &feed) {
+        if (place >= walk.total) return 0;
+        tile = walk.get(a, place, words);
+        if (tile.fm != FM) return 2;
         rows_feed<T>(feed, a, tile, tid);
-        contract<T>(acc, feed, lds, tid);
+        return 1;
     }
-    Scales<T, FM> scales;
-    scales.load(a, tile, tid);
-    char *out = a.out + tile.row0 * a.out_pitch + (int64_t)tile.col0 * Pack<OUT>::kBytes;
-    const int live = tile.live, cols = a.cols - tile.col0;
-    const bool more = next < walk.total;
-    if (more) {
-        tile = walk.find(a, next, tid, reinterpret_cast<int *>(lds + kScratchOff));
+    __device__ __forceinline__ void other(int slab, uint32_t at) const { rows_issue<T, QX>(a, tile, slab, at, tid); }
+};
+
+// The tiles of height FM that follow each other in the walk, `st.tile` on.  Returns whether one of another height follows.
+template <class T, bool QX, class OUT, int FM>
+__device__ __forceinline__ bool rows_run(const RowsArgs &a, const Walk &walk, RowsState &st, char *lds, int tid) {
+    Feed<FM, false, QX> feed;
+    rows_feed<T>(feed, a, st.tile, tid);
+    char *scratch = lds + kScratchOff + uniform(tid >> 6) * kScratchBytes;
+    while (true) {
+        typename T::Acc acc[4][FM] = {};
+        Scales<T, FM> scales;
+        scales.load(a, st.tile, tid);
+        RowsNext<T, QX, OUT, FM> next{a, walk, scales, reinterpret_cast<int *>(lds + kScratchOff), tid, walk_place(++st.turn), Tile()};
+        const int kind = contract<T>(acc, feed, lds, tid, st.stage, next);
+        scales.keep(scratch, tid & 63);
+        store_tile<T, OUT, FM>(acc, scales, lds, a.out + st.tile.row0 * a.out_pitch + (int64_t)st.tile.col0 * Pack<OUT>::kBytes, a.out_pitch,
+                               st.tile.live, a.cols - st.tile.col0, tid);
+        st.tile = next.tile;
+        if (kind != 1) return kind != 0;
     }
-    scales.keep(lds + kScratchOff + uniform(tid >> 6) * kScratchBytes, tid & 63);
-    if (more) rows_start<T, QX>(a, tile, lds, tid);
-    store_tile<T, OUT, FM>(acc, scales, lds, out, a.out_pitch, live, cols, tid);
-    return more;
 }
 
 template <class T, bool QX, class OUT>
@@ -311,71 +365,132 @@ __global__ __launch_bounds__(kThreads, 1) void grouped_mm_kernel(RowsArgs a) {
     int *words = reinterpret_cast<int *>(lds + kScratchOff);
     Walk walk;
     walk.setup(a, tid, words);
-    int i = 0;
-    if (walk_place(0) >= walk.total) return;
-    Tile tile = walk.find(a, walk_place(0), tid, words);
-    rows_start<T, QX>(a, tile, lds, tid);
+    const int place = walk_place(0);
+    if (place >= walk.total) return;
+    walk.post(place, tid, words);
+    ring::all_read();
+    RowsState st{walk.get(a, place, words), 0, 0};
+    const uint32_t at = ring::lds_addr(lds) + uniform(tid >> 6) * 1024;
+    rows_issue<T, QX>(a, st.tile, 0, at, tid);
+    rows_issue<T, QX>(a, st.tile, 1, at + kStageStride, tid);
+    wait_copies<Geo<1>::kCopies>();
     bool more = true;
     while (more) {
-        const int next = walk_place(++i);
-        switch (tile.fm) {
-            case 1: more = rows_tile<T, QX, OUT, 1>(a, walk, tile, next, lds, tid); break;
-            case 2: more = rows_tile<T, QX, OUT, 2>(a, walk, tile, next, lds, tid); break;
-            case 3: more = rows_tile<T, QX, OUT, 3>(a, walk, tile, next, lds, tid); break;
-            default: more = rows_tile<T, QX, OUT, 4>(a, walk, tile, next, lds, tid); break;
+        switch (st.tile.fm) {
+            case 1: more = rows_run<T, QX, OUT, 1>(a, walk, st, lds, tid); break;
+            case 2: more = rows_run<T, QX, OUT, 2>(a, walk, st, lds, tid); break;
+            case 3: more = rows_run<T, QX, OUT, 3>(a, walk, st, lds, tid); break;
+            default: more = rows_run<T, QX, OUT, 4>(a, walk, st, lds, tid); break;
         }
     }
 }
 
 // ------------------------------------------------------------------------------- gradient of the weights
 
+struct Place {
+    int group, begin, rows;  // of x and dy
+    int row0, col0;          // of the tile in dw[group]
+};
+
+// Walk over the tiles of all groups: [group, the longest first][8 column tiles][row tile][column tile].  The longest first, as
+// a tile's time is that of its group's rows (up to kThreads groups; thread i holds the rank of group i).
+struct WgradWalk {
+    int row_tiles, col_tiles, per, total, rank;
+
+    static __device__ __forceinline__ int end(const WgradArgs &a, int g) { return min(max(a.offsets[g], 0), a.rows); }
+    template <int FM>
+    __device__ __forceinline__ void setup(const WgradArgs &a, int tid, int *words) {
+        row_tiles = (a.out_rows + 64 * FM - 1) / (64 * FM);
+        col_tiles = (a.cols + kCols - 1) / kCols;
+        per = row_tiles * col_tiles;
+        total = per * a.n_groups;
+        rank = -1;
+        if (a.n_groups <= kThreads) {
+            const int mine = tid < a.n_groups ? end(a, tid) - (tid == 0 ? 0 : end(a, tid - 1)) : 0;
+            words[8 + tid] = mine;
+            ring::all_read();
+            rank = 0;
+            for (int g = 0; g < a.n_groups; ++g) {
+                const int v = words[8 + g];
+                rank += v > mine || (v == mine && g < tid) ? 1 : 0;
+            }
+            ring::all_read();  // the words may be written again
+        }
+    }
+    __device__ __forceinline__ void post(const WgradArgs &a, int t, int tid, int *words) const {
+        if (rank == t / per && tid < a.n_groups) words[0] = tid;
+    }
+    template <int FM>
+    __device__ __forceinline__ Place get(const WgradArgs &a, int t, const int *words) const {
+        Place p;
+        const int turn = t / per, local = t - turn * per, band = local / (row_tiles * kWalkCols);
+        const int width = min(kWalkCols, col_tiles - band * kWalkCols), rem = local - band * row_tiles * kWalkCols;
+        p.group = a.n_groups <= kThreads ? uniform(words[0]) : turn;
+        p.row0 = rem / width * (64 * FM);
+        p.col0 = (band * kWalkCols + rem % width) * kCols;
+        p.begin = uniform(p.group == 0 ? 0 : end(a, p.group - 1));
+        p.rows = uniform(max(end(a, p.group) - p.begin, 0));
+        return p;
+    }
+};
+
+template <class T, int FM>
+__device__ __forceinline__ void wgrad_feed(Feed<FM, true, true> &feed, const WgradArgs &a, const Place &p, int tid) {
+    feed.p.setup(tid, a.dy + p.begin * a.dy_pitch + p.row0 * T::kBytes, a.dy_pitch, min(64 * FM, a.out_rows - p.row0));
+    feed.q.setup(tid, a.x + p.begin * a.x_pitch + p.col0 * T::kBytes, a.x_pitch, min(kCols, a.cols - p.col0));
+    feed.set_length(p.rows, T::kBytes);
+    feed.set_ahead(tid, a.dy_pitch, min(64 * FM, a.out_rows - p.row0), a.x_pitch, min(kCols, a.cols - p.col0));
+}
+
+template <class T, int FM>
+struct WgradNext {
+    const WgradArgs &a;
+    const WgradWalk &walk;
+    int *words;
+    int tid, t;
+    Place place;  // the next one, behind take()
+
+    __device__ __forceinline__ void post() const {
+        if (t < walk.total) walk.post(a, t, tid, words);
+    }
+    __device__ __forceinline__ void pin() {}
+    __device__ __forceinline__ int take(Feed<FM, true, true> &feed) {
+        if (t >= walk.total) return 0;
+        place = walk.template get<FM>(a, t, words);
+        wgrad_feed<T>(feed, a, place, tid);
+        return 1;
+    }
+    __device__ __forceinline__ void other(int, uint32_t) const {}
+};
+
 template <class T, int FM>
 __global__ __launch_bounds__(kThreads, 1) void grouped_mm_wgrad_kernel(WgradArgs a) {
     __shared__ __attribute__((aligned(1024))) char lds[kLdsBytes];
     const int tid = threadIdx.x;
-    const int row_tiles = (a.out_rows + 64 * FM - 1) / (64 * FM), col_tiles = (a.cols + kCols - 1) / kCols;
-    const int per = row_tiles * col_tiles, total = per * a.n_groups;
-    struct Place {
-        int group, row0, col0;
-    };
-    auto place = [&](int t) {
-        Place p;
-        p.group = t / per;
-        const int local = t - p.group * per, band = local / (row_tiles * kWalkCols);
-        const int width = min(kWalkCols, col_tiles - band * kWalkCols), rem = local - band * row_tiles * kWalkCols;
-        p.row0 = rem / width * (64 * FM);
-        p.col0 = (band * kWalkCols + rem % width) * kCols;
-        return p;
-    };
-    auto set = [&](Feed<FM, true, true> &feed, const Place &p) {
-        const int begin = p.group == 0 ? 0 : min(max(a.offsets[p.group - 1], 0), a.rows);
-        const int end = max(min(max(a.offsets[p.group], 0), a.rows), begin);
-        feed.p.setup(tid, a.dy + begin * a.dy_pitch + p.row0 * T::kBytes, a.dy_pitch, min(64 * FM, a.out_rows - p.row0));
-        feed.q.setup(tid, a.x + begin * a.x_pitch + p.col0 * T::kBytes, a.x_pitch, min(kCols, a.cols - p.col0));
-        feed.set_length(uniform(end - begin), T::kBytes);
-        feed.set_ahead(tid, a.dy_pitch, min(64 * FM, a.out_rows - p.row0), a.x_pitch, min(kCols, a.cols - p.col0));
-    };
-    int i = 0, t = walk_place(0);
-    if (t >= total) return;
-    Place p = place(t);
+    int *words = reinterpret_cast<int *>(lds + kScratchOff);
+    int turn = 0;
+    if (walk_place(0) >= (a.out_rows + 64 * FM - 1) / (64 * FM) * ((a.cols + kCols - 1) / kCols) * a.n_groups) return;
+    WgradWalk walk;
+    walk.setup<FM>(a, tid, words);
+    walk.post(a, walk_place(0), tid, words);
+    ring::all_read();
+    Place p = walk.get<FM>(a, walk_place(0), words);
     Feed<FM, true, true> feed;
-    set(feed, p);
-    feed.start(tid, lds);
+    wgrad_feed<T>(feed, a, p, tid);
+    const uint32_t at = ring::lds_addr(lds) + uniform(tid >> 6) * 1024;
+    feed.issue_all(tid, at, 0);
+    feed.issue_all(tid, at + kStageStride, 1);
+    wait_copies<Geo<FM>::kCopies>();
+    uint32_t stage = 0;
     while (true) {
         typename T::Acc acc[4][FM] = {};
-        contract<T>(acc, feed, lds, tid);
+        WgradNext<T, FM> next{a, walk, words, tid, walk_place(++turn), Place()};
+        const int kind = contract<T>(acc, feed, lds, tid, stage, next);
         const int64_t pitch = (int64_t)a.cols * T::kBytes;
-        char *out = a.dw + ((int64_t)p.group * a.out_rows + p.row0) * pitch + (int64_t)p.col0 * T::kBytes;
-        const int live = a.out_rows - p.row0, cols = a.cols - p.col0;
-        t = walk_place(++i);
-        const bool more = t < total;
-        if (more) {
-            p = place(t);
-            set(feed, p);
-            feed.start(tid, lds);
-        }
-        store_tile<T, T, FM>(acc, Scales<T, FM>(), lds, out, pitch, live, cols, tid);
-        if (!more) return;
+        store_tile<T, T, FM>(acc, Scales<T, FM>(), lds, a.dw + ((int64_t)p.group * a.out_rows + p.row0) * pitch + (int64_t)p.col0 * T::kBytes,
+                             pitch, a.out_rows - p.row0, a.cols - p.col0, tid);
+        p = next.place;
+        if (kind == 0) return;
     }
 }
 

@@ -10,14 +10,14 @@
 // card's power limit every byte moved costs clock.  One wave per SIMD holds 256 accumulators (FM = 4) and two sets of
 // operand fragments; the next 16-wide step's fragments are read under the current step's matrix instructions.
 //
-// LDS: a ring of stages, each a slab of 128 bytes of contraction (64 elements of 16 bits, 128 of 8): the tile's P rows,
+// LDS: two stages, each a slab of 128 bytes of contraction (64 elements of 16 bits, 128 of 8): the tile's P rows,
 // then the 256 Q rows.  Along: rows of 128 B, chunk c (16 B) of row r in slot c ^ ((r >> 1) & 7).  Across (16-bit types
 // only): one row per k of 2 bytes per i, 32-byte group c of row k in slot c ^ 2 (k & 3), read through the transposing
 // LDS read: four k rows x 16 columns per 16 lanes, which the swizzle spreads over all banks.  The copies go straight to
 // LDS, 1 KB per wave instruction; the swizzle is applied to the lanes' addresses.
 //
 // One barrier per slab, in the last step, where the slab's last fragments are in registers: it certifies that the next
-// slab has landed and hands this slab's stage to the copies of the slab S behind it.
+// slab has landed and hands this slab's stage to the copies of the slab two behind it, which may be the next tile's.
 //
 // Ends: rows and columns outside the operand are read from its last one inside (they only reach outputs that are not
 // stored); contraction elements outside it come from a page of zeros, in both operands, so that nothing that lies there
@@ -65,16 +65,14 @@ struct I8 {  // sums in 32-bit integers: exact
     }
 };
 
+constexpr int kStageStride = 64 * 1024;  // of the tallest tile, so that tiles of different height follow each other in the ring
 template <int FM>
 struct Geo {
     static constexpr int kRows = 64 * FM;
     static constexpr int kPBytes = kRows * kSlab;
-    static constexpr int kStageBytes = kPBytes + kQBytes;
-    static constexpr int kFit = kScratchOff / kStageBytes;
-    static constexpr int kStages = kFit < 4 ? kFit : 4;
     static constexpr int kPPieces = kPBytes / 1024 / kWaves, kQPieces = kQBytes / 1024 / kWaves;  // copies per wave
     static constexpr int kCopies = kPPieces + kQPieces;
-    static_assert(kStages >= 2, "a stage to compute on and one to fill");
+    static_assert(kPBytes + kQBytes <= kStageStride && 2 * kStageStride <= kScratchOff, "two stages fit in front of the scratch");
 };
 
 // What lies behind the end of a contraction.
@@ -125,16 +123,13 @@ struct Operand {
         base = ring::uniform_ptr(src);
         step = ACROSS ? 64 * pitch : kSlab;
         const int wave = tid >> 6, lane = tid & 63, sub = lane / kLanes, slot = lane % kLanes;
+        const int row = wave * kPerPiece + sub;  // of the first piece; the swizzle is the same for all
+        const uint32_t first = (uint32_t)row * (uint32_t)pitch, next = (uint32_t)(kWaves * kPerPiece) * (uint32_t)pitch;
+        // (a slot holds chunk slot ^ 4 (row & 3): 2 (row & 3) in groups of two chunks)
+        const uint32_t last = ACROSS ? ~0u : (uint32_t)(live - 1) * (uint32_t)pitch;
+        const uint32_t chunk = ACROSS ? (uint32_t)min(slot ^ ((row & 3) << 2), live / 8 - 1) * 16u : (uint32_t)(slot ^ ((row >> 1) & 7)) * 16u;
 #pragma unroll
-        for (int i = 0; i < kPieces; ++i) {
-            const int row = (wave + kWaves * i) * kPerPiece + sub;
-            if constexpr (ACROSS) {
-                const int chunk = slot ^ ((row & 3) << 2);  // 2 (row & 3) in groups of two chunks
-                off[i] = (uint32_t)row * (uint32_t)pitch + (uint32_t)min(chunk, live / 8 - 1) * 16u;
-            } else {
-                off[i] = (uint32_t)min(row, live - 1) * (uint32_t)pitch + (uint32_t)(slot ^ ((row >> 1) & 7)) * 16u;
-            }
-        }
+        for (int i = 0; i < kPieces; ++i) off[i] = min(first + i * next, last) + chunk;
     }
     // Byte offset of line `i` of a slab (ROWS lines of 128 B).
     static __device__ __forceinline__ uint32_t line(int i, int64_t pitch, int live) {
@@ -181,8 +176,8 @@ struct Reader {
         if constexpr (ACROSS) {
             typedef __attribute__((address_space(3))) s16x4 *lds4;
             typedef short s16x8 __attribute__((ext_vector_type(8)));
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at[f] + j * 16 * (ROWS * 2)));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(at[f] + j * 16 * (ROWS * 2) + 4 * (ROWS * 2)));
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(at[f] + j * 16 * (ROWS * 2)));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(uintptr_t)(at[f] + j * 16 * (ROWS * 2) + 4 * (ROWS * 2)));
             return __builtin_bit_cast(i32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             typedef const __attribute__((address_space(3))) i32x4 *lds16;
@@ -202,7 +197,7 @@ struct Feed {
     using G = Geo<FM>;
     Operand<G::kRows, PX> p;
     Operand<kCols, QX> q;
-    int n_slabs, full;  // slabs, and how many of them are whole
+    int n_slabs, full;  // slabs (two at least: what is behind the end is zeros), and how many of them are whole
     int len_p, len_q;   // contraction in bytes (along) or elements (across)
     // Lines of a slab that this workgroup asks the L2 for, kAhead slabs in front of its copies: of the row tile that its eight
     // neighbours on the XCD share an eighth, of the column tile that four share a quarter, 24 lines per wave.  (The barrier
@@ -217,7 +212,7 @@ struct Feed {
         ahead = is_p ? p.base + Operand<G::kRows, PX>::line((slot & 7) * 8 * FM + wave * 2 * FM + min(lane, 2 * FM - 1), p_pitch, p_live)
                      : q.base + Operand<kCols, QX>::line(((slot >> 3) & 3) * 64 + wave * 16 + lane - 8, q_pitch, q_live);
         ahead_step = is_p ? p.step : q.step;
-        ahead_slab = min(G::kStages + kAhead, full - 1);
+        ahead_slab = min(2 + kAhead, full - 1);
         ahead += ahead_slab * ahead_step;
         if (full == 0) ahead = reinterpret_cast<const char *>(&g_zeros);
     }
@@ -230,7 +225,7 @@ struct Feed {
         len_p = PX ? elements : elements * bytes_per;
         len_q = QX ? elements : elements * bytes_per;
         full = elements * bytes_per / kSlab;
-        n_slabs = (elements * bytes_per + kSlab - 1) / kSlab;
+        n_slabs = max((elements * bytes_per + kSlab - 1) / kSlab, 2);
     }
     // `at`: the wave's first piece in the stage.
     template <int C>
@@ -247,43 +242,35 @@ struct Feed {
             unrolled<G::kPPieces>([&](auto c) { p.template issue_end<c.value, 0>(tid, p_slab, at, len_p - slab * (PX ? 64 : kSlab)); });
         }
     }
-    // The first slabs, up to all stages.
-    __device__ __forceinline__ void start(int tid, const char *lds) {
-        const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), at = ring::lds_addr(lds);
-#pragma unroll 1
-        for (int s = 0; s < min(G::kStages, n_slabs); ++s) {
-            issue_all(tid, at + s * G::kStageBytes + wave * 1024, s);
-        }
-    }
 };
 
-// Waits until at most `slabs` (wave-uniform, <= 2) slabs of copies are in flight and this wave's LDS reads have returned, then joins
-// the barrier.
-template <int COPIES>
-__device__ __forceinline__ void landed(int slabs) {
-    if (slabs <= 0) ring::wait_and_barrier<0>();
-    else if (slabs == 1) ring::wait_and_barrier<COPIES>();
-    else ring::wait_and_barrier<2 * COPIES>();
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
-// The contraction of one tile whose first slabs are on their way (Feed::start).  acc[f][t]: column fragment 4 wn + f
-// against row fragment FM wm + t.  Every wave is past the reads of the last slab when one returns (n_slabs > 0): the stages
-// may be filled again.
-template <class T, int FM, bool PX, bool QX>
-__device__ __forceinline__ void contract(typename T::Acc (&acc)[4][FM], Feed<FM, PX, QX> &feed, const char *lds, int tid) {
+// The contraction of one tile.  acc[f][t]: column fragment 4 wn + f against row fragment FM wm + t.  The copies run through
+// from tile to tile: slab k is in stage (stage + k) % 2, slabs 0 and 1 are on their way (slab 0 of this wave has landed) when a
+// tile begins, and while its last two slabs are computed, the first two of the next tile follow them into the ring.
+//   next.post()          behind the first barrier: looks for the next tile
+//   next.pin()           before the first slab but one is waited for: loads of the caller's have landed
+//   next.take(feed)      behind a later barrier, when the last copy of this tile is out: 0: there is none; 1: one of the same
+//                        height, which `feed` is now; 2: one of another, which next.other(slab, at) copies
+// Returns what take() did.  Every wave is past the last slab's reads when one returns: the scratch may be used.
+template <class T, int FM, bool PX, bool QX, class Next>
+__device__ __forceinline__ int contract(typename T::Acc (&acc)[4][FM], Feed<FM, PX, QX> &feed, const char *lds, int tid, uint32_t &stage,
+                                        Next &next) {
     using G = Geo<FM>;
-    constexpr int S = G::kStages, READS = 4 + FM, MM = 4 * FM;
+    constexpr int READS = 4 + FM, MM = 4 * FM;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), base = ring::lds_addr(lds);
+    const uint32_t sink = base + kScratchOff + wave * kScratchBytes + kScratchBytes - 256;
     const int lane = tid & 63, n = feed.n_slabs;
-    if (n == 0) {
-        ring::wait_and_barrier<0>();
-        return;
-    }
     Reader<G::kRows, PX> rp;
     Reader<kCols, QX> rq;
-    rp.setup(lane, (wave >> 1) * FM, base);
-    rq.setup(lane, (wave & 1) * 4, base + G::kPBytes);
-    landed<G::kCopies>(min(S, n) - 1);
+    rp.setup(lane, (wave >> 1) * FM, base + stage * kStageStride);
+    rq.setup(lane, (wave & 1) * 4, base + stage * kStageStride + G::kPBytes);
+    ring::all_read();  // every wave's share of slab 0 has landed; the scratch is free
+    next.post();
 
     i32x4 a[2][4], b[2][FM];
     auto read = [&](int r, int set, int j) {
@@ -293,13 +280,13 @@ __device__ __forceinline__ void contract(typename T::Acc (&acc)[4][FM], Feed<FM,
 #pragma unroll
     for (int r = 0; r < READS; ++r) read(r, 0, 0);
 
-    // Where the next copies go: the wave's first piece in the stage of slab k, and slab k + S of the operands.
-    uint32_t into = base + wave * 1024;
-    const char *p_slab = feed.p.base + S * feed.p.step, *q_slab = feed.q.base + S * feed.q.step;
-    uint32_t stage = 0, by = 0;  // of slab k; to the next one
+    // Where the next copies go: the wave's first piece in the stage of slab k, and slab k + 2 of the operands.
+    uint32_t into = base + stage * kStageStride + wave * 1024;
+    const char *p_slab = feed.p.base + 2 * feed.p.step, *q_slab = feed.q.base + 2 * feed.q.step;
+    uint32_t by = 0;
     // Step J of a slab: its matrix instructions, the reads of the next step's fragments behind the first half of them, and
-    // copies FROM .. TO - 1 of a slab spread over all of them.  `more(m)` runs behind instruction m.
-    auto step = [&](auto J, auto read_next, auto from, auto to, auto more) {
+    // copies FROM .. TO - 1 of a slab spread over all of them, if `go`.  `more(m)` runs behind instruction m.
+    auto step = [&](auto J, auto read_next, auto from, auto to, bool go, auto more) {
         constexpr int j = J.value, set = j & 1, FROM = from.value, COUNT = to.value - from.value;
         unrolled<MM>([&](auto M) {
             constexpr int m = M.value, t = m >> 2, f = m & 3;
@@ -310,7 +297,9 @@ __device__ __forceinline__ void contract(typename T::Acc (&acc)[4][FM], Feed<FM,
                     if (r * MM / (2 * READS) == m) read(r, set ^ 1, (j + 1) & 3);
             }
             unrolled<COUNT>([&](auto c) {
-                if constexpr ((c.value * MM + MM / 2) / COUNT == m) feed.template issue<FROM + c.value>(into, p_slab, q_slab);
+                if constexpr ((c.value * MM + MM / 2) / COUNT == m) {
+                    if (go) feed.template issue<FROM + c.value>(into, p_slab, q_slab);
+                }
             });
             more(M);
             PMOE_GMM_FENCE();
@@ -322,58 +311,77 @@ __device__ __forceinline__ void contract(typename T::Acc (&acc)[4][FM], Feed<FM,
     // Copies are spread over two steps: in one, the four waves ask the address path of the CU for more than it takes (16 cycles
     // a copy) and stand still; in three, the last ones have too little time to land.
     constexpr int C1 = G::kCopies / 2, C2 = G::kCopies;
-
     auto nothing = [](auto) {};
-    // The readers on to the next stage, among the last instructions of step 2, whose reads are the stage's last.
+    // The readers on to the other stage, among the last instructions of step 2, whose reads are the stage's last.
     auto move = [&](auto M) {
         constexpr int m = M.value;
         if constexpr (m == MM / 2) {
-            by = stage + 1 == S ? 0u - (S - 1) * G::kStageBytes : G::kStageBytes;
-            stage = stage + 1 == S ? 0 : stage + 1;
+            by = stage == 0 ? kStageStride : 0u - kStageStride;
+            stage ^= 1;
         } else if constexpr (m > MM / 2) {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (MM / 2 + 1 + i * (MM / 2 - 1) / 8 == m) (i < 4 ? rp.at[i & 3] : rq.at[i & 3]) += by;
         }
     };
-    // The slabs of the loops begin with step 3 of slab k and end with step 2 of slab k + 1.  No branch stands between matrix
-    // instructions: with them in branches the compiler keeps a second set of accumulators and spills.
-    step(PMOE_INT(0), Yes(), PMOE_INT(0), PMOE_INT(0), nothing);
-    step(PMOE_INT(1), Yes(), PMOE_INT(0), PMOE_INT(0), nothing);
-    step(PMOE_INT(2), Yes(), PMOE_INT(0), PMOE_INT(0), move);
+    // The slabs of the loops begin with step 3 of slab k and end with step 2 of slab k + 1.  Matrix instructions stand in no
+    // branch: with them in branches the compiler keeps a second set of accumulators and spills.
+    step(PMOE_INT(0), Yes(), PMOE_INT(0), PMOE_INT(0), false, nothing);
+    step(PMOE_INT(1), Yes(), PMOE_INT(0), PMOE_INT(0), false, nothing);
+    step(PMOE_INT(2), Yes(), PMOE_INT(0), PMOE_INT(0), false, move);
+    wait_copies<0>();
+    next.pin();
     int k = 0;
-    for (; k + S < feed.full; ++k) {
-        // slab k + 1 has landed; behind it are the line asked for ahead and the slabs up to k + S - 1 (the first S slabs
-        // have no line behind them)
-        if (k >= S) ring::wait_and_barrier<1 + (S - 2) * (G::kCopies + 1)>();
-        else ring::wait_and_barrier<(S - 2) * G::kCopies>();
+    for (; k + 2 < feed.full; ++k) {
+        ring::wait_and_barrier<1>();  // slab k + 1 has landed (behind it is the line asked for ahead)
         PMOE_GMM_FENCE();
-        step(PMOE_INT(3), Yes(), PMOE_INT(0), PMOE_INT(C1), nothing);
-        step(PMOE_INT(0), Yes(), PMOE_INT(C1), PMOE_INT(C2), nothing);
-        step(PMOE_INT(1), Yes(), PMOE_INT(0), PMOE_INT(0), [&](auto M) {  // (no copy of the slab may follow)
-            if constexpr (M.value == MM / 2) feed.ask_ahead(base + kScratchOff + wave * kScratchBytes);
+        step(PMOE_INT(3), Yes(), PMOE_INT(0), PMOE_INT(C1), true, nothing);
+        step(PMOE_INT(0), Yes(), PMOE_INT(C1), PMOE_INT(C2), true, nothing);
+        step(PMOE_INT(1), Yes(), PMOE_INT(0), PMOE_INT(0), false, [&](auto M) {  // (no copy of the slab may follow)
+            if constexpr (M.value == MM / 2) feed.ask_ahead(sink);
             if constexpr (M.value == MM / 2 + 1) {
                 p_slab += feed.p.step;
                 q_slab += feed.q.step;
-                into = base + wave * 1024 + stage * G::kStageBytes;
+                into = base + stage * kStageStride + wave * 1024;
             }
         });
-        step(PMOE_INT(2), Yes(), PMOE_INT(0), PMOE_INT(0), move);
+        step(PMOE_INT(2), Yes(), PMOE_INT(0), PMOE_INT(0), false, move);
     }
+    int kind = 0;
     for (; k + 1 < n; ++k) {
-        landed<G::kCopies>(min(S - 2, n - 2 - k));
-        if (k + S < n) feed.issue_all(tid, into, k + S);
-        into = base + wave * 1024 + stage * G::kStageBytes;
+        ring::wait_and_barrier<0>();
+        bool go = false;
+        if (k + 2 < n) {
+            feed.issue_all(tid, into, k + 2);  // the slab with the end, or behind it
+        } else {
+            kind = next.take(feed);
+            go = kind == 1 && feed.full >= 1;
+            if (kind == 1 && !go) feed.issue_all(tid, into, 0);
+            if (kind == 2) next.other(0, into);
+            p_slab = feed.p.base;
+            q_slab = feed.q.base;
+        }
         PMOE_GMM_FENCE();
-        step(PMOE_INT(3), Yes(), PMOE_INT(0), PMOE_INT(0), nothing);
-        step(PMOE_INT(0), Yes(), PMOE_INT(0), PMOE_INT(0), nothing);
-        step(PMOE_INT(1), Yes(), PMOE_INT(0), PMOE_INT(0), nothing);
-        step(PMOE_INT(2), Yes(), PMOE_INT(0), PMOE_INT(0), move);
+        step(PMOE_INT(3), Yes(), PMOE_INT(0), PMOE_INT(C1), go, nothing);
+        step(PMOE_INT(0), Yes(), PMOE_INT(C1), PMOE_INT(C2), go, nothing);
+        step(PMOE_INT(1), Yes(), PMOE_INT(0), PMOE_INT(0), false, nothing);
+        into = base + stage * kStageStride + wave * 1024;
+        step(PMOE_INT(2), Yes(), PMOE_INT(0), PMOE_INT(0), false, move);
     }
-    ring::wait_and_barrier<0>();
+    ring::all_read();
+    const bool go = kind == 1 && feed.full >= 2;
+    if (kind == 1 && !go) feed.issue_all(tid, into, 1);
+    if (kind == 2) next.other(1, into);
+    p_slab = feed.p.base + feed.p.step;
+    q_slab = feed.q.base + feed.q.step;
     PMOE_GMM_FENCE();
-    step(PMOE_INT(3), No(), PMOE_INT(0), PMOE_INT(0), nothing);
+    step(PMOE_INT(3), No(), PMOE_INT(0), PMOE_INT(C2), go, nothing);
 #undef PMOE_INT
+    stage ^= 1;  // slab 0 of the next tile took the place of the last slab but one
+    // it has landed once at most the copies of its slab 1 are under way (10 in the lowest tile)
+    if (kind == 1) wait_copies<G::kCopies>();
+    else wait_copies<Geo<1>::kCopies>();
+    return kind;
 }
 
 }  // namespace gmm
