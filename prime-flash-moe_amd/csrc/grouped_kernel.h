@@ -247,41 +247,64 @@ struct Scales<I8, FM> {
 
 // A tile's way out: 32 rows x 256 B (8-bit products: 128 B) at a time through the wave's scratch, chunk c of row r in slot
 // c ^ r (modulo the chunks of a row), and from there in whole rows.  `out`: the tile's first element.  `live`, `cols`: rows and
-// columns to store.
+// columns to store.  A part is read back while the next one is converted and written behind it (the LDS serves a wave in order),
+// and stored behind that.
 template <class T, class OUT, int FM>
 __device__ __forceinline__ void store_tile(const typename T::Acc (&acc)[4][FM], const Scales<T, FM> &scales, char *lds, char *out,
                                            int64_t pitch, int live, int cols, int tid) {
     using P = Pack<OUT>;
-    constexpr int ROW = Scales<T, FM>::kRowBytes, CHUNKS = ROW / 16;
+    constexpr int ROW = Scales<T, FM>::kRowBytes, CHUNKS = ROW / 16, PER_READ = 64 / CHUNKS, READS = 32 / PER_READ;
     constexpr int FRAGS = ROW / (32 * P::kBytes);  // column fragments that go through at a time
-    constexpr int PER = 16 / P::kBytes;            // columns of a chunk
+    constexpr int PARTS = FM * 4 / FRAGS;
     const int wave = uniform(tid >> 6), lane = tid & 63;
     char *scratch = lds + kScratchOff + wave * kScratchBytes;
     const int r = lane & 31, half = lane >> 5, sx = r % CHUNKS;
+    const int sub = lane / CHUNKS, chunk = lane % CHUNKS;
+    // rows and columns of the wave's part of the tile, from its own first ones
+    const int first_row = (wave >> 1) * FM * 32, first_col = (wave & 1) * 128;
+    out += first_row * pitch + first_col * P::kBytes;
+    live -= first_row;
+    cols -= first_col;
+    const uint32_t lane_off = (uint32_t)sub * (uint32_t)pitch + chunk * 16;
+    const bool whole = live >= 32 * FM && cols >= 128;
+    auto put = [&](auto part) {
+        constexpr int t = part.value / (4 / FRAGS), h = part.value % (4 / FRAGS);
 #pragma unroll
-    for (int t = 0; t < FM; ++t)
+        for (int f = 0; f < FRAGS; ++f)
 #pragma unroll
-        for (int h = 0; h < 4 / FRAGS; ++h) {
-#pragma unroll
-            for (int f = 0; f < FRAGS; ++f)
-#pragma unroll
-                for (int i4 = 0; i4 < 4; ++i4) {
-                    const float4 v = scales.apply(acc[h * FRAGS + f][t], h * FRAGS + f, t, i4, scratch, half);
-                    if constexpr (P::kBytes == 2)
-                        *reinterpret_cast<uint2 *>(scratch + r * ROW + (((4 * f + i4) ^ sx) << 4) + half * 8) = P::four(v.x, v.y, v.z, v.w);
-                    else
-                        *reinterpret_cast<uint4 *>(scratch + r * ROW + (((8 * f + 2 * i4 + half) ^ sx) << 4)) = P::four(v.x, v.y, v.z, v.w);
-                }
-            __builtin_amdgcn_wave_barrier();
-            const int chunk = lane % CHUNKS, col = ((wave & 1) * 4 + h * FRAGS) * 32 + chunk * PER;
-#pragma unroll
-            for (int it = 0; it < CHUNKS / 2; ++it) {
-                const int row = it * (64 / CHUNKS) + lane / CHUNKS, at = ((wave >> 1) * FM + t) * 32 + row;
-                const uint4 v = *reinterpret_cast<const uint4 *>(scratch + row * ROW + ((chunk ^ (row % CHUNKS)) << 4));
-                if (at < live && col < cols) *reinterpret_cast<uint4 *>(out + at * pitch + col * P::kBytes) = v;
+            for (int i4 = 0; i4 < 4; ++i4) {
+                const float4 v = scales.apply(acc[h * FRAGS + f][t], h * FRAGS + f, t, i4, scratch, half);
+                if constexpr (P::kBytes == 2)
+                    *reinterpret_cast<uint2 *>(scratch + r * ROW + (((4 * f + i4) ^ sx) << 4) + half * 8) = P::four(v.x, v.y, v.z, v.w);
+                else
+                    *reinterpret_cast<uint4 *>(scratch + r * ROW + (((8 * f + 2 * i4 + half) ^ sx) << 4)) = P::four(v.x, v.y, v.z, v.w);
             }
-            __builtin_amdgcn_wave_barrier();
+    };
+    put(std::integral_constant<int, 0>());
+    unrolled<PARTS>([&](auto part) {
+        constexpr int t = part.value / (4 / FRAGS), h = part.value % (4 / FRAGS);
+        i32x4 v[READS];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int it = 0; it < READS; ++it) {
+            const int row = it * PER_READ + sub;
+            v[it] = *reinterpret_cast<const i32x4 *>(scratch + row * ROW + ((chunk ^ (row % CHUNKS)) << 4));
         }
+        __builtin_amdgcn_wave_barrier();
+        if constexpr (part.value + 1 < PARTS) put(std::integral_constant<int, part.value + 1>());
+        PMOE_GMM_FENCE();
+        char *to = out + t * 32 * pitch + h * ROW;  // wave-uniform
+        if (whole) {
+#pragma unroll
+            for (int it = 0; it < READS; ++it) *reinterpret_cast<i32x4 *>(to + it * PER_READ * pitch + lane_off) = v[it];
+        } else {
+            const int rows = h * (ROW / P::kBytes) + chunk * (16 / P::kBytes) < cols ? live - t * 32 - sub : 0;
+#pragma unroll
+            for (int it = 0; it < READS; ++it)
+                if (it * PER_READ < rows) *reinterpret_cast<i32x4 *>(to + it * PER_READ * pitch + lane_off) = v[it];
+        }
+        PMOE_GMM_FENCE();
+    });
 }
 
 // ------------------------------------------------------------------------------- rows by their expert's weights
@@ -345,7 +368,7 @@ __device__ __forceinline__ bool rows_run(const RowsArgs &a, const Walk &walk, Ro
     rows_feed<T>(feed, a, st.tile, tid);
     char *scratch = lds + kScratchOff + uniform(tid >> 6) * kScratchBytes;
     while (true) {
-        typename T::Acc acc[4][FM] = {};
+        typename T::Acc acc[4][FM];
         Scales<T, FM> scales;
         scales.load(a, st.tile, tid);
         RowsNext<T, QX, OUT, FM> next{a, walk, scales, reinterpret_cast<int *>(lds + kScratchOff), tid, walk_place(++st.turn), Tile()};
@@ -483,7 +506,7 @@ __global__ __launch_bounds__(kThreads, 1) void grouped_mm_wgrad_kernel(WgradArgs
     wait_copies<Geo<FM>::kCopies>();
     uint32_t stage = 0;
     while (true) {
-        typename T::Acc acc[4][FM] = {};
+        typename T::Acc acc[4][FM];
         WgradNext<T, FM> next{a, walk, words, tid, walk_place(++turn), Place()};
         const int kind = contract<T>(acc, feed, lds, tid, stage, next);
         const int64_t pitch = (int64_t)a.cols * T::kBytes;

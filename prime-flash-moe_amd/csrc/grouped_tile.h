@@ -270,7 +270,6 @@ __device__ __forceinline__ int contract(typename T::Acc (&acc)[4][FM], Feed<FM, 
     rp.setup(lane, (wave >> 1) * FM, base + stage * kStageStride);
     rq.setup(lane, (wave & 1) * 4, base + stage * kStageStride + G::kPBytes);
     ring::all_read();  // every wave's share of slab 0 has landed; the scratch is free
-    next.post();
 
     i32x4 a[2][4], b[2][FM];
     auto read = [&](int r, int set, int j) {
@@ -279,18 +278,20 @@ __device__ __forceinline__ int contract(typename T::Acc (&acc)[4][FM], Feed<FM, 
     };
 #pragma unroll
     for (int r = 0; r < READS; ++r) read(r, 0, 0);
+    next.post();
 
     // Where the next copies go: the wave's first piece in the stage of slab k, and slab k + 2 of the operands.
     uint32_t into = base + stage * kStageStride + wave * 1024;
     const char *p_slab = feed.p.base + 2 * feed.p.step, *q_slab = feed.q.base + 2 * feed.q.step;
     uint32_t by = 0;
     // Step J of a slab: its matrix instructions, the reads of the next step's fragments behind the first half of them, and
-    // copies FROM .. TO - 1 of a slab spread over all of them, if `go`.  `more(m)` runs behind instruction m.
+    // copies FROM .. TO - 1 of a slab spread over all of them, if `go`.  `more(m)` runs behind instruction m.  J == 4: step 0 of
+    // the first slab, where the sums begin.
     auto step = [&](auto J, auto read_next, auto from, auto to, bool go, auto more) {
-        constexpr int j = J.value, set = j & 1, FROM = from.value, COUNT = to.value - from.value;
+        constexpr int j = J.value % 4, set = j & 1, FROM = from.value, COUNT = to.value - from.value;
         unrolled<MM>([&](auto M) {
             constexpr int m = M.value, t = m >> 2, f = m & 3;
-            acc[f][t] = T::mfma(a[set][f], b[set][t], acc[f][t]);
+            acc[f][t] = T::mfma(a[set][f], b[set][t], J.value == 4 ? typename T::Acc{} : acc[f][t]);
             if constexpr (read_next.value) {
 #pragma unroll
                 for (int r = 0; r < READS; ++r)
@@ -326,7 +327,7 @@ __device__ __forceinline__ int contract(typename T::Acc (&acc)[4][FM], Feed<FM, 
     };
     // The slabs of the loops begin with step 3 of slab k and end with step 2 of slab k + 1.  Matrix instructions stand in no
     // branch: with them in branches the compiler keeps a second set of accumulators and spills.
-    step(PMOE_INT(0), Yes(), PMOE_INT(0), PMOE_INT(0), false, nothing);
+    step(PMOE_INT(4), Yes(), PMOE_INT(0), PMOE_INT(0), false, nothing);
     step(PMOE_INT(1), Yes(), PMOE_INT(0), PMOE_INT(0), false, nothing);
     step(PMOE_INT(2), Yes(), PMOE_INT(0), PMOE_INT(0), false, move);
     wait_copies<0>();
