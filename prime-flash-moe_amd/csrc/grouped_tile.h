@@ -378,8 +378,8 @@ __device__ __forceinline__ int contract(typename T::Acc (&acc)[4][FM], Feed<FM, 
     PMOE_GMM_FENCE();
     step(PMOE_INT(3), No(), PMOE_INT(0), PMOE_INT(C2), go, nothing);
 #undef PMOE_INT
-    stage ^= 1;  // slab 0 of the next tile took the place of the last slab but one
-    // it has landed once at most the copies of its slab 1 are under way (10 in the lowest tile)
+    // Slab 0 of the next tile took the place of the last slab but one, which `stage` is back at.  It has landed once at most
+    // the copies of its slab 1 are under way (10 in the lowest tile).
     if (kind == 1) wait_copies<G::kCopies>();
     else wait_copies<Geo<1>::kCopies>();
     return kind;

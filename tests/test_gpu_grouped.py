@@ -10,6 +10,16 @@ pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float16]
 
 
+@pytest.fixture(params=[0, 8], ids=["whole device", "8 CUs"])
+def cus(request):
+    """Launches sized for the device, and for one of eight CUs: small cases then take the kernels of large ones, and many tiles
+    follow each other in a workgroup."""
+    from prime_moe import _native
+    _native.load().pmoe_set_compute_units(request.param)
+    yield request.param
+    _native.load().pmoe_set_compute_units(0)
+
+
 def make(shape, gen, dtype, device, std=1.0):
     return (torch.randn(shape, generator=gen) * std).to(dtype).to(device)
 
@@ -28,13 +38,15 @@ RAGGED = [
     ([513, 1], 1),
     ([0, 0], 5),
     ([700], 0),
+    ([17, 0, 15, 16, 48], 3),
+    ([2, 1, 1, 0, 5, 3], 0),
 ]
 
 
 @pytest.mark.parametrize("counts,behind", RAGGED)
 @pytest.mark.parametrize("N,K", [(8, 8), (24, 64), (256, 128), (264, 72), (520, 1000), (128, 136)])
 @pytest.mark.parametrize("across", [False, True])
-def test_forward(device, counts, behind, N, K, across):
+def test_forward(device, cus, counts, behind, N, K, across):
     import prime_moe
     gen = torch.Generator().manual_seed(N * 1000 + K + len(counts))
     ends = np.cumsum(counts).tolist()
@@ -51,7 +63,7 @@ def test_forward(device, counts, behind, N, K, across):
 
 @pytest.mark.parametrize("counts,behind", RAGGED)
 @pytest.mark.parametrize("N,K", [(8, 8), (24, 64), (256, 128), (264, 72), (520, 1000), (1032, 264)])
-def test_weight_gradient(device, counts, behind, N, K):
+def test_weight_gradient(device, cus, counts, behind, N, K):
     import prime_moe
     gen = torch.Generator().manual_seed(N * 1000 + K + len(counts))
     ends = np.cumsum(counts).tolist()
@@ -67,7 +79,7 @@ def test_weight_gradient(device, counts, behind, N, K):
 
 
 @pytest.mark.parametrize("E,total", [(1, 5), (7, 100), (64, 4000), (257, 300), (1000, 2500), (1024, 1024)])
-def test_many_groups(device, E, total):
+def test_many_groups(device, cus, E, total):
     import prime_moe
     gen = torch.Generator().manual_seed(E)
     ends = R.sized(total, E, gen)
@@ -90,7 +102,7 @@ def test_no_rows(device):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_what_lies_next_to_the_operands_does_not_count(device, dtype):
+def test_what_lies_next_to_the_operands_does_not_count(device, cus, dtype):
     """NaNs between the rows of strided operands, in rows behind the last group and in the rows of other groups."""
     import prime_moe
     gen = torch.Generator().manual_seed(5)
@@ -192,7 +204,7 @@ def test_gradients_of_gradients(device):
         assert ((g.double() - ref).abs() <= bound).all()
 
 
-def test_sums_are_held_in_32_bits(device):
+def test_sums_are_held_in_32_bits(device, cus):
     """A long contraction of small terms onto a large one: sums in 16 bits would lose them."""
     import prime_moe
     K = 16384
@@ -207,7 +219,7 @@ def test_sums_are_held_in_32_bits(device):
 
 
 @pytest.mark.parametrize("what", ["x", "out", "dy"])
-def test_beyond_32_bit_offsets(device, what):
+def test_beyond_32_bit_offsets(device, cus, what):
     """Operands and outputs above 4 GiB: rows near both ends."""
     import prime_moe
     gen = torch.Generator(device=device).manual_seed(8)
@@ -241,7 +253,7 @@ def test_beyond_32_bit_offsets(device, what):
         R.check(y[r:r + 1], ref, mags, K)
 
 
-def test_offsets_out_of_order_do_no_harm(device):
+def test_offsets_out_of_order_do_no_harm(device, cus):
     """Offsets that are not ends of groups: every access stays inside the arguments (rows come out as something)."""
     import prime_moe
     gen = torch.Generator().manual_seed(9)
@@ -253,7 +265,7 @@ def test_offsets_out_of_order_do_no_harm(device):
         assert y.shape == (100, 40) and dw.shape == (4, 40, 64)
 
 
-def test_same_bits_again_and_on_poisoned_lds(device):
+def test_same_bits_again_and_on_poisoned_lds(device, cus):
     import prime_moe
     from prime_moe import _native
     gen = torch.Generator().manual_seed(10)
@@ -303,7 +315,7 @@ def test_captured_training_step(device):
             assert torch.equal(got, want)
 
 
-def test_two_streams_at_once(device):
+def test_two_streams_at_once(device, cus):
     import prime_moe
     gen = torch.Generator().manual_seed(12)
     ends = R.sized(3000, 5, gen)

@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import grouped_ref as R
+from test_gpu_grouped import cus  # noqa: F401 (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -23,7 +24,7 @@ def check(got, ref):
 
 @pytest.mark.parametrize("counts,behind", [([1], 0), ([0, 3, 0], 0), ([63, 64, 65, 1, 0, 2], 7), ([255, 256, 257], 0), ([130, 31], 300), ([0], 4), ([700], 0)])
 @pytest.mark.parametrize("N,K", [(8, 16), (24, 128), (256, 256), (264, 144), (520, 1008)])
-def test_grouped(device, counts, behind, N, K):
+def test_grouped(device, cus, counts, behind, N, K):
     import prime_moe
     gen = torch.Generator().manual_seed(N + K + len(counts))
     ends = np.cumsum(counts).tolist()
@@ -41,7 +42,7 @@ def test_grouped(device, counts, behind, N, K):
 
 @pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 33, 64, 65, 127, 255, 256, 300, 1025])
 @pytest.mark.parametrize("N,K", [(8, 16), (136, 400), (512, 2048)])
-def test_dense(device, M, N, K):
+def test_dense(device, cus, M, N, K):
     import prime_moe
     gen = torch.Generator().manual_seed(M)
     x, w = ints((M, K), gen, device), ints((N, K), gen, device)
@@ -51,7 +52,7 @@ def test_dense(device, M, N, K):
         check(prime_moe.grouped_mm_int8(x, w, xs, ws, out_dtype=dtype), ref)
 
 
-def test_sums_are_exact(device):
+def test_sums_are_exact(device, cus):
     """The largest sums there are, and sums that an accumulator of 24 bits would round."""
     import prime_moe
     one = lambda n: torch.ones((n,), device=device)
@@ -74,7 +75,7 @@ def test_sums_are_exact(device):
     assert (y == float(1024 * 16129 + 1 - 1023 * 16129)).all()
 
 
-def test_strides_and_empty(device):
+def test_strides_and_empty(device, cus):
     import prime_moe
     gen = torch.Generator().manual_seed(3)
     x, w = ints((70, 256), gen, device)[:, 16:-48], ints((3, 40, 320), gen, device)[:, :, 32:224]
@@ -89,7 +90,7 @@ def test_strides_and_empty(device):
     assert torch.isnan(y[5]).all() and torch.isfinite(y[:5]).all() and torch.isfinite(y[6:]).all() and (y[66:] == 0).all()
 
 
-def test_weights_beyond_32_bit_offsets(device):
+def test_weights_beyond_32_bit_offsets(device, cus):
     import prime_moe
     gen = torch.Generator(device=device).manual_seed(4)
     E, N, K = 5, 32768, 32768
