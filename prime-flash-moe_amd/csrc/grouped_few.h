@@ -12,6 +12,8 @@
 // stage are 8 chunks of 16 B, chunk c of row r in slot c ^ (r / 2) % 8: the reads of 16 rows cover all banks once.  The waves'
 // sums meet in LDS and are added in wave order.
 #pragma once
+#include <algorithm>
+
 #include "grouped_kernel.h"
 
 namespace pmoe {
@@ -47,12 +49,19 @@ struct Span {
     bool zero;  // rows behind the last group
 };
 
-// The `slot`-th group that has rows; behind those, the rows behind the last group; begin == end: neither.  A wave at a time,
-// lane l looks at groups c l .. c l + c - 1.  As Walk: a group begins at the furthest end in front of it.
+// The `slot`-th block of up to BLOCK rows of a group (0: all of them); behind those, the rows behind the last group; begin ==
+// end: neither.  A wave at a time, lane l looks at groups c l .. c l + c - 1.  As Walk: a group begins at the furthest end in
+// front of it.
+template <int BLOCK>
+__device__ __forceinline__ int blocks_of(int rows) {
+    return BLOCK > 0 ? (rows + BLOCK - 1) / max(BLOCK, 1) : rows > 0;
+}
+template <int BLOCK>
 __device__ __forceinline__ Span find_span(const RowsArgs &a, int slot) {
     Span s = {0, 0, a.rows, false};
     if (a.offsets == nullptr) {
-        if (slot != 0) s.end = 0;
+        if (BLOCK > 0) s.begin = min(slot * BLOCK, a.rows), s.end = min(s.begin + BLOCK, a.rows);
+        else if (slot != 0) s.end = 0;
         return s;
     }
     const int lane = threadIdx.x & 63, c = (a.n_groups + 63) / 64, g0 = c * lane;
@@ -67,7 +76,7 @@ __device__ __forceinline__ Span find_span(const RowsArgs &a, int slot) {
     int count = 0, begin = first;
     for (int i = 0; i < c; ++i) {
         const int end = g0 + i < a.n_groups ? max(group_end(a, g0 + i), begin) : begin;
-        count += end > begin;
+        count += blocks_of<BLOCK>(end - begin);
         begin = end;
     }
     int incl = count;
@@ -88,7 +97,12 @@ __device__ __forceinline__ Span find_span(const RowsArgs &a, int slot) {
             begin = first;
             for (int i = 0; i < c; ++i) {
                 const int end = g0 + i < a.n_groups ? max(group_end(a, g0 + i), begin) : begin;
-                if (end > begin && left-- == 0) s = {g0 + i, begin, end, false};
+                const int blocks = blocks_of<BLOCK>(end - begin);
+                if (left >= 0 && left < blocks) {
+                    const int from = BLOCK > 0 ? begin + left * BLOCK : begin;
+                    s = {g0 + i, from, BLOCK > 0 ? min(from + BLOCK, end) : end, false};
+                }
+                left -= blocks;
                 begin = end;
             }
         }
@@ -119,18 +133,19 @@ __device__ __forceinline__ void wait_copies(int n) {
 constexpr int kMaxStages = 4;
 constexpr int kCH = 128;          // bytes of a row that a wave copies at a time
 constexpr int kRing = 10 * 1024;  // of a wave: sixteen waves per CU
+constexpr int kBlockRing = 20 * 1024, kBlock = 64;  // blocks of 64 rows: eight waves per CU
 
 // LDS of a workgroup: a ring per wave; the waves' sums lie where their own rings were.
-template <int U, int WAVES>
+template <int U, int WAVES, int RING>
 struct Shared {
-    char ring[WAVES][kRing];
-    static_assert(kRing >= U * 64 * 16, "a wave's sums of one fragment of rows fit its ring");
+    char ring[WAVES][RING];
+    static_assert(RING >= U * 64 * 16, "a wave's sums of one fragment of rows fit its ring");
 };
 
 // One pass of up to 16 R rows over the workgroup's 16 U weight rows.
-template <class T, class OUT, int U, int R, int WAVES>
-__device__ __forceinline__ void pass(const RowsArgs &a, int group, int row0, int live, int col0, Shared<U, WAVES> &sh) {
-    static_assert(kRing >= 16 * (U + R) * kCH, "a stage fits the ring");
+template <class T, class OUT, int U, int R, int WAVES, int RING>
+__device__ __forceinline__ void pass(const RowsArgs &a, int group, int row0, int live, int col0, Shared<U, WAVES, RING> &sh) {
+    static_assert(RING >= 16 * (U + R) * kCH, "a stage fits the ring");
     constexpr int CH = kCH;
     using Acc = typename Mini<T>::Acc;
     constexpr int CHUNKS = CH / 16, PER = 1024 / CH;      // chunks of a row; rows that a copy moves
@@ -154,7 +169,7 @@ __device__ __forceinline__ void pass(const RowsArgs &a, int group, int row0, int
     }
     const int x_copies = (live + PER - 1) / PER;
     const int copies = W_COPIES + x_copies, stage_bytes = copies * 1024;
-    const int stages = min(min(kRing / stage_bytes, kMaxStages), 40 / copies + 1);
+    const int stages = min(min(RING / stage_bytes, kMaxStages), 40 / copies + 1);
     const uint32_t base = ring::lds_addr(sh.ring[wave]);
     const int n = (chunks - wave + WAVES - 1) / WAVES;  // chunks of this wave
     // Each workgroup begins at another chunk of its rows: workgroups that run side by side read the same place in rows that lie a
@@ -241,12 +256,13 @@ __device__ __forceinline__ void pass(const RowsArgs &a, int group, int row0, int
     __syncthreads();  // the rings may be filled again
 }
 
-template <class T, class OUT, int U, int WAVES>
+// BLOCK == 0: a job is all rows of a group, 32 at a time; otherwise one block of up to BLOCK rows.
+template <class T, class OUT, int U, int WAVES, int RING, int BLOCK>
 __global__ __launch_bounds__(64 * WAVES) void grouped_mm_few_kernel(RowsArgs a, int strips) {
     static_assert(U <= WAVES, "a wave adds up the sums of one unit");
-    __shared__ __attribute__((aligned(1024))) Shared<U, WAVES> sh;
+    __shared__ __attribute__((aligned(1024))) Shared<U, WAVES, RING> sh;
     const int slot = (int)blockIdx.x / strips, col0 = ((int)blockIdx.x - slot * strips) * 16 * U;
-    const Span s = find_span(a, slot);
+    const Span s = find_span<BLOCK>(a, slot);
     if (s.zero) {
         constexpr int PER = 16 / Pack<OUT>::kBytes;
         const int chunks = min(16 * U, a.cols - col0) / PER;
@@ -257,35 +273,52 @@ __global__ __launch_bounds__(64 * WAVES) void grouped_mm_few_kernel(RowsArgs a, 
     for (int row0 = s.begin; row0 < s.end;) {
         const int left = s.end - row0;
         if (left <= 16) {
-            pass<T, OUT, U, 1, WAVES>(a, s.group, row0, left, col0, sh);
+            pass<T, OUT, U, 1, WAVES, RING>(a, s.group, row0, left, col0, sh);
             row0 += 16;
-        } else {
-            pass<T, OUT, U, 2, WAVES>(a, s.group, row0, min(left, 32), col0, sh);
+        } else if (BLOCK == 0 || left <= 32) {
+            pass<T, OUT, U, 2, WAVES, RING>(a, s.group, row0, min(left, 32), col0, sh);
             row0 += 32;
+        } else if constexpr (BLOCK > 0) {
+            pass<T, OUT, U, BLOCK / 16, WAVES, RING>(a, s.group, row0, left, col0, sh);
+            row0 += BLOCK;
         }
     }
 }
 
-// Whether a product goes to these kernels: few rows per group on average.  (Both ways are right for any rows.)
-inline bool takes(const RowsArgs &a) {
-    return a.rows <= 16 * (int64_t)a.n_groups && ((int64_t)a.cols / 16 + 1) * (a.n_groups + 1) < INT32_MAX;
+template <class T, class OUT, int U, int WAVES, int RING, int BLOCK>
+void launch_as(const RowsArgs &a, int64_t slots, hipStream_t stream) {
+    const int strips = (a.cols + 16 * U - 1) / (16 * U);
+    hipLaunchKernelGGL((grouped_mm_few_kernel<T, OUT, U, WAVES, RING, BLOCK>), dim3((uint32_t)(strips * slots)), dim3(64 * WAVES), 0, stream,
+                       a, strips);
 }
 
+// Launches these kernels if they are the faster ones.  (Both ways are right for any rows.)
 template <class T, class OUT>
-void launch(const RowsArgs &a, hipStream_t stream) {
-    const int slots = (int)(a.rows < a.n_groups ? a.rows : a.n_groups) + (a.offsets != nullptr ? 1 : 0);
-    const int strips1 = (a.cols + 15) / 16, strips2 = (a.cols + 31) / 32;
-    const int64_t jobs1 = (int64_t)strips1 * slots, cus = resident_grid();
-    // Few jobs: eight waves share one, so that a CU's share is under way at once (one row through 4096 x 7168 in 8 bits: 7.5 us
-    // instead of 10.4 with four); with more than two jobs per CU four (8 of 128 experts of 1536 x 2048: 12.3 us instead of
-    // 14.9).  Wider jobs read x less often: 32 weight rows where there are many (64 tokens on 256 experts of 4096 x 7168 in 8 bits:
-    // 590 us instead of 664).
-    if (jobs1 <= 2 * cus)
-        hipLaunchKernelGGL((grouped_mm_few_kernel<T, OUT, 1, 8>), dim3((uint32_t)jobs1), dim3(512), 0, stream, a, strips1);
-    else if (jobs1 <= 8 * cus)
-        hipLaunchKernelGGL((grouped_mm_few_kernel<T, OUT, 1, 4>), dim3((uint32_t)jobs1), dim3(256), 0, stream, a, strips1);
-    else
-        hipLaunchKernelGGL((grouped_mm_few_kernel<T, OUT, 2, 4>), dim3((uint32_t)(strips2 * (int64_t)slots)), dim3(256), 0, stream, a, strips2);
+bool launch(const RowsArgs &a, hipStream_t stream) {
+    const int64_t cus = resident_grid(), behind = a.offsets != nullptr ? 1 : 0;
+    const int64_t slots = std::min(a.rows, a.n_groups) + behind, strips = (a.cols + 15) / 16;
+    if (a.rows <= 16 * (int64_t)a.n_groups && strips * slots < INT32_MAX) {
+        // Few jobs: eight waves share one, so that a CU's share is under way at once (one row through 4096 x 7168 in 8 bits: 7.5
+        // us instead of 10.4 with four); with more than two jobs per CU four (8 of 128 experts of 1536 x 2048: 12.3 us instead
+        // of 14.9).  Wider jobs read x less often: 32 weight rows where there are many (64 tokens on 256 experts of 4096 x
+        // 7168 in 8 bits: 590 us instead of 664).
+        if (strips * slots <= 2 * cus) launch_as<T, OUT, 1, 8, kRing, 0>(a, slots, stream);
+        else if (strips * slots <= 8 * cus) launch_as<T, OUT, 1, 4, kRing, 0>(a, slots, stream);
+        else launch_as<T, OUT, 2, 4, kRing, 0>(a, slots, stream);
+        return true;
+    }
+    // Blocks of 64 rows x 32 columns (16, with at most one such job per CU), where tiles of 256 columns would leave CUs idle: a
+    // tile's contraction is one workgroup's, a block's is shared by eight waves and so short that even eight jobs per CU are
+    // faster (8 experts of 512 x 4096 in bf16, 256 to 1024 tokens' rows: 83 -> 24, 100 -> 67 us; 128 to 1024 rows through 4096 x
+    // 7168 in 8 bits: 48 -> 18, 72 -> 63, 77 -> 120 us with 16 jobs per CU).
+    const int64_t blocks = a.rows / kBlock + slots, block_jobs = (strips + 1) / 2 * blocks;
+    const int64_t tiles = (a.rows / 256 + std::min(a.rows, a.n_groups)) * ((a.cols + kCols - 1) / kCols);
+    if (tiles <= cus && block_jobs <= 8 * cus) {
+        if (block_jobs <= cus) launch_as<T, OUT, 1, 8, kBlockRing, kBlock>(a, blocks, stream);
+        else launch_as<T, OUT, 2, 8, kBlockRing, kBlock>(a, blocks, stream);
+        return true;
+    }
+    return false;
 }
 
 }  // namespace few

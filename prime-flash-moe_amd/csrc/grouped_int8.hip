@@ -13,7 +13,7 @@ using namespace pmoe::gmm;
 
 template <class OUT>
 void launch(const RowsArgs &a, int grid, hipStream_t stream) {
-    if (few::takes(a)) return few::launch<I8, OUT>(a, stream);
+    if (few::launch<I8, OUT>(a, stream)) return;
     hipLaunchKernelGGL((grouped_mm_kernel<I8, false, OUT>), dim3(grid), dim3(kThreads), 0, stream, a);
 }
 

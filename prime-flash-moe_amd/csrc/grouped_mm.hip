@@ -13,7 +13,7 @@ using namespace pmoe::gmm;
 template <class T, bool QX>
 void launch_rows(const RowsArgs &a, int grid, hipStream_t stream) {
     if constexpr (!QX)
-        if (few::takes(a)) return few::launch<T, T>(a, stream);
+        if (few::launch<T, T>(a, stream)) return;
     hipLaunchKernelGGL((grouped_mm_kernel<T, QX, T>), dim3(grid), dim3(kThreads), 0, stream, a);
 }
 
