@@ -81,6 +81,7 @@ extern "C" int pmoe_grouped_mm(const void *x, const void *w, void *out, const in
     a.rows = (int)M;
     a.cols = N;
     a.depth = K;
+    a.once = stores_once(M * N * 2);
     const int grid = grid_of(tiles);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == PMOE_DTYPE_BF16) w_across ? launch_rows<Bf16, true>(a, grid, s) : launch_rows<Bf16, false>(a, grid, s);
@@ -110,6 +111,7 @@ extern "C" int pmoe_grouped_mm_wgrad(const void *dy, const void *x, void *dw, co
     a.rows = (int)M;
     a.out_rows = N;
     a.cols = K;
+    a.once = stores_once((int64_t)n_groups * N * K * 2);
     hipStream_t s = static_cast<hipStream_t>(stream);
     // (tiles of 128 rows where those of 256 would leave CUs idle)
     const int64_t tall = (int64_t)n_groups * ((N + 255) / 256) * ((K + kCols - 1) / kCols);

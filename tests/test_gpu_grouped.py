@@ -204,6 +204,40 @@ def test_gradients_of_gradients(device):
         assert ((g.double() - ref).abs() <= bound).all()
 
 
+def test_gradients_of_shared_and_absent_operands(device):
+    """One matrix for all experts (expanded), rows without an expert, no rows at all."""
+    import prime_moe
+    gen = torch.Generator().manual_seed(17)
+    ends, N, K = [40, 40, 100], 40, 72
+    off = ends_tensor(ends, device)
+    w = make((N, K), gen, torch.bfloat16, device, 0.2).requires_grad_()
+    x, dy = make((110, K), gen, torch.bfloat16, device).requires_grad_(), make((110, N), gen, torch.bfloat16, device)
+    y = prime_moe.grouped_mm(x, w.expand(3, N, K), off)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    ref, mags = R.mm(dy, w.detach().t().expand(3, K, N), ends)
+    R.check(dx, ref, mags, N)
+    parts, mags = R.wgrad(dy, x.detach(), ends)
+    # each expert's part is rounded to bf16, then the sum of two (torch adds them in fp32 and rounds once)
+    bound = 2.0 ** -8 * (parts.abs().sum(0) * 1.01 + parts.sum(0).abs()) + 100 * 2.0 ** -23 * mags.sum(0)
+    assert ((dw.double() - parts.sum(0)).abs() <= bound * 1.01 + 1e-30).all()
+    none = x.detach()[:0].requires_grad_()
+    y = prime_moe.grouped_mm(none, w.expand(3, N, K), torch.zeros_like(off))
+    dx, dw = torch.autograd.grad(y, (none, w), dy[:0])
+    assert dx.shape == (0, K) and (dw == 0).all()
+    with torch.no_grad():
+        assert not prime_moe.grouped_mm(x, w.expand(3, N, K), off).requires_grad
+
+
+def test_offsets_that_change_before_the_backward_pass_are_noticed(device):
+    import prime_moe
+    off = ends_tensor([3, 8], device)
+    x, w = torch.ones((8, 16), dtype=torch.bfloat16, device=device, requires_grad=True), torch.ones((2, 8, 16), dtype=torch.bfloat16, device=device)
+    y = prime_moe.grouped_mm(x, w, off)
+    off[0] = 5
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_sums_are_held_in_32_bits(device, cus):
     """A long contraction of small terms onto a large one: sums in 16 bits would lose them."""
     import prime_moe
