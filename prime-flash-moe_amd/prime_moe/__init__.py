@@ -12,6 +12,10 @@ key ``CUDA``.  Argument checks raise ``RuntimeError`` for the conditions the ref
 Extras that the reference leaves to its callers: a fake impl for ``moe_align`` (so all
 three ops trace), :func:`quantize_mx`, the OCP-MX quantiser in front of the mxfp8 op, and
 :func:`route`, the router front-end (top-k + softmax + ``moe_align``) in front of both.
+
+Next to the fused forward pass, the experts' products on their own, for training, other activations and 8-bit integers:
+:func:`grouped_mm` (differentiable), :func:`grouped_mm_wgrad`, :func:`grouped_mm_int8`, :func:`quantize_int8` and
+:func:`expert_offsets`, which makes their ``offsets`` from a schedule.
 """
 from __future__ import annotations
 
