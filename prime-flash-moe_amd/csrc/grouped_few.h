@@ -308,12 +308,12 @@ bool launch(const RowsArgs &a, hipStream_t stream) {
         return true;
     }
     // Blocks of 64 rows x 32 columns (16, with at most one such job per CU), where tiles of 256 columns would leave CUs idle: a
-    // tile's contraction is one workgroup's, a block's is shared by eight waves and so short that even eight jobs per CU are
-    // faster (8 experts of 512 x 4096 in bf16, 256 to 1024 tokens' rows: 83 -> 24, 100 -> 67 us; 128 to 1024 rows through 4096 x
-    // 7168 in 8 bits: 48 -> 18, 72 -> 63, 77 -> 120 us with 16 jobs per CU).
+    // tile's contraction is one workgroup's, a block's is shared by eight waves, and so up to three jobs per CU are faster (8
+    // experts of 512 x 4096 in bf16, beside tiles of the height that suits them best: 1.4 jobs per CU 24 us instead of 48, 2.4 37
+    // instead of 48; 8 of 1024 x 4096: 2.9 38 instead of 49, but 4.9 65 instead of 48).
     const int64_t blocks = a.rows / kBlock + slots, block_jobs = (strips + 1) / 2 * blocks;
     const int64_t tiles = (a.rows / 256 + std::min(a.rows, a.n_groups)) * ((a.cols + kCols - 1) / kCols);
-    if (tiles <= cus && block_jobs <= 8 * cus) {
+    if (tiles <= cus && block_jobs <= 3 * cus) {
         if (block_jobs <= cus) launch_as<T, OUT, 1, 8, kBlockRing, kBlock>(a, blocks, stream);
         else launch_as<T, OUT, 2, 8, kBlockRing, kBlock>(a, blocks, stream);
         return true;

@@ -12,6 +12,8 @@ constexpr int64_t kMaxStride = 4 << 20;        // 16-bit elements: 256 rows stay
 // Tiles a launch can have at most, -1 if they cannot be counted in 32 bits.
 int64_t most_tiles(int64_t rows, int cols, int n_groups);
 int grid_of(int64_t tiles);
+// Whether even tiles of 128 rows are more than one round of workgroups.
+bool fills(int64_t rows, int cols);
 
 }  // namespace gmm
 }  // namespace pmoe

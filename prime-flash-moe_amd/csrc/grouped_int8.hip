@@ -15,7 +15,7 @@ template <class OUT>
 void launch(const RowsArgs &a, int grid, hipStream_t stream) {
     if (few::launch<I8, OUT>(a, stream)) return;
     // A dense product whose last round of tiles would be a few rows high: these go to the kernels for few rows, which spread their
-    // contraction over the whole chip (4097 rows x 4096 x 7168: 147 -> 109 us; the 4097th alone took a workgroup 40 us) unless
+    // contraction over the whole chip (4097 rows x 4096 x 7168: 147 -> 104 us; the 4097th alone took a workgroup 40 us) unless
     // they are wide (73 rows of 28672 columns: 70 us there, 50 in tiles).
     const int col_tiles = (a.cols + kCols - 1) / kCols, round = resident_grid() / col_tiles * 256;
     const int rest = a.offsets == nullptr && round > 0 && a.rows > round ? a.rows % round : 0;
@@ -69,7 +69,8 @@ extern "C" int pmoe_grouped_mm_int8(const void *x, const void *w, const float *x
     a.once = stores_once(M * a.out_pitch);
     a.x_scale = x_scale;
     a.w_scale = w_scale;
-    const int grid = grid_of(tiles);
+    a.fills = fills(M, N);
+    const int grid = grid_of(a.fills ? tiles : 4 * tiles);  // (a tile of 256 rows may be four of 64)
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (out_dtype == PMOE_DTYPE_BF16) launch<Bf16>(a, grid, s);
     else if (out_dtype == PMOE_DTYPE_F16) launch<F16>(a, grid, s);

@@ -24,6 +24,7 @@ struct RowsArgs {
     int depth;               // contraction, elements
     const float *x_scale, *w_scale;  // 8-bit integers: (rows), (groups, cols)
     bool once;               // see stores_once
+    bool fills;              // even tiles of 128 rows are more than one round of the grid
 };
 // dw[g] = sum over the group's rows of dy[r] x[r]^T; strides in bytes.
 struct WgradArgs {
@@ -63,8 +64,37 @@ struct Walk {
     int begin[5];   // first rows of the thread's groups, and the end of the last one
     int before[4];  // row tiles in front of each
     int row_tiles, col_tiles, live_rows, total;
+    int shift;  // a tile has at most 2^shift rows
 
-    static __device__ __forceinline__ int tiles_of(int rows) { return (rows + 255) / 256; }
+    __device__ __forceinline__ int tiles_of(int rows) const { return (rows + (1 << shift) - 1) >> shift; }
+    // Tiles of 128 or 64 rows where they still are one round of the grid: so many CUs would stand still beside taller ones, and a
+    // slab of fewer rows is over sooner (8 experts of 512 columns, contraction 4096, bf16: 1020 rows 67 -> 49 us, 8192 rows 69 ->
+    // 63; 512 rows of one group x 4096 x 4096: 71 -> 42; 510 rows whose tiles are short, contraction 512: 16.2 -> 14.6).
+    __device__ __forceinline__ void choose_height(const RowsArgs &a, int tid, int *words) {
+        shift = 8;
+        if (a.fills) return;
+        int n[2] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) n[c] += (begin[i + 1] - begin[i] + (64 << c) - 1) >> (6 + c);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+#pragma unroll
+            for (int d = 32; d > 0; d /= 2) n[c] += __shfl_xor(n[c], d, 64);
+            if ((tid & 63) == 0) words[4 * c + (tid >> 6)] = n[c];
+        }
+        ring::all_read();
+#pragma unroll
+        for (int c = 1; c >= 0; --c) {
+            int sum = 0;
+#pragma unroll
+            for (int w = 0; w < kWaves; ++w) sum += words[4 * c + w];
+            if ((int64_t)sum * col_tiles <= gridDim.x) shift = 6 + c;
+        }
+        ring::all_read();  // the words may be written again
+        shift = uniform(shift);
+    }
     static __device__ __forceinline__ int height_of(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 63) & ~63; }
     __device__ __forceinline__ void setup(const RowsArgs &a, int tid, int *words) {
         const int g0 = 4 * tid, lane = tid & 63, wave = tid >> 6;
@@ -89,10 +119,13 @@ struct Walk {
             live_rows = max(live_rows, words[w]);
         }
         live_rows = uniform(live_rows);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) begin[i + 1] = max(begin[i + 1], begin[i]);
+        col_tiles = (a.cols + kCols - 1) / kCols;
+        choose_height(a, tid, words);
         int count[4], fm[4], sum[4] = {}, incl[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            begin[i + 1] = max(begin[i + 1], begin[i]);
             const int rows = begin[i + 1] - begin[i];
             count[i] = tiles_of(rows);
             fm[i] = rows > 0 ? height_of(rows, count[i]) / 64 : 0;
@@ -131,23 +164,28 @@ struct Walk {
         }
         ring::all_read();  // the words may be written again
         row_tiles = uniform(row_tiles);
-        col_tiles = (a.cols + kCols - 1) / kCols;
         total = (row_tiles + (a.rows - live_rows + 255) / 256) * col_tiles;
     }
 
     // Tile t < total, through four words of LDS: post(), a barrier, get().
     __device__ __forceinline__ void post(int t, int tid, int *words) const {
+        int mine = -1, from = 0, rows = 0, local = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int rows = begin[i + 1] - begin[i], rt = tiles_of(rows), local = t - before[i] * col_tiles;
-            if (rows > 0 && local >= 0 && local < rt * col_tiles) {
-                const int band = local / (rt * kWalkCols), width = min(kWalkCols, col_tiles - band * kWalkCols);
-                const int rem = local - band * rt * kWalkCols, m = rem / width, height = height_of(rows, rt);
-                words[0] = 4 * tid + i;
-                words[1] = begin[i] + m * height;
-                words[2] = min(height, rows - m * height);
-                words[3] = band * kWalkCols + rem - m * width;
-            }
+            const int n = begin[i + 1] - begin[i], at = t - before[i] * col_tiles;
+            const bool hit = (n > 0) & (at >= 0) & (at < tiles_of(n) * col_tiles);
+            mine = hit ? i : mine;
+            from = hit ? begin[i] : from;
+            rows = hit ? n : rows;
+            local = hit ? at : local;
+        }
+        if (mine >= 0) {
+            const int rt = tiles_of(rows), band = local / (rt * kWalkCols), width = min(kWalkCols, col_tiles - band * kWalkCols);
+            const int rem = local - band * rt * kWalkCols, m = rem / width, height = height_of(rows, rt);
+            words[0] = 4 * tid + mine;
+            words[1] = from + m * height;
+            words[2] = min(height, rows - m * height);
+            words[3] = band * kWalkCols + rem - m * width;
         }
     }
     __device__ __forceinline__ Tile get(const RowsArgs &a, int t, const int *words) const {

@@ -26,6 +26,7 @@ int64_t most_tiles(int64_t rows, int cols, int n_groups) {
     const int64_t t = (rows / 256 + n_groups + 2) * ((cols + kCols - 1) / kCols);
     return t < (1ll << 31) - 8192 ? t : -1;
 }
+bool fills(int64_t rows, int cols) { return rows / 128 * ((cols + kCols - 1) / kCols) > resident_grid(); }
 int grid_of(int64_t tiles) { return (int)std::min<int64_t>(resident_grid(), (tiles + 7) / 8 * 8); }
 
 }  // namespace gmm
@@ -82,7 +83,8 @@ extern "C" int pmoe_grouped_mm(const void *x, const void *w, void *out, const in
     a.cols = N;
     a.depth = K;
     a.once = stores_once(M * N * 2);
-    const int grid = grid_of(tiles);
+    a.fills = fills(M, N);
+    const int grid = grid_of(a.fills ? tiles : 4 * tiles);  // (a tile of 256 rows may be four of 64)
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == PMOE_DTYPE_BF16) w_across ? launch_rows<Bf16, true>(a, grid, s) : launch_rows<Bf16, false>(a, grid, s);
     else w_across ? launch_rows<F16, true>(a, grid, s) : launch_rows<F16, false>(a, grid, s);
