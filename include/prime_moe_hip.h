@@ -182,7 +182,7 @@ int pmoe_route(const void *logits, int logits_dtype, const float *bias, int32_t 
  * activations, training, 8-bit integers).  No counterpart in the reference.  Rows are sorted by expert: group g holds rows
  * offsets[g-1] .. offsets[g]-1 (from 0 for g == 0), offsets (n_groups) int32 on the device, non-decreasing and within
  * 0 .. M, at most 1024 groups.  Offsets that are not leave the outputs unspecified, but no access leaves the arguments.
- * Strides are in elements; the dimension without a stride is contiguous.  Nothing is allocated, no call needs a workspace,
+ * Strides are in elements; the dimension without a stride is contiguous.  Operands and outputs are 16-byte aligned.  Nothing is allocated, no call needs a workspace,
  * the outputs do not depend on anything but the inputs (no atomics), and no call synchronises the host.
  *
  * expert_offsets -- the ends of the groups of a schedule of pmoe_moe_align with block_m == pad_to == 1 (a sorted

@@ -1,5 +1,7 @@
 // Limits that the entry points of the ragged expert products share.
 #pragma once
+#include <initializer_list>
+
 #include "pmoe_common.h"
 
 namespace pmoe {
@@ -22,3 +24,7 @@ bool fills(int64_t rows, int cols);
     PMOE_REQUIRE((stride) >= (width) && (stride) % (unit) == 0 && (stride) <= (most),                                             \
                  "%s: rows %lld elements apart (supported: %lld .. %lld, multiples of %d)", what, (long long)(stride),            \
                  (long long)(width), (long long)(most), (int)(unit))
+
+#define PMOE_REQUIRE_ALIGNED(what, ...)                                                                                           \
+    for (const void *p : std::initializer_list<const void *>{__VA_ARGS__})                                                        \
+        PMOE_REQUIRE(reinterpret_cast<uintptr_t>(p) % 16 == 0, "%s: operands and outputs must be 16-byte aligned", what)

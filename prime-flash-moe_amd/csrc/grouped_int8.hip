@@ -51,6 +51,7 @@ extern "C" int pmoe_grouped_mm_int8(const void *x, const void *w, const float *x
     PMOE_REQUIRE(w_group_stride % 16 == 0 && w_group_stride >= 0, "grouped_mm_int8: the stride of w between groups must be a multiple of 16");
     if (M == 0) return PMOE_OK;
     PMOE_REQUIRE(x && w && x_scale && w_scale && out, "grouped_mm_int8: null pointer");
+    PMOE_REQUIRE_ALIGNED("grouped_mm_int8", x, w, out);
     const int64_t tiles = most_tiles(M, N, n_groups);
     PMOE_REQUIRE(tiles > 0, "grouped_mm_int8: too many tiles");
     RowsArgs a = {};

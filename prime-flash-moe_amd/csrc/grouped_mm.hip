@@ -67,6 +67,7 @@ extern "C" int pmoe_grouped_mm(const void *x, const void *w, void *out, const in
     PMOE_REQUIRE(w_group_stride % 8 == 0 && w_group_stride >= 0, "grouped_mm: the stride of w between groups must be a multiple of 8");
     if (M == 0) return PMOE_OK;
     PMOE_REQUIRE(x && w && out && offsets, "grouped_mm: null pointer");
+    PMOE_REQUIRE_ALIGNED("grouped_mm", x, w, out);
     const int64_t tiles = most_tiles(M, N, n_groups);
     PMOE_REQUIRE(tiles > 0, "grouped_mm: too many tiles");
     RowsArgs a = {};
@@ -100,6 +101,7 @@ extern "C" int pmoe_grouped_mm_wgrad(const void *dy, const void *x, void *dw, co
     PMOE_REQUIRE_STRIDE("grouped_mm_wgrad: dy", dy_stride, N, 8, kMaxStride);
     PMOE_REQUIRE_STRIDE("grouped_mm_wgrad: x", x_stride, K, 8, kMaxStride);
     PMOE_REQUIRE(dw && offsets && (M == 0 || (dy && x)), "grouped_mm_wgrad: null pointer");
+    PMOE_REQUIRE_ALIGNED("grouped_mm_wgrad", dy, x, dw);
     const int64_t tiles = (int64_t)n_groups * ((N + 127) / 128) * ((K + kCols - 1) / kCols);
     PMOE_REQUIRE(tiles < (1ll << 31) - 8192, "grouped_mm_wgrad: too many tiles");
     WgradArgs a = {};

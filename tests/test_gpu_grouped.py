@@ -61,6 +61,22 @@ def test_forward(device, cus, counts, behind, N, K, across):
         assert (y[ends[-1]:] == 0).all()
 
 
+# on eight CUs and two tiles of columns: tiles of 64 rows up to 256 rows, of 128 up to 512, of 256 beyond
+@pytest.mark.parametrize("counts,behind", [([256], 0), ([257], 0), ([512], 3), ([513], 0), ([1100], 260), ([64, 0, 63, 65], 0),
+                                           ([65, 64, 65], 0), ([128, 128, 129], 0), ([300, 212], 0)])
+@pytest.mark.parametrize("across", [False, True])
+def test_heights_of_tiles(device, cus, counts, behind, across):
+    import prime_moe
+    gen = torch.Generator().manual_seed(len(counts) + counts[0])
+    ends, N, K = np.cumsum(counts).tolist(), 512, 256
+    x = make((ends[-1] + behind, K), gen, torch.bfloat16, device)
+    w = make((len(counts), N, K), gen, torch.bfloat16, device, K ** -0.5)
+    y = prime_moe.grouped_mm(x, w.transpose(1, 2).contiguous().transpose(1, 2) if across else w, ends_tensor(ends, device))
+    ref, mags = R.mm(x, w, ends)
+    R.check(y, ref, mags, K)
+    assert (y[ends[-1]:] == 0).all()
+
+
 @pytest.mark.parametrize("counts,behind", RAGGED)
 @pytest.mark.parametrize("N,K", [(8, 8), (24, 64), (256, 128), (264, 72), (520, 1000), (1032, 264)])
 def test_weight_gradient(device, cus, counts, behind, N, K):
@@ -367,6 +383,42 @@ def test_two_streams_at_once(device, cus):
     for i in range(2):
         for y in got[i]:
             assert torch.equal(y, want[i])
+
+
+def test_backward_of_another_stream(device):
+    import prime_moe
+    gen = torch.Generator().manual_seed(21)
+    ends = R.sized(900, 4, gen)
+    off = ends_tensor(ends, device)
+    x, w = make((900, 256), gen, torch.bfloat16, device), make((4, 128, 256), gen, torch.bfloat16, device, 0.05)
+    g = make((900, 128), gen, torch.bfloat16, device)
+    want = (prime_moe.grouped_mm(g, w.transpose(1, 2), off), prime_moe.grouped_mm_wgrad(g, x, off))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        a, b = x.detach().requires_grad_(), w.detach().requires_grad_()
+        y = prime_moe.grouped_mm(a, b, off)
+    torch.cuda.current_stream().wait_stream(side)
+    got = torch.autograd.grad(y, (a, b), g)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_traced_training_step(device):
+    import prime_moe
+    gen = torch.Generator().manual_seed(22)
+    ends = R.sized(300, 4, gen)
+    off = ends_tensor(ends, device)
+    x = make((300, 256), gen, torch.bfloat16, device).requires_grad_()
+    w = make((4, 128, 256), gen, torch.bfloat16, device, 0.05).requires_grad_()
+    g = make((300, 128), gen, torch.bfloat16, device)
+
+    def step(x, w, off):
+        return prime_moe.grouped_mm(x, w, off)
+
+    want = torch.autograd.grad(step(x, w, off), (x, w), g)
+    got = torch.autograd.grad(torch.compile(step, backend="aot_eager", fullgraph=True)(x, w, off), (x, w), g)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
 def test_registration(device):

@@ -133,6 +133,19 @@ def test_c_side_refuses_before_any_launch():
     assert lib.pmoe_quantize_int8(None, 1, None, None, 0, 64, 64, None) == 0
 
 
+def test_c_side_refuses_addresses_that_are_not_aligned():
+    from prime_moe import _native
+    lib, at = _native.load(), 1 << 20
+    for off_by in ((8, 0, 0), (0, 8, 0), (0, 0, 2)):
+        x, w, out = (at + o for o in off_by)
+        assert lib.pmoe_grouped_mm(x, w, out, at, 2, 4, 32, 64, 64, 64, 2048, 0, 1, None) == 1
+        assert b"aligned" in lib.pmoe_last_error()
+        assert lib.pmoe_grouped_mm_wgrad(x, w, out, at, 2, 4, 32, 64, 32, 64, 1, None) == 1
+        assert b"aligned" in lib.pmoe_last_error()
+        assert lib.pmoe_grouped_mm_int8(x, w, at, at, out, None, 1, 4, 32, 64, 64, 64, 0, 1, None) == 1
+        assert b"aligned" in lib.pmoe_last_error()
+
+
 def test_cpu_tensors_are_refused():
     import prime_moe
     for call in (lambda: prime_moe.grouped_mm(t(4, 64), t(2, 32, 64), off(1, 4)), lambda: prime_moe.grouped_mm_wgrad(t(4, 32), t(4, 64), off(4)),
