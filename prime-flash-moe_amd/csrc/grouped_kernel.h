@@ -70,9 +70,11 @@ struct Walk {
     // Tiles of 128 or 64 rows where they still are one round of the grid: so many CUs would stand still beside taller ones, and a
     // slab of fewer rows is over sooner (8 experts of 512 columns, contraction 4096, bf16: 1020 rows 67 -> 49 us, 8192 rows 69 ->
     // 63; 512 rows of one group x 4096 x 4096: 71 -> 42; 510 rows whose tiles are short, contraction 512: 16.2 -> 14.6).
+    // (Between its words and setup's furthest ends, which a wave may still be reading, there is no barrier: they are others.)
     __device__ __forceinline__ void choose_height(const RowsArgs &a, int tid, int *words) {
         shift = 8;
         if (a.fills) return;
+        int *const counts = words + kWaves;
         int n[2] = {};
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -82,14 +84,14 @@ struct Walk {
         for (int c = 0; c < 2; ++c) {
 #pragma unroll
             for (int d = 32; d > 0; d /= 2) n[c] += __shfl_xor(n[c], d, 64);
-            if ((tid & 63) == 0) words[4 * c + (tid >> 6)] = n[c];
+            if ((tid & 63) == 0) counts[kWaves * c + (tid >> 6)] = n[c];
         }
         ring::all_read();
 #pragma unroll
         for (int c = 1; c >= 0; --c) {
             int sum = 0;
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) sum += words[4 * c + w];
+            for (int w = 0; w < kWaves; ++w) sum += counts[kWaves * c + w];
             if ((int64_t)sum * col_tiles <= gridDim.x) shift = 6 + c;
         }
         ring::all_read();  // the words may be written again
