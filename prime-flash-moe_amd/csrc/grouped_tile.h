@@ -87,21 +87,22 @@ __device__ const uint4 g_zeros = {0, 0, 0, 0};
 // Copies to `lds` (wave-uniform byte address) + OFF.  One scalar instruction in front of each: what stands between two matrix
 // instructions of the only wave of a SIMD has 32 cycles, and a longer chain of dependent scalar instructions (a wave number
 // read, shifted and added for every copy) cost 50 cycles a copy.
+// (The wait state behind it is the one that the instruction set asks for between a scalar write of M0 and a load to LDS.)
 template <int OFF>
 __device__ __forceinline__ void copy16(const char *base, uint32_t voff, uint32_t lds) {
-    asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(base), "s"(lds), "n"(OFF) : "memory", "scc");
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(base), "s"(lds), "n"(OFF) : "memory", "scc");
 }
 // The same with the non-temporal hint, for what no other workgroup reads.
 template <int OFF>
 __device__ __forceinline__ void copy16_once(const char *base, uint32_t voff, uint32_t lds) {
-    asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1 nt" : : "v"(voff), "s"(base), "s"(lds), "n"(OFF) : "memory", "scc");
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" : : "v"(voff), "s"(base), "s"(lds), "n"(OFF) : "memory", "scc");
 }
 template <int OFF>
 __device__ __forceinline__ void copy16_at(const char *src, uint32_t lds) {
-    asm volatile("s_add_u32 m0, %1, %2\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds), "n"(OFF) : "memory", "scc");
+    asm volatile("s_add_u32 m0, %1, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(src), "s"(lds), "n"(OFF) : "memory", "scc");
 }
 __device__ __forceinline__ void copy4_at(const char *src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" : : "v"(src), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(src), "s"(lds) : "memory");
 }
 // Calls f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>).
 template <int N, class F>

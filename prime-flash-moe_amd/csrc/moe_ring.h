@@ -89,17 +89,19 @@ __device__ __forceinline__ uint32_t lds_addr(const char *p) {
 // compiles the two translation units that include this file to assembly and fails if a kernel that contains a
 // copy touches M0 anywhere outside these statements (tests/test_host.py); a GPU test runs the tile paths with the
 // most copies between two barriers on poisoned LDS (tests/test_gpu_lds_copies.py).
+// The instruction set asks software for a wait state between a scalar write of M0 and a load to LDS that reads it; what the
+// compiler would put in for its own code stands in the statements here, where it does not look.
 __device__ __forceinline__ void copy16(const char *base, uint32_t voff, const char *lds_dst) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(base), "s"(lds_addr(lds_dst)) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(voff), "s"(base), "s"(lds_addr(lds_dst)) : "memory");
 }
 // The same copy with the non-temporal hint, for weight rows that no other workgroup reads (an expert with a
 // single row tile): the lines leave the caches first.  The decode shape streams its weights 12 % faster
 // with it; weight rows that several row tiles share lose up to 20 % with it.
 __device__ __forceinline__ void copy16_once(const char *base, uint32_t voff, const char *lds_dst) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" : : "v"(voff), "s"(base), "s"(lds_addr(lds_dst)) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" : : "v"(voff), "s"(base), "s"(lds_addr(lds_dst)) : "memory");
 }
 __device__ __forceinline__ void copy4(const char *base, uint32_t voff, const char *lds_dst) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" : : "v"(voff), "s"(base), "s"(lds_addr(lds_dst)) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(voff), "s"(base), "s"(lds_addr(lds_dst)) : "memory");
 }
 // A wave-uniform pointer, read through lane 0 so that the compiler keeps it in scalar registers.
 __device__ __forceinline__ const char *uniform_ptr(const char *p) {
