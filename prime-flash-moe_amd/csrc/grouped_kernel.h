@@ -97,7 +97,7 @@ struct Walk {
         ring::all_read();  // the words may be written again
         shift = uniform(shift);
     }
-    static __device__ __forceinline__ int height_of(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 63) & ~63; }
+    static __device__ __forceinline__ int height_of(int rows, int tiles) { return ((rows - 1) / tiles + 64) & ~63; }  // rows >= 1
     __device__ __forceinline__ void setup(const RowsArgs &a, int tid, int *words) {
         const int g0 = 4 * tid, lane = tid & 63, wave = tid >> 6;
         // A group begins where the furthest end in front of it is (its predecessor's, if the ends are in order), so that

@@ -40,3 +40,9 @@ def walk(tmp_path_factory):
 def test_walks_do_not_depend_on_the_order_of_the_waves(walk):
     res = subprocess.run([walk], capture_output=True, text=True, timeout=300)
     assert res.returncode == 0, res.stderr
+
+
+def test_walk_over_the_longest_groups(walk):
+    """Groups of nearly 2^31 rows: no sum of rows and tiles passes 32 bits."""
+    res = subprocess.run([walk, "huge"], capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0, res.stderr
