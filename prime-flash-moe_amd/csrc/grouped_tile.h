@@ -231,8 +231,9 @@ struct Feed {
     __device__ __forceinline__ void set_length(int elements, int bytes_per) {
         len_p = PX ? elements : elements * bytes_per;
         len_q = QX ? elements : elements * bytes_per;
-        full = elements * bytes_per / kSlab;
-        n_slabs = max((elements * bytes_per + kSlab - 1) / kSlab, 2);
+        const int per = kSlab / bytes_per;  // (the bytes of a group's rows may pass 32 bits; an operand's along do not)
+        full = elements / per;
+        n_slabs = max(full + (elements % per > 0), 2);
     }
     // `at`: the wave's first piece in the stage.
     template <int C>

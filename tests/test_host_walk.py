@@ -46,3 +46,17 @@ def test_walk_over_the_longest_groups(walk):
     """Groups of nearly 2^31 rows: no sum of rows and tiles passes 32 bits."""
     res = subprocess.run([walk, "huge"], capture_output=True, text=True, timeout=300)
     assert res.returncode == 0, res.stderr
+
+
+def test_slabs_of_the_longest_contractions(tmp_path):
+    from prime_moe import build
+    tile = open(os.path.join(build.CSRC, "grouped_tile.h")).read()
+    (tmp_path / "slabs.inc").write_text(cut(tile, "constexpr int kSlab"))
+    member = re.search(r"^    __device__ __forceinline__ void set_length\(.*?^    \}\n", tile, re.M | re.S)
+    (tmp_path / "set_length.inc").write_text(member.group(0))
+    exe = str(tmp_path / "slabs")
+    res = subprocess.run(["g++", "-std=c++17", "-O1", "-fwrapv", "-I", str(tmp_path), os.path.join(HERE, "host", "slabs.cpp"), "-o", exe],
+                         capture_output=True, text=True)
+    assert res.returncode == 0, res.stderr[-3000:]
+    res = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert res.returncode == 0, res.stderr
