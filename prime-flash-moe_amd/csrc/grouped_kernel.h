@@ -312,7 +312,9 @@ __device__ __forceinline__ void store_tile(const typename T::Acc (&acc)[4][FM], 
     out += first_row * pitch + first_col * P::kBytes;
     live -= first_row;
     cols -= first_col;
-    const uint32_t lane_off = (uint32_t)sub * (uint32_t)pitch + chunk * 16;
+    // (32 bits hold three rows of 2^29 bytes, or seven of an 8-bit product in 16 bits; seven of 2^30 they do not)
+    using Offset = std::conditional_t<P::kBytes == 4, int64_t, uint32_t>;
+    const Offset lane_off = (Offset)sub * (Offset)pitch + chunk * 16;
     const bool whole = live >= 32 * FM && cols >= 128;
     auto put = [&](auto part) {
         constexpr int t = part.value / (4 / FRAGS), h = part.value % (4 / FRAGS);
