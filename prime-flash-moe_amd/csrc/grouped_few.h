@@ -297,7 +297,8 @@ template <class T, class OUT>
 bool launch(const RowsArgs &a, hipStream_t stream) {
     const int64_t cus = resident_grid(), behind = a.offsets != nullptr ? 1 : 0;
     const int64_t slots = std::min(a.rows, a.n_groups) + behind, strips = (a.cols + 15) / 16;
-    if (a.rows <= 16 * (int64_t)a.n_groups && strips * slots < INT32_MAX) {
+    // (A launch has less than 2^32 threads: 256 a job of 32 weight rows where jobs are many.)
+    if (a.rows <= 16 * (int64_t)a.n_groups && (strips + 1) / 2 * slots <= UINT32_MAX / 256) {
         // Few jobs: eight waves share one, so that a CU's share is under way at once (one row through 4096 x 7168 in 8 bits: 7.5
         // us instead of 10.4 with four); with more than two jobs per CU four (8 of 128 experts of 1536 x 2048: 12.3 us instead
         // of 14.9).  Wider jobs read x less often: 32 weight rows where there are many (64 tokens on 256 experts of 4096 x
