@@ -408,14 +408,19 @@ struct GroupedMmWgrad : torch::autograd::Function<GroupedMmWgrad> {
         return {ddy, dx, Tensor()};
     }
 };
-bool differentiated(const Tensor &a, const Tensor &b) { return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad()); }
+// A dual tensor has a tangent and need not require gradients: without a tangent of its own the output would stand for one that
+// does not change.
+bool differentiated(const char *op, const Tensor &a, const Tensor &b) {
+    REQUIRE(!a._fw_grad(0).defined() && !b._fw_grad(0).defined(), op, ": forward-mode derivatives are not implemented");
+    return at::GradMode::is_enabled() && (a.requires_grad() || b.requires_grad());
+}
 Tensor grouped_mm_autograd(const Tensor &x, const Tensor &w, const Tensor &offsets) {
-    if (differentiated(x, w)) return GroupedMm::apply(x, w, offsets);
+    if (differentiated("grouped_mm", x, w)) return GroupedMm::apply(x, w, offsets);
     at::AutoDispatchBelowADInplaceOrView below;
     return call_mm(x, w, offsets);
 }
 Tensor grouped_mm_wgrad_autograd(const Tensor &dy, const Tensor &x, const Tensor &offsets) {
-    if (differentiated(dy, x)) return GroupedMmWgrad::apply(dy, x, offsets);
+    if (differentiated("grouped_mm_wgrad", dy, x)) return GroupedMmWgrad::apply(dy, x, offsets);
     at::AutoDispatchBelowADInplaceOrView below;
     return call_wgrad(dy, x, offsets);
 }

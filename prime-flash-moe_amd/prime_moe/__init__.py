@@ -230,9 +230,9 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch
     ``x`` (M, K), ``w`` (E, N, K), both bfloat16 or float16; ``offsets`` (E,) int32 on the same GPU, non-decreasing, at most
     1024 experts.  Rows from ``offsets[-1]`` on come out as zeros.  Sums in fp32, rounded once.  ``x`` needs a contiguous last
     dimension; ``w`` may be stored either way (``w.transpose(1, 2)`` of an (E, K, N) tensor).  K, N and the strides are
-    multiples of 8, tensors start 16-byte aligned.  Differentiable in ``x`` and ``w`` (any number of times).  Offsets are
-    read on the device and not checked: with other values the output is unspecified, but nothing outside the arguments is read
-    or written.
+    multiples of 8, tensors start 16-byte aligned.  Differentiable in ``x`` and ``w`` (backward, any number of times; a tensor
+    with a forward-mode tangent is refused).  Offsets are read on the device and not checked: with other values the output is
+    unspecified, but nothing outside the arguments is read or written.
     """
     return torch.ops.prime_moe.grouped_mm(x, w, offsets)
 
