@@ -368,10 +368,11 @@ Tensor call_wgrad(const Tensor &dy, const Tensor &x, const Tensor &offsets) {
     return op.call(dy, x, offsets);
 }
 
+// (contiguous() would return a contiguous tensor that begins at an odd element, such as a piece of a flat gradient, as it is)
 Tensor laid_out(const Tensor &t) {
-    const bool fine = (t.size(1) == 1 || t.stride(1) == 1) && (t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) % 8 == 0 && t.stride(0) <= 4 << 20)) &&
-                      t.storage_offset() % 8 == 0;
-    return fine ? t : t.contiguous();
+    const bool rows = t.dim() == 2 && (t.size(1) == 1 || t.stride(1) == 1) &&
+                      (t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) % 8 == 0 && t.stride(0) <= 4 << 20));
+    return (rows || t.is_contiguous()) && t.storage_offset() % 8 == 0 ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 
 struct GroupedMm : torch::autograd::Function<GroupedMm> {
@@ -401,7 +402,7 @@ struct GroupedMmWgrad : torch::autograd::Function<GroupedMmWgrad> {
         const auto saved = ctx->get_saved_variables();
         Tensor ddy, dx;
         if (grads[0].defined()) {
-            const Tensor g = grads[0].contiguous();  // (E, N, K)
+            const Tensor g = laid_out(grads[0]);  // (E, N, K)
             if (ctx->needs_input_grad(0)) ddy = call_mm(saved[1], g, saved[2]);
             if (ctx->needs_input_grad(1)) dx = call_mm(saved[0], g.transpose(1, 2), saved[2]);
         }
