@@ -56,9 +56,9 @@ __device__ __forceinline__ uint32_t quantize4(float a, float b, float c, float d
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float q = rintf(x[j] * inv);
-        const float r = fmaf(-q, scale, x[j]), half = 0.5f * scale;
+        const float r = fmaf(-q, scale, x[j]), twice = 2.0f * fabsf(r);  // (half of the smallest scales would be rounded)
         const bool odd = ((int)q & 1) != 0;
-        if (fabsf(r) > half || (fabsf(r) == half && odd)) q += copysignf(1.0f, r);
+        if (twice > scale || (twice == scale && odd)) q += copysignf(1.0f, r);
         out |= ((uint32_t)(int)q & 0xffu) << (8 * j);
     }
     return out;
