@@ -8,8 +8,8 @@
 // 155 us, 5.2 TB/s of reads and writes; a large copy on the same card 4.8).  64 rows of 7168: 6 us, a launch and a latency.
 #include <algorithm>
 
+#include "grouped_host.h"
 #include "moe_tile.h"
-#include "pmoe_common.h"
 
 namespace {
 
@@ -143,6 +143,7 @@ extern "C" int pmoe_quantize_int8(const void *src, int dtype, void *q, float *sc
     PMOE_REQUIRE(stride >= cols && stride % 8 == 0, "quantize_int8: rows %lld elements apart (supported: multiples of 8 from %d on)", (long long)stride, cols);
     if (rows == 0) return PMOE_OK;
     PMOE_REQUIRE(src && q && scales, "quantize_int8: null pointer");
+    PMOE_REQUIRE_ALIGNED("quantize_int8", src, q);
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (dtype == PMOE_DTYPE_BF16) launch<FromBf16>(src, stride * 2, q, scales, rows, cols, s);
     else if (dtype == PMOE_DTYPE_F16) launch<FromF16>(src, stride * 2, q, scales, rows, cols, s);
