@@ -55,8 +55,8 @@ struct Tile {
     bool zero;       // rows behind the last group: their outputs are zero
 };
 
-// Walk over the tiles of a launch.  A group's rows are cut into as few tiles as there can be, of even height (in steps of
-// 64 rows).  The walk takes the tallest tiles first: tile number t runs through [height, 4 to 1][group][8 column tiles][row
+// Walk over the tiles of a launch.  A group's rows are cut into as few tiles as there can be, of their even share rounded up to
+// 64 rows (the last one has what is left: 1025 rows are four tiles of 256 and one of a row).  The walk takes the tallest tiles first: tile number t runs through [height, 4 to 1][group][8 column tiles][row
 // tile][column tile], and the rows behind the last group follow.  The workgroups, which take every grid-th tile, then have
 // equal shares of every height (in the order of the groups: the largest share 16 % above the mean with 128 groups of 512
 // rows on average), and a tile is nearly always followed by one of its own height.  Thread i holds groups 4 i .. 4 i + 3.

@@ -20,8 +20,8 @@
 // slab has landed and hands this slab's stage to the copies of the slab two behind it, which may be the next tile's.
 //
 // Bound by the matrix pipe and the card's power: in a long contraction a slab of the tallest tile takes 2130 cycles, 2048 of
-// them matrix instructions, and the clock falls as they fill up (8192 x 8192 x 8192 in bf16: 1.44 PFLOP/s along, 1.45 with one
-// operand across, 1.46 with both; the library's 1.61, 1.38 and 1.19).  A tile costs about 10 000 cycles besides: the way out
+// them matrix instructions, and the clock falls as they fill up (8192 x 8192 x 8192 in bf16: 1.40 PFLOP/s along, with one
+// operand across and with both; the library's on the same card 1.57, 1.34 and 1.16).  A tile costs about 10 000 cycles besides: the way out
 // (7000, the L2's writes), the first fragments, the next tile's addresses.  Where weights are read by two or three tiles (128
 // experts of 512 rows) the slabs wait for memory, 700 cycles a step of 64 rows instead of 512.
 //

@@ -218,8 +218,9 @@ def expert_offsets(expert_ids: torch.Tensor, num_tokens_post_padded: torch.Tenso
     """``offsets`` of the ragged products below, from a schedule of ``moe_align`` / :func:`route` with ``block_m=1``.
 
     Such a schedule is the permutation that sorts the pairs by expert without padding: ``sorted_token_ids`` holds the pair of
-    every row, ``expert_ids`` its expert.  Returns the end of every expert's rows, ``(num_experts,)`` int32; pairs that the
-    schedule drops (ids outside the experts) lie behind the last end.
+    every row, ``expert_ids`` its expert.  Returns the end of every expert's rows, ``(num_experts,)`` int32.  Pairs that the
+    schedule drops (ids outside the experts) are in none of its rows: behind the last end ``sorted_token_ids`` is -1, which a
+    program that drops pairs has to leave out (or clamp, with the weight zero) before it gathers and scatters by it.
     """
     return torch.ops.prime_moe.expert_offsets(expert_ids, num_tokens_post_padded, num_experts)
 
@@ -229,7 +230,8 @@ def grouped_mm(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor) -> torch
 
     ``x`` (M, K), ``w`` (E, N, K), both bfloat16 or float16; ``offsets`` (E,) int32 on the same GPU, non-decreasing, at most
     1024 experts.  Rows from ``offsets[-1]`` on come out as zeros.  Sums in fp32, rounded once.  ``x`` needs a contiguous last
-    dimension; ``w`` may be stored either way (``w.transpose(1, 2)`` of an (E, K, N) tensor).  K, N and the strides are
+    dimension; ``w`` may be stored either way (``w.transpose(1, 2)`` of an (E, K, N) tensor; for few rows per expert, as in
+    decoding, (E, N, K) is 1.4 to 5.6 times faster, as only that layout has a streaming kernel).  K, N and the strides are
     multiples of 8, tensors start 16-byte aligned.  Differentiable in ``x`` and ``w`` (backward, any number of times; a tensor
     with a forward-mode tangent is refused).  Offsets are read on the device and not checked: with other values the output is
     unspecified, but nothing outside the arguments is read or written.
