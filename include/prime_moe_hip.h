@@ -170,7 +170,7 @@ int pmoe_quantize_mx(const void *src_bf16, void *q, void *scales, int64_t rows, 
  */
 #define PMOE_DTYPE_F32 0
 #define PMOE_DTYPE_BF16 1
-#define PMOE_DTYPE_F16 2 /* the ragged products and quantize_int8 only */
+#define PMOE_DTYPE_F16 2 /* the ragged products, the quantisers to integers and moe_layer only */
 int pmoe_route(const void *logits, int logits_dtype, const float *bias, int32_t *topk_ids,
                float *topk_weights, int32_t *sorted_token_ids, int32_t *expert_ids,
                int32_t *num_tokens_post_padded, int n_tokens, int num_experts, int top_k,
@@ -225,6 +225,47 @@ int pmoe_grouped_mm_int8(const void *x, const void *w, const float *x_scale, con
  */
 int pmoe_quantize_int8(const void *src, int dtype, void *q, float *scales, int64_t rows, int cols, int64_t stride,
                        void *stream);
+
+/*
+ * Weights of 4 bits: a matrix (N,K) of value * scale, an integer from -8 to 7 and a bf16 or fp16 number per `group` (32, 64 or
+ * 128) consecutive values of a row.  No counterpart in the reference.  N is a multiple of 16, K of group; what follows holds
+ * tiles of 16 rows x 128 columns, the last ones filled up with zeros:
+ *   q      [N/16][ceil(K/128)][1024 bytes]: byte 16 (r + 16 c) + 4 j + b holds row r, columns 32 j + 8 c + (0,2), (4,6), (1,3),
+ *          (5,7) for b = 0 .. 3, the first in the low four bits, as value + 8
+ *   scale  [N/16][ceil(K/128)][16 rows][128/group]
+ * A stack of matrices is one behind the other.  All addresses are 16-byte aligned.
+ *
+ * quantize_int4 -- src (rows,cols), contiguous, bf16, fp16 or fp32, rows a multiple of 16 (a stack: all its rows):
+ *   scale = the number of scale_dtype nearest to max(amax c, least), c = 1 / 7 in fp32, least = 2^-126 (bf16) or 2^-24 (fp16); value =
+ *   the integer nearest to the exact quotient, ties to even, from -8 to 7.  A group with an infinity or a NaN, or whose scale
+ *   is beyond the type, gets the scale NaN and zeros.
+ * dequantize_int4 -- out (rows,cols) = value * scale in the scales' type, rounded once.
+ */
+int pmoe_quantize_int4(const void *src, int dtype, void *q, void *scales, int scale_dtype, int64_t rows, int cols, int group,
+                       void *stream);
+int pmoe_dequantize_int4(const void *q, const void *scales, void *out, int dtype, int64_t rows, int cols, int group,
+                         void *stream);
+
+/*
+ * grouped_mm_int4 -- pmoe_grouped_mm with weights of 4 bits, made for few rows per group: x (M,K), out (M,N) and w_scale bf16 or
+ *   fp16 (dtype), fp32 sums, rounded once; zero for rows behind the last group.  offsets == NULL: one matrix for all rows.
+ *   A row of x that holds an infinity or a NaN comes out as NaN.  Every 32 rows of a group read its weights again.
+ */
+int pmoe_grouped_mm_int4(const void *x, const void *w, const void *w_scale, void *out, const int32_t *offsets, int n_groups,
+                         int64_t M, int N, int K, int group, int64_t x_stride, int dtype, void *stream);
+
+/*
+ * moe_layer -- a whole layer for up to 16 tokens: logits = x gate^T (+ bias), top_k and softmax as pmoe_route, out = the sum
+ *   over a token's experts of weight * w2[e] swiglu(w1[e] x).  No counterpart in the reference.
+ *   x (T,K), gate (E,K), out (T,K); w1 (E,2H,K), gate rows first, and w2 (E,K,H); all of dtype (bf16 or fp16) and contiguous,
+ *   or, with group != 0, w1 and w2 of 4 bits with their scales.  bias (E) fp32 or null.  topk_ids, topk_weights (T,top_k): what was
+ *   chosen.  K and H are multiples of 8, with weights of 4 bits of 16 and of group.  num_experts <= 512, top_k <= min(32, E).
+ *   The workspace, 256-byte aligned, is scratch of this one call.
+ */
+size_t pmoe_moe_layer_workspace_bytes(int T, int H, int num_experts, int top_k);
+int pmoe_moe_layer(const void *x, const void *gate, const float *bias, const void *w1, const void *w1_scale, const void *w2,
+                   const void *w2_scale, int group, void *out, int32_t *topk_ids, float *topk_weights, int T, int K, int H,
+                   int num_experts, int top_k, int dtype, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,147 @@
+// Weights of 4 bits with a scale per 32, 64 or 128 values of a row, gfx950: their layout in memory, and how a wave multiplies
+// them with rows of 16-bit numbers.
+//
+// A weight is q s, q an integer in -8 .. 7, s a 16-bit number.  A matrix (N, K) is held in tiles of 16 rows x 128 columns, 1 KB
+// each, [N / 16][K / 128]; lane l of the wave that takes a tile reads its 16 bytes at 16 l, so that a load of the wave is 1 KB in
+// one piece (rows of their own would be 64 bytes of 16 rows per load).  With r = l % 16, c = l / 16: dword j of the lane holds row
+// r, columns 32 j + 8 c .. + 7, which is what a matrix instruction of 16 x 16 x 32 wants of the lane.  In the dword, as q + 8,
+// columns 0, 2, 4, 6, 1, 3, 5, 7 from the lowest bits up: a shift and a mask leave two neighbours in the halves of a register.
+// Scales: [N / 16][K / 128][16 rows][128 / group].  What a last tile has behind column K is q = 0, s = 0.
+//
+// To 16 bits without arithmetic: q + 8 in the highest bits of the mantissa of 16.0 is the number 24 + q.  The 24 too much leaves
+// the sum again as a matrix instruction of its own, with -24 in place of the weights, once per row of x and group for all strips
+// of weights of a wave.  (Products and sums are fp32: what cancels costs two bits of 24, where the result keeps 8 or 11.  A row of
+// x with an infinity comes out as NaN, where the exact weights would leave an infinity.)  Eight weights are four shifts and four
+// and-ors; conversions to fp32 and back would be twenty instructions, which is more than there is time for at the rate of the memory:
+// 21 weights a cycle and CU.
+//
+// Sums of a group are scaled in fp32, by four multiply-adds per 128 / group tiles.
+#pragma once
+#include "grouped_few.h"
+
+namespace pmoe {
+namespace int4 {
+
+using gmm::Bf16;
+using gmm::F16;
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kTileRows = 16, kTileCols = 128, kTileBytes = 1024;
+
+__host__ __device__ inline int tiles_of(int k) { return (k + kTileCols - 1) / kTileCols; }
+
+template <class T>
+struct Num;
+template <>
+struct Num<Bf16> {
+    static constexpr uint32_t kMinus24 = 0xc1c0c1c0u;
+    static __device__ __forceinline__ i32x4 wide(uint32_t w) {
+        constexpr uint32_t M = 0x00780078u, B = 0x41804180u;
+        return i32x4{(int)((w << 3 & M) | B), (int)((w >> 1 & M) | B), (int)((w >> 5 & M) | B), (int)((w >> 9 & M) | B)};
+    }
+    static __device__ __forceinline__ float to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
+    static __device__ __forceinline__ uint16_t from_f32(float v) { return (uint16_t)pack2_bf16(v, 0.f); }
+    static __device__ __forceinline__ bool finite(uint16_t v) { return (v & 0x7f80u) != 0x7f80u; }
+    static constexpr uint16_t kNan = 0x7fc0;
+    static constexpr float kLeastScale = 0x1p-126f;
+};
+template <>
+struct Num<F16> {
+    static constexpr uint32_t kMinus24 = 0xce00ce00u;
+    static __device__ __forceinline__ i32x4 wide(uint32_t w) {
+        constexpr uint32_t M = 0x03c003c0u, B = 0x4c004c00u;
+        return i32x4{(int)((w << 6 & M) | B), (int)((w << 2 & M) | B), (int)((w >> 2 & M) | B), (int)((w >> 6 & M) | B)};
+    }
+    static __device__ __forceinline__ float to_f32(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
+    static __device__ __forceinline__ uint16_t from_f32(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+    static __device__ __forceinline__ bool finite(uint16_t v) { return (v & 0x7c00u) != 0x7c00u; }
+    static constexpr uint16_t kNan = 0x7e00;
+    static constexpr float kLeastScale = 0x1p-24f;
+};
+
+__device__ __forceinline__ i32x4 load_once16(const char *p) { return __builtin_nontemporal_load(reinterpret_cast<const i32x4 *>(p)); }
+
+// The scales of a lane's row in a tile.
+template <int GROUP>
+struct TileScales {
+    static constexpr int kCount = kTileCols / GROUP, kBytes = kTileRows * kCount * 2;  // of a row, of a tile
+    uint16_t v[kCount];
+    __device__ __forceinline__ void load(const char *tile, int r) {
+        const char *p = tile + r * kCount * 2;
+        if constexpr (kCount == 4) {
+            const uint2 u = *reinterpret_cast<const uint2 *>(p);
+            v[0] = (uint16_t)u.x, v[1] = (uint16_t)(u.x >> 16), v[2] = (uint16_t)u.y, v[3] = (uint16_t)(u.y >> 16);
+        } else if constexpr (kCount == 2) {
+            const uint32_t u = *reinterpret_cast<const uint32_t *>(p);
+            v[0] = (uint16_t)u, v[1] = (uint16_t)(u >> 16);
+        } else {
+            v[0] = *reinterpret_cast<const uint16_t *>(p);
+        }
+    }
+};
+
+// acc[u][t] += rows of x times the weights of tiles t0 .. t1 - 1 of U strips (16 weight rows each), for one wave.  Lane l, r = l %
+// 16, c = l / 16: `w[u]`, `s[u]` begin strip u; `x[t]` is row 16 t + r of x (any row that can be read, where there are fewer).
+// acc[u][t][i]: weight row r, row 16 t + 4 c + i of x.  `k`: columns, a multiple of 32; nothing of x is read behind them.
+// S: tiles whose loads are in flight together.
+template <class T, int GROUP, int U, int R, int S>
+__device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[U], const char *const (&s)[U], const char *const (&x)[R], int t0,
+                                     int t1, int k) {
+    using Sc = TileScales<GROUP>;
+    const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+    const i32x4 minus = {(int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24};
+    for (int t = t0; t < t1; t += S) {
+        i32x4 wv[S][U], xv[S][R][4];
+        Sc sc[S][U];
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+            if (t + i < t1) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    wv[i][u] = load_once16(w[u] + (int64_t)(t + i) * kTileBytes + lane * 16);
+                    sc[i][u].load(s[u] + (int64_t)(t + i) * Sc::kBytes, r);
+                }
+                const int left = k - (t + i) * kTileCols;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int q = 0; q < R; ++q) {
+                        xv[i][q][j] = i32x4{0, 0, 0, 0};
+                        if (32 * j < left) xv[i][q][j] = *reinterpret_cast<const i32x4 *>(x[q] + (int64_t)(t + i) * 256 + j * 64 + c * 16);
+                    }
+            }
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+            if (t + i < t1) {
+                f32x4 sum[U][R], less[R];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool first = j % (GROUP / 32) == 0, last = (j + 1) % (GROUP / 32) == 0;
+                    if (first) {  // -24 times the sums of the group's part of x
+#pragma unroll
+                        for (int q = 0; q < R; ++q) {
+                            less[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                            for (int m = 0; m < GROUP / 32; ++m) less[q] = gmm::few::Mini<T>::mfma(xv[i][q][j + m], minus, less[q]);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const i32x4 b = Num<T>::wide((uint32_t)wv[i][u][j]);
+#pragma unroll
+                        for (int q = 0; q < R; ++q) {
+                            sum[u][q] = gmm::few::Mini<T>::mfma(xv[i][q][j], b, first ? less[q] : sum[u][q]);
+                            if (last) {
+                                const float f = Num<T>::to_f32(sc[i][u].v[j / (GROUP / 32)]);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[u][q][e] = fmaf(sum[u][q][e], f, acc[u][q][e]);
+                            }
+                        }
+                    }
+                }
+            }
+    }
+}
+
+}  // namespace int4
+}  // namespace pmoe

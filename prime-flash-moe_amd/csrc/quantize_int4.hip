@@ -1,0 +1,176 @@
+// To 4 bits and back (layout: int4_tile.h).
+//
+// scale = the 16-bit number nearest to max(amax c, least) with c = 1 / 7 in fp32; q = the integer nearest to the exact quotient of
+// value and scale, ties to even, from -8 to 7: the remainder value - q scale, which an fma gives without rounding, corrects the first
+// guess value (1 / scale), which is off by one at most.  A group with an infinity, a NaN, or a scale beyond the 16-bit type
+// gets the scale NaN and q = 0.
+//
+// Bound by memory.  A wave takes a tile: its loads are 64 contiguous bytes of 16 rows, whole lines over four of them, its stores 1 KB.
+#include <algorithm>
+
+#include "grouped_host.h"
+#include "int4_tile.h"
+
+namespace {
+
+using namespace pmoe;
+using namespace pmoe::int4;
+
+struct F32 {};
+template <class FROM>
+struct Load {
+    static constexpr int kBytes = 2;
+    static __device__ __forceinline__ void eight(const char *p, float (&v)[8]) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[2 * i] = Num<FROM>::to_f32((uint16_t)w[i]), v[2 * i + 1] = Num<FROM>::to_f32((uint16_t)(w[i] >> 16));
+    }
+};
+template <>
+struct Load<F32> {
+    static constexpr int kBytes = 4;
+    static __device__ __forceinline__ void eight(const char *p, float (&v)[8]) {
+        const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+};
+
+__device__ __forceinline__ int nearest(float x, float scale, float inv) {
+    float q = rintf(x * inv);
+    const float rest = fmaf(-q, scale, x), twice = 2.0f * fabsf(rest);
+    const bool odd = ((int)q & 1) != 0;
+    if (twice > scale || (twice == scale && odd)) q += copysignf(1.0f, rest);
+    return (int)fminf(fmaxf(q, -8.0f), 7.0f);
+}
+
+// Position of column k (0 .. 7) of a dword, in nibbles.
+__device__ __forceinline__ constexpr int nibble(int k) { return k / 2 + k % 2 * 4; }
+
+template <class FROM, class T, int GROUP>
+__global__ __launch_bounds__(256) void quantize_int4_kernel(const char *__restrict__ src, char *__restrict__ q, char *__restrict__ scales,
+                                                            int64_t n_tiles, int tiles, int cols) {
+    using Sc = TileScales<GROUP>;
+    constexpr int PER = GROUP / 32;
+    const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+    for (int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); tile < n_tiles; tile += (int64_t)gridDim.x * 4) {
+        const int64_t strip = tile / tiles;
+        const int col0 = (int)(tile - strip * tiles) * kTileCols;
+        const char *p = src + ((strip * 16 + r) * cols + col0 + 8 * c) * Load<FROM>::kBytes;
+        float v[4][8] = {};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (col0 + 32 * j < cols) Load<FROM>::eight(p + 32 * j * Load<FROM>::kBytes, v[j]);
+        uint32_t out[4];
+#pragma unroll
+        for (int g = 0; g < Sc::kCount; ++g) {
+            uint32_t peak = 0;  // largest magnitude as its bits: infinity and the NaNs are above all numbers
+#pragma unroll
+            for (int j = 0; j < PER; ++j)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) peak = max(peak, __float_as_uint(v[g * PER + j][k]) & 0x7fffffffu);
+            peak = max(peak, (uint32_t)__shfl_xor((int)peak, 16, 64));
+            peak = max(peak, (uint32_t)__shfl_xor((int)peak, 32, 64));
+            uint16_t s16 = Num<T>::from_f32(fmaxf(__uint_as_float(peak) * (1.0f / 7.0f), Num<T>::kLeastScale));
+            const bool fine = peak < 0x7f800000u && Num<T>::finite(s16), inside = col0 + g * GROUP < cols;
+            if (!fine) s16 = Num<T>::kNan;
+            const float scale = Num<T>::to_f32(s16), inv = 1.0f / scale;
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                uint32_t word = 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) word |= (uint32_t)(fine ? nearest(v[g * PER + j][k], scale, inv) + 8 : 8) << (4 * nibble(k));
+                out[g * PER + j] = word;
+            }
+            if (c == 0) reinterpret_cast<uint16_t *>(scales + tile * Sc::kBytes)[r * Sc::kCount + g] = inside ? s16 : 0;
+        }
+        *reinterpret_cast<uint4 *>(q + tile * kTileBytes + lane * 16) = make_uint4(out[0], out[1], out[2], out[3]);
+    }
+}
+
+template <class T, int GROUP>
+__global__ __launch_bounds__(256) void dequantize_int4_kernel(const char *__restrict__ q, const char *__restrict__ scales, char *__restrict__ out,
+                                                              int64_t n_tiles, int tiles, int cols) {
+    using Sc = TileScales<GROUP>;
+    const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+    for (int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); tile < n_tiles; tile += (int64_t)gridDim.x * 4) {
+        const int64_t strip = tile / tiles;
+        const int col0 = (int)(tile - strip * tiles) * kTileCols;
+        const uint4 u = *reinterpret_cast<const uint4 *>(q + tile * kTileBytes + lane * 16);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        Sc sc;
+        sc.load(scales + tile * Sc::kBytes, r);
+        char *p = out + ((strip * 16 + r) * cols + col0 + 8 * c) * 2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float s = Num<T>::to_f32(sc.v[j / (GROUP / 32)]);
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = (float)((int)(w[j] >> (4 * nibble(k)) & 15u) - 8) * s;
+            const uint2 lo = gmm::Pack<T>::four(v[0], v[1], v[2], v[3]), hi = gmm::Pack<T>::four(v[4], v[5], v[6], v[7]);
+            if (col0 + 32 * j < cols) *reinterpret_cast<uint4 *>(p + 64 * j) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
+    }
+}
+
+int grid_for(int64_t tiles) { return (int)std::min<int64_t>((tiles + 3) / 4, 16384); }
+
+template <class FROM, class T>
+int quantize(const void *src, void *q, void *scales, int64_t n_tiles, int tiles, int cols, int group, hipStream_t s) {
+    const char *from = static_cast<const char *>(src);
+    char *to = static_cast<char *>(q), *sc = static_cast<char *>(scales);
+    const dim3 grid(grid_for(n_tiles)), block(256);
+    if (group == 32) hipLaunchKernelGGL((quantize_int4_kernel<FROM, T, 32>), grid, block, 0, s, from, to, sc, n_tiles, tiles, cols);
+    else if (group == 64) hipLaunchKernelGGL((quantize_int4_kernel<FROM, T, 64>), grid, block, 0, s, from, to, sc, n_tiles, tiles, cols);
+    else hipLaunchKernelGGL((quantize_int4_kernel<FROM, T, 128>), grid, block, 0, s, from, to, sc, n_tiles, tiles, cols);
+    return check_launch("quantize_int4 launch");
+}
+template <class T>
+int dequantize(const void *q, const void *scales, void *out, int64_t n_tiles, int tiles, int cols, int group, hipStream_t s) {
+    const char *from = static_cast<const char *>(q), *sc = static_cast<const char *>(scales);
+    char *to = static_cast<char *>(out);
+    const dim3 grid(grid_for(n_tiles)), block(256);
+    if (group == 32) hipLaunchKernelGGL((dequantize_int4_kernel<T, 32>), grid, block, 0, s, from, sc, to, n_tiles, tiles, cols);
+    else if (group == 64) hipLaunchKernelGGL((dequantize_int4_kernel<T, 64>), grid, block, 0, s, from, sc, to, n_tiles, tiles, cols);
+    else hipLaunchKernelGGL((dequantize_int4_kernel<T, 128>), grid, block, 0, s, from, sc, to, n_tiles, tiles, cols);
+    return check_launch("dequantize_int4 launch");
+}
+
+int check_sizes(const char *what, int64_t rows, int cols, int group) {
+    PMOE_REQUIRE(group == 32 || group == 64 || group == 128, "%s: group must be 32, 64 or 128, got %d", what, group);
+    PMOE_REQUIRE(rows >= 0 && rows % 16 == 0 && cols > 0 && cols % group == 0 && cols <= gmm::kMaxSide,
+                 "%s: rows (%lld) must be a multiple of 16, cols (%d) a positive multiple of group (%d) up to 2^28", what, (long long)rows, cols, group);
+    return PMOE_OK;
+}
+
+}  // namespace
+
+extern "C" int pmoe_quantize_int4(const void *src, int dtype, void *q, void *scales, int scale_dtype, int64_t rows, int cols, int group,
+                                  void *stream) {
+    PMOE_REQUIRE(dtype == PMOE_DTYPE_BF16 || dtype == PMOE_DTYPE_F16 || dtype == PMOE_DTYPE_F32, "quantize_int4: dtype must be bf16, fp16 or fp32");
+    PMOE_REQUIRE(scale_dtype == PMOE_DTYPE_BF16 || scale_dtype == PMOE_DTYPE_F16, "quantize_int4: scale_dtype must be bf16 or fp16");
+    if (int rc = check_sizes("quantize_int4", rows, cols, group)) return rc;
+    if (rows == 0) return PMOE_OK;
+    PMOE_REQUIRE(src && q && scales, "quantize_int4: null pointer");
+    PMOE_REQUIRE_ALIGNED("quantize_int4", src, q, scales);
+    const int tiles = tiles_of(cols);
+    const int64_t n_tiles = rows / 16 * tiles;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const bool to_bf16 = scale_dtype == PMOE_DTYPE_BF16;
+    if (dtype == PMOE_DTYPE_BF16) return to_bf16 ? quantize<Bf16, Bf16>(src, q, scales, n_tiles, tiles, cols, group, s) : quantize<Bf16, F16>(src, q, scales, n_tiles, tiles, cols, group, s);
+    if (dtype == PMOE_DTYPE_F16) return to_bf16 ? quantize<F16, Bf16>(src, q, scales, n_tiles, tiles, cols, group, s) : quantize<F16, F16>(src, q, scales, n_tiles, tiles, cols, group, s);
+    return to_bf16 ? quantize<F32, Bf16>(src, q, scales, n_tiles, tiles, cols, group, s) : quantize<F32, F16>(src, q, scales, n_tiles, tiles, cols, group, s);
+}
+
+extern "C" int pmoe_dequantize_int4(const void *q, const void *scales, void *out, int dtype, int64_t rows, int cols, int group, void *stream) {
+    PMOE_REQUIRE(dtype == PMOE_DTYPE_BF16 || dtype == PMOE_DTYPE_F16, "dequantize_int4: dtype must be bf16 or fp16");
+    if (int rc = check_sizes("dequantize_int4", rows, cols, group)) return rc;
+    if (rows == 0) return PMOE_OK;
+    PMOE_REQUIRE(q && scales && out, "dequantize_int4: null pointer");
+    PMOE_REQUIRE_ALIGNED("dequantize_int4", q, scales, out);
+    const int tiles = tiles_of(cols);
+    const int64_t n_tiles = rows / 16 * tiles;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    return dtype == PMOE_DTYPE_BF16 ? dequantize<Bf16>(q, scales, out, n_tiles, tiles, cols, group, s)
+                                    : dequantize<F16>(q, scales, out, n_tiles, tiles, cols, group, s);
+}

@@ -490,6 +490,188 @@ std::tuple<Tensor, Tensor> quantize_int8(const Tensor &x) {
     return {q, scale};
 }
 
+// ------------------------------------------------------------------------------- weights of 4 bits, whole layers
+
+// A stack of matrices in tiles of 16 x 128 with its scales (see prime_moe_hip.h); `lead`: dimensions in front of a matrix.
+struct Int4 {
+    int64_t rows = 0, tiles = 0, group = 0;
+};
+Int4 int4_of(const char *op, const char *name, const Tensor &q, const Tensor &scale, int64_t lead, bool placement) {
+    REQUIRE(q.scalar_type() == at::kByte && q.dim() == lead + 3 && q.size(-1) == 1024, op, ": ", name, " must be uint8 of shape (",
+            lead ? "E, " : "", "N/16, ceil(K/128), 1024), as quantize_int4 makes it");
+    const int64_t per = scale.dim() == lead + 4 ? scale.size(-1) : 0;
+    REQUIRE((per == 1 || per == 2 || per == 4) && scale.size(-2) == 16 && scale.sizes().slice(0, lead + 2) == q.sizes().slice(0, lead + 2), op,
+            ": the scales of ", name, " must have the shape (", lead ? "E, " : "", "N/16, ceil(K/128), 16, 128/group), as quantize_int4 makes them");
+    require_16bit(op, "the scales", scale);
+    require_contiguous(op, {{name, &q}, {"the scales", &scale}});
+    if (placement) require_aligned(op, {{name, &q}, {"the scales", &scale}}, 16);
+    return {q.size(-3) * 16, q.size(-2), 128 / per};
+}
+void require_columns(const char *op, const char *name, const Int4 &w, int64_t k) {
+    REQUIRE(k > 0 && k % w.group == 0 && (k + 127) / 128 == w.tiles, op, ": ", name, " has ", w.tiles, " tiles of 128 columns in groups of ",
+            w.group, ", which does not fit ", k, " columns");
+}
+
+struct Int4Mm {
+    Rows x;
+    Int4 w;
+};
+Int4Mm check_grouped_mm_int4(const Tensor &x, const Tensor &w, const Tensor &w_scale, const std::optional<Tensor> &offsets, bool placement) {
+    const char *op = "grouped_mm_int4";
+    const bool dense = !offsets.has_value();
+    REQUIRE(x.dim() == 2, op, ": x must be 2-D (M, K)");
+    require_16bit(op, "x", x);
+    const Int4 m = int4_of(op, "w", w, w_scale, dense ? 0 : 1, placement);
+    REQUIRE(w_scale.scalar_type() == x.scalar_type(), op, ": x and w_scale must have the same dtype");
+    REQUIRE(x.size(0) <= kMostRows, op, ": too many rows");
+    require_side(op, "N", m.rows, 16);
+    require_side(op, "K", x.size(1), 32);
+    require_columns(op, "w", m, x.size(1));
+    if (!dense) require_groups(op, *offsets, w.size(0));
+    const Int4Mm p{rows_of(op, "x", x, 8), m};
+    if (placement) {
+        require_same_device(op, {{"x", &x}, {"w", &w}, {"w_scale", &w_scale}});
+        if (!dense) require_same_device(op, {{"x", &x}, {"offsets", &*offsets}});
+        require_aligned(op, {{"x", &x}}, 16);
+    }
+    return p;
+}
+Tensor grouped_mm_int4(const Tensor &x, const Tensor &w, const Tensor &w_scale, const std::optional<Tensor> &offsets) {
+    const Int4Mm p = check_grouped_mm_int4(x, w, w_scale, offsets, true);
+    const c10::Device dev = x.device();
+    const c10::DeviceGuard guard(dev);
+    Tensor out = empty({x.size(0), p.w.rows}, x.scalar_type(), dev);
+    check_status(pmoe_grouped_mm_int4(x.const_data_ptr(), w.const_data_ptr(), w_scale.const_data_ptr(), out.data_ptr(),
+                                      offsets.has_value() ? offsets->const_data_ptr<int32_t>() : nullptr, offsets.has_value() ? (int)w.size(0) : 1,
+                                      x.size(0), (int)p.w.rows, (int)x.size(1), (int)p.w.group, p.x.stride, dtype_code(x.scalar_type()),
+                                      stream_of(dev)));
+    return out;
+}
+
+void check_quantize_int4(const Tensor &w, int64_t group, at::ScalarType scale_dtype, bool placement) {
+    const char *op = "quantize_int4";
+    REQUIRE(dtype_code(w.scalar_type()) >= 0, op, ": w must be bfloat16, float16 or float32");
+    REQUIRE(scale_dtype == at::kBFloat16 || scale_dtype == at::kHalf, op, ": scale_dtype must be bfloat16 or float16");
+    REQUIRE(w.dim() >= 2, op, ": w must have two dimensions or more");
+    REQUIRE(group == 32 || group == 64 || group == 128, op, ": group must be 32, 64 or 128, got ", group);
+    require_side(op, "N", w.size(-2), 16);
+    require_side(op, "K", w.size(-1), group);
+    require_contiguous(op, {{"w", &w}});
+    if (placement) {
+        require_same_device(op, {{"w", &w}});
+        require_aligned(op, {{"w", &w}}, 16);
+    }
+}
+std::tuple<Tensor, Tensor> quantize_int4(const Tensor &w, int64_t group, at::ScalarType scale_dtype) {
+    check_quantize_int4(w, group, scale_dtype, true);
+    const c10::Device dev = w.device();
+    const c10::DeviceGuard guard(dev);
+    std::vector<int64_t> size = w.sizes().slice(0, w.dim() - 2).vec();
+    const int64_t cols = w.size(-1);
+    size.insert(size.end(), {w.size(-2) / 16, (cols + 127) / 128, 1024});
+    Tensor q = empty(size, at::kByte, dev);
+    size.back() = 16;
+    size.push_back(128 / group);
+    Tensor scale = empty(size, scale_dtype, dev);
+    check_status(pmoe_quantize_int4(w.const_data_ptr(), dtype_code(w.scalar_type()), q.data_ptr(), scale.data_ptr(), dtype_code(scale_dtype),
+                                    w.numel() / cols, (int)cols, (int)group, stream_of(dev)));
+    return {q, scale};
+}
+
+Int4 check_dequantize_int4(const Tensor &q, const Tensor &scale, int64_t columns, bool placement) {
+    const char *op = "dequantize_int4";
+    REQUIRE(q.dim() >= 3, op, ": q must be uint8 of shape (..., N/16, ceil(K/128), 1024), as quantize_int4 makes it");
+    const Int4 w = int4_of(op, "q", q, scale, q.dim() - 3, placement);
+    require_side(op, "columns", columns, w.group);
+    require_columns(op, "q", w, columns);
+    if (placement) require_same_device(op, {{"q", &q}, {"scale", &scale}});
+    return w;
+}
+Tensor dequantize_int4(const Tensor &q, const Tensor &scale, int64_t columns) {
+    const Int4 w = check_dequantize_int4(q, scale, columns, true);
+    const c10::Device dev = q.device();
+    const c10::DeviceGuard guard(dev);
+    std::vector<int64_t> size = q.sizes().slice(0, q.dim() - 3).vec();
+    size.insert(size.end(), {w.rows, columns});
+    Tensor out = empty(size, scale.scalar_type(), dev);
+    check_status(pmoe_dequantize_int4(q.const_data_ptr(), scale.const_data_ptr(), out.data_ptr(), dtype_code(scale.scalar_type()),
+                                      out.numel() / columns, (int)columns, (int)w.group, stream_of(dev)));
+    return out;
+}
+
+struct Layer {
+    const Tensor &x, &gate, &w1, &w2;
+    const Tensor *w1_scale, *w2_scale;  // null: weights of 16 bits
+    int64_t top_k;
+    const std::optional<Tensor> &bias;
+};
+struct LayerSizes {
+    int64_t hidden, group;  // columns of the activation
+};
+constexpr int64_t kMostTokens = 16, kMostExperts = 512, kMostTopK = 32;
+LayerSizes check_layer(const char *op, const Layer &l, bool placement) {
+    REQUIRE(l.x.dim() == 2 && l.gate.dim() == 2 && l.gate.size(1) == l.x.size(1), op, ": x must be 2-D (T, K), gate 2-D (E, K)");
+    const int64_t T = l.x.size(0), K = l.x.size(1), E = l.gate.size(0);
+    require_16bit(op, "x", l.x);
+    REQUIRE(l.gate.scalar_type() == l.x.scalar_type(), op, ": x and gate must have the same dtype");
+    REQUIRE(T <= kMostTokens, op, " takes up to ", kMostTokens, " tokens, got ", T, " (more: route and fused_moe_bf16)");
+    REQUIRE(E > 0 && E <= kMostExperts, op, " supports 1..", kMostExperts, " experts, got ", E);
+    REQUIRE(l.top_k > 0 && l.top_k <= std::min(kMostTopK, E), op, ": top_k must be in 1..min(", kMostTopK, ", E), got ", l.top_k);
+    LayerSizes z{0, 0};
+    if (l.w1_scale != nullptr) {
+        const Int4 up = int4_of(op, "w1", l.w1, *l.w1_scale, 1, placement), down = int4_of(op, "w2", l.w2, *l.w2_scale, 1, placement);
+        z = {up.rows / 2, up.group};
+        REQUIRE(up.group == down.group, op, ": w1 and w2 must have groups of the same size");
+        REQUIRE(l.w1_scale->scalar_type() == l.x.scalar_type() && l.w2_scale->scalar_type() == l.x.scalar_type(), op, ": x and the scales must have the same dtype");
+        REQUIRE(l.w1.size(0) == E && l.w2.size(0) == E, op, ": w1 and w2 must hold the experts of gate (", E, ")");
+        REQUIRE(up.rows % 32 == 0, op, ": the rows of w1, 2H, must be a multiple of 32, got ", up.rows);
+        require_columns(op, "w1", up, K);
+        require_columns(op, "w2", down, z.hidden);
+        REQUIRE(down.rows == K, op, ": w2 must have K (", K, ") rows, got ", down.rows);
+    } else {
+        REQUIRE(l.w1.dim() == 3 && l.w1.size(0) == E && l.w1.size(2) == K && l.w1.size(1) % 2 == 0, op, ": w1 must have shape (E, 2H, K)");
+        z.hidden = l.w1.size(1) / 2;
+        REQUIRE(l.w2.dim() == 3 && l.w2.size(0) == E && l.w2.size(1) == K && l.w2.size(2) == z.hidden, op, ": w2 must have shape (E, K, H)");
+        REQUIRE(l.w1.scalar_type() == l.x.scalar_type() && l.w2.scalar_type() == l.x.scalar_type(), op, ": x, w1 and w2 must have the same dtype");
+        require_contiguous(op, {{"w1", &l.w1}, {"w2", &l.w2}});
+    }
+    REQUIRE(K > 0 && K % 8 == 0 && K <= 1 << 20 && z.hidden > 0 && z.hidden % 8 == 0 && z.hidden <= 1 << 20, op, ": K (", K, ") and H (", z.hidden,
+            ") must be positive multiples of 8 up to 2^20");
+    require_contiguous(op, {{"x", &l.x}, {"gate", &l.gate}});
+    if (l.bias.has_value())
+        REQUIRE(l.bias->scalar_type() == at::kFloat && l.bias->is_contiguous() && l.bias->dim() == 1 && l.bias->size(0) == E, op,
+                ": bias must be a contiguous float32 (E,) tensor");
+    if (placement) {
+        require_same_device(op, {{"x", &l.x}, {"gate", &l.gate}, {"w1", &l.w1}, {"w2", &l.w2}});
+        if (l.w1_scale != nullptr) require_same_device(op, {{"x", &l.x}, {"w1_scale", l.w1_scale}, {"w2_scale", l.w2_scale}});
+        if (l.bias.has_value()) require_same_device(op, {{"x", &l.x}, {"bias", &*l.bias}});
+        require_aligned(op, {{"x", &l.x}, {"gate", &l.gate}, {"w1", &l.w1}, {"w2", &l.w2}}, 16);
+    }
+    return z;
+}
+std::tuple<Tensor, Tensor, Tensor> run_layer(const char *op, const Layer &l) {
+    const LayerSizes z = check_layer(op, l, true);
+    const c10::Device dev = l.x.device();
+    const c10::DeviceGuard guard(dev);
+    const int64_t T = l.x.size(0), E = l.gate.size(0);
+    Tensor out = empty(l.x.sizes(), l.x.scalar_type(), dev), ids = empty({T, l.top_k}, at::kInt, dev), weights = empty({T, l.top_k}, at::kFloat, dev);
+    const Tensor ws = workspace(pmoe_moe_layer_workspace_bytes((int)T, (int)z.hidden, (int)E, (int)l.top_k), dev);
+    check_status(pmoe_moe_layer(l.x.const_data_ptr(), l.gate.const_data_ptr(), l.bias.has_value() ? l.bias->const_data_ptr<float>() : nullptr,
+                                l.w1.const_data_ptr(), l.w1_scale ? l.w1_scale->const_data_ptr() : nullptr, l.w2.const_data_ptr(),
+                                l.w2_scale ? l.w2_scale->const_data_ptr() : nullptr, (int)z.group, out.data_ptr(), ids.data_ptr<int32_t>(),
+                                weights.data_ptr<float>(), (int)T, (int)l.x.size(1), (int)z.hidden, (int)E, (int)l.top_k,
+                                dtype_code(l.x.scalar_type()), ws.data_ptr(), (size_t)ws.numel(), stream_of(dev)));
+    return {out, ids, weights};
+}
+std::tuple<Tensor, Tensor, Tensor> moe_layer(const Tensor &x, const Tensor &gate, const Tensor &w1, const Tensor &w2, int64_t top_k,
+                                             const std::optional<Tensor> &bias) {
+    return run_layer("moe_layer", {x, gate, w1, w2, nullptr, nullptr, top_k, bias});
+}
+std::tuple<Tensor, Tensor, Tensor> moe_layer_int4(const Tensor &x, const Tensor &gate, const Tensor &w1, const Tensor &w1_scale, const Tensor &w2,
+                                                  const Tensor &w2_scale, int64_t top_k, const std::optional<Tensor> &bias) {
+    return run_layer("moe_layer_int4", {x, gate, w1, w2, &w1_scale, &w2_scale, top_k, bias});
+}
+
 void check_expert_offsets(const Tensor &expert_ids, const Tensor &total, int64_t num_experts, bool placement) {
     const char *op = "expert_offsets";
     const Arg ae{"expert_ids", &expert_ids}, at_{"num_tokens_post_padded", &total};
@@ -567,6 +749,11 @@ TORCH_LIBRARY_IMPL(prime_moe, CUDA, m) {
     m.impl("grouped_mm_int8", &grouped_mm_int8);
     m.impl("quantize_int8", &quantize_int8);
     m.impl("expert_offsets", &expert_offsets);
+    m.impl("grouped_mm_int4", &grouped_mm_int4);
+    m.impl("quantize_int4", &quantize_int4);
+    m.impl("dequantize_int4", &dequantize_int4);
+    m.impl("moe_layer", &moe_layer);
+    m.impl("moe_layer_int4", &moe_layer_int4);
 }
 
 TORCH_LIBRARY_IMPL(prime_moe, AutogradCUDA, m) {
@@ -585,6 +772,14 @@ PYBIND11_MODULE(_torch_ops, m) {
     m.def("validate_grouped_mm_int8", [](const Tensor &x, const Tensor &w, const Tensor &xs, const Tensor &ws, const std::optional<Tensor> &o,
                                          at::ScalarType t) { check_grouped_mm_int8(x, w, xs, ws, o, t, false); }, nogil);
     m.def("validate_quantize_int8", [](const Tensor &x) { check_quantize_int8(x, false); }, nogil);
+    m.def("validate_grouped_mm_int4", [](const Tensor &x, const Tensor &w, const Tensor &ws, const std::optional<Tensor> &o) {
+        check_grouped_mm_int4(x, w, ws, o, false); }, nogil);
+    m.def("validate_quantize_int4", [](const Tensor &w, int64_t g, at::ScalarType t) { check_quantize_int4(w, g, t, false); }, nogil);
+    m.def("validate_dequantize_int4", [](const Tensor &q, const Tensor &s, int64_t c) { check_dequantize_int4(q, s, c, false); }, nogil);
+    m.def("validate_moe_layer", [](const Tensor &x, const Tensor &g, const Tensor &w1, const Tensor &w2, int64_t k, const std::optional<Tensor> &b) {
+        check_layer("moe_layer", {x, g, w1, w2, nullptr, nullptr, k, b}, false); }, nogil);
+    m.def("validate_moe_layer_int4", [](const Tensor &x, const Tensor &g, const Tensor &w1, const Tensor &s1, const Tensor &w2, const Tensor &s2,
+                                        int64_t k, const std::optional<Tensor> &b) { check_layer("moe_layer_int4", {x, g, w1, w2, &s1, &s2, k, b}, false); }, nogil);
     m.def("validate_expert_offsets", [](const Tensor &e, const Tensor &n, int64_t k) { check_expert_offsets(e, n, k, false); }, nogil);
     m.def("quantize_mx", &quantize_mx, nogil);
     m.def("route", &route, nogil);

@@ -16,6 +16,9 @@ three ops trace), :func:`quantize_mx`, the OCP-MX quantiser in front of the mxfp
 Next to the fused forward pass, the experts' products on their own, for training, other activations and 8-bit integers:
 :func:`grouped_mm` (differentiable), :func:`grouped_mm_wgrad`, :func:`grouped_mm_int8`, :func:`quantize_int8` and
 :func:`expert_offsets`, which makes their ``offsets`` from a schedule.
+
+For decoding: :func:`moe_layer`, a whole layer for up to 16 tokens, and experts of 4 bits in it (:func:`moe_layer_int4`) and on
+their own (:func:`grouped_mm_int4`; :func:`quantize_int4`, :func:`pack_int4`, :func:`dequantize_int4`).
 """
 from __future__ import annotations
 
@@ -41,6 +44,12 @@ _LIB.define("grouped_mm(Tensor x, Tensor w, Tensor offsets) -> Tensor")
 _LIB.define("grouped_mm_wgrad(Tensor dy, Tensor x, Tensor offsets) -> Tensor")
 _LIB.define("grouped_mm_int8(Tensor x, Tensor w, Tensor x_scale, Tensor w_scale, Tensor? offsets, ScalarType out_dtype) -> Tensor")
 _LIB.define("quantize_int8(Tensor x) -> (Tensor, Tensor)")
+_LIB.define("grouped_mm_int4(Tensor x, Tensor w, Tensor w_scale, Tensor? offsets) -> Tensor")
+_LIB.define("quantize_int4(Tensor w, int group, ScalarType scale_dtype) -> (Tensor, Tensor)")
+_LIB.define("dequantize_int4(Tensor q, Tensor scale, int columns) -> Tensor")
+_LIB.define("moe_layer(Tensor x, Tensor gate, Tensor w1, Tensor w2, int top_k, Tensor? bias) -> (Tensor, Tensor, Tensor)")
+_LIB.define("moe_layer_int4(Tensor x, Tensor gate, Tensor w1, Tensor w1_scale, Tensor w2, Tensor w2_scale, int top_k, Tensor? bias) "
+            "-> (Tensor, Tensor, Tensor)")
 
 
 try:
@@ -62,7 +71,8 @@ except ImportError as _err:
 
     _torch_ops = _Unavailable(str(_err))
     for _op in ("moe_align", "fused_moe_bf16", "fused_moe_mxfp8", "expert_offsets", "grouped_mm", "grouped_mm_wgrad",
-                "grouped_mm_int8", "quantize_int8"):
+                "grouped_mm_int8", "quantize_int8", "grouped_mm_int4", "quantize_int4", "dequantize_int4", "moe_layer",
+                "moe_layer_int4"):
         _LIB.impl(_op, _torch_ops._raise, "CUDA")
 
 
@@ -140,6 +150,30 @@ def _quantize_int8_fake(x):
     return x.new_empty(x.shape, dtype=torch.int8), x.new_empty(x.shape[:-1], dtype=torch.float32)
 
 
+def _grouped_mm_int4_fake(x, w, w_scale, offsets):
+    return x.new_empty((x.shape[0], w.shape[-3] * 16))
+
+
+def _quantize_int4_fake(w, group, scale_dtype):
+    lead, (n, k) = w.shape[:-2], w.shape[-2:]
+    tiles = (k + 127) // 128
+    return (w.new_empty((*lead, n // 16, tiles, 1024), dtype=torch.uint8),
+            w.new_empty((*lead, n // 16, tiles, 16, 128 // group), dtype=scale_dtype))
+
+
+def _dequantize_int4_fake(q, scale, columns):
+    return scale.new_empty((*q.shape[:-3], q.shape[-3] * 16, columns))
+
+
+def _moe_layer_fake(x, gate, w1, w2, top_k, bias):
+    pairs = (x.shape[0], top_k)
+    return torch.empty_like(x), x.new_empty(pairs, dtype=torch.int32), x.new_empty(pairs, dtype=torch.float32)
+
+
+def _moe_layer_int4_fake(x, gate, w1, w1_scale, w2, w2_scale, top_k, bias):
+    return _moe_layer_fake(x, gate, w1, w2, top_k, bias)
+
+
 torch.library.register_fake("prime_moe::moe_align", _moe_align_fake, lib=_LIB)
 torch.library.register_fake("prime_moe::fused_moe_bf16", _fused_moe_bf16_fake, lib=_LIB)
 torch.library.register_fake("prime_moe::fused_moe_mxfp8", _fused_moe_mxfp8_fake, lib=_LIB)
@@ -148,6 +182,11 @@ torch.library.register_fake("prime_moe::grouped_mm", _grouped_mm_fake, lib=_LIB)
 torch.library.register_fake("prime_moe::grouped_mm_wgrad", _grouped_mm_wgrad_fake, lib=_LIB)
 torch.library.register_fake("prime_moe::grouped_mm_int8", _grouped_mm_int8_fake, lib=_LIB)
 torch.library.register_fake("prime_moe::quantize_int8", _quantize_int8_fake, lib=_LIB)
+torch.library.register_fake("prime_moe::grouped_mm_int4", _grouped_mm_int4_fake, lib=_LIB)
+torch.library.register_fake("prime_moe::quantize_int4", _quantize_int4_fake, lib=_LIB)
+torch.library.register_fake("prime_moe::dequantize_int4", _dequantize_int4_fake, lib=_LIB)
+torch.library.register_fake("prime_moe::moe_layer", _moe_layer_fake, lib=_LIB)
+torch.library.register_fake("prime_moe::moe_layer_int4", _moe_layer_int4_fake, lib=_LIB)
 
 
 # ------------------------------------------------------------------------------- public wrappers
@@ -270,7 +309,95 @@ def quantize_int8(x: torch.Tensor):
     return torch.ops.prime_moe.quantize_int8(x)
 
 
+def quantize_int4(w: torch.Tensor, group: int = 128, scale_dtype: torch.dtype = None):
+    """``(q, scale)``: a matrix (N, K), or a stack (..., N, K), to 4 bits with a scale per ``group`` (32, 64 or 128) values of a row.
+
+    A weight stands for ``value * scale``: ``scale`` is the number of ``scale_dtype`` (bfloat16 or float16; ``w``'s own type, and
+    bfloat16 for float32) nearest to ``max(amax * (1 / 7), least)`` in float32, ``least`` being 2**-126 (bfloat16) or 2**-24
+    (float16), ``value`` the integer nearest to ``w / scale`` (exactly, ties to even) from -8 to 7.  A group that holds an infinity or
+    a NaN, or whose scale is beyond the type, gets the scale NaN and zeros.
+
+    ``w`` is contiguous, bfloat16, float16 or float32; N is a multiple of 16, K of ``group``.  ``q`` (..., N / 16, ceil(K / 128),
+    1024) uint8 and ``scale`` (..., N / 16, ceil(K / 128), 16, 128 / group) hold tiles of 16 x 128 in the order the kernels read;
+    :func:`pack_int4` makes them from integers of another quantiser, :func:`dequantize_int4` gives the weights back.
+    """
+    if scale_dtype is None:
+        scale_dtype = torch.bfloat16 if w.dtype == torch.float32 else w.dtype
+    return torch.ops.prime_moe.quantize_int4(w, group, scale_dtype)
+
+
+def pack_int4(values: torch.Tensor, scale: torch.Tensor):
+    """``(q, scale)`` as :func:`quantize_int4` lays them out, from integers ``values`` (..., N, K) int8, -8 to 7, and their scales
+    (..., N, K / group), bfloat16 or float16.  Load-time work, plain torch, on the device of ``values``."""
+    if values.dtype != torch.int8 or values.dim() < 2:
+        raise RuntimeError("pack_int4: values must be int8 (..., N, K)")
+    if scale.dtype not in (torch.bfloat16, torch.float16):
+        raise RuntimeError("pack_int4: scale must be bfloat16 or float16")
+    lead, (n, k) = values.shape[:-2], values.shape[-2:]
+    group = k // scale.shape[-1] if scale.dim() == values.dim() and scale.shape[-1] > 0 else 0
+    if group not in (32, 64, 128) or scale.shape != (*lead, n, k // group) or k % group != 0:
+        raise RuntimeError(f"pack_int4: scale must be (..., N, K / group) with a group of 32, 64 or 128, got {tuple(scale.shape)} "
+                           f"for values {tuple(values.shape)}")
+    if n == 0 or n % 16 != 0:
+        raise RuntimeError(f"pack_int4: N must be a positive multiple of 16, got {n}")
+    if values.numel() > 0 and not (int(values.amin()) >= -8 and int(values.amax()) <= 7):
+        raise RuntimeError("pack_int4: values must lie in -8 .. 7")
+    tiles, per = (k + 127) // 128, 128 // group
+    v = torch.nn.functional.pad(values, (0, tiles * 128 - k)) + 8
+    # axes: [lead, strip, row, tile, 32 columns, 8 columns, column] -> two columns a byte -> [lead, strip, tile, 8 columns, row, 32 columns, byte]
+    v = v.view(torch.uint8).reshape(-1, n // 16, 16, tiles, 4, 4, 8)
+    v = v[..., [0, 4, 1, 5]] | (v[..., [2, 6, 3, 7]] << 4)
+    q = v.permute(0, 1, 3, 5, 2, 4, 6).reshape(*lead, n // 16, tiles, 1024)
+    s = torch.nn.functional.pad(scale, (0, tiles * per - scale.shape[-1])).reshape(-1, n // 16, 16, tiles, per)
+    return q.contiguous(), s.transpose(2, 3).reshape(*lead, n // 16, tiles, 16, per).contiguous()
+
+
+def dequantize_int4(q: torch.Tensor, scale: torch.Tensor, columns: int = None) -> torch.Tensor:
+    """The weights (..., N, K) that ``(q, scale)`` stand for, in the type of ``scale``; for products of many rows, with
+    :func:`grouped_mm` for example.  ``columns``: K, where it is not a multiple of 128."""
+    return torch.ops.prime_moe.dequantize_int4(q, scale, q.shape[-2] * 128 if columns is None else columns)
+
+
+def grouped_mm_int4(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, offsets: torch.Tensor = None) -> torch.Tensor:
+    """:func:`grouped_mm` with weights of 4 bits: ``w``, ``w_scale`` from :func:`quantize_int4` or :func:`pack_int4`, of (E, N, K)
+    weights, or of an (N, K) matrix without ``offsets`` (a dense product).
+
+    Made for few rows per expert, as in decoding: every 32 rows of an expert read its weights again (for many rows:
+    :func:`dequantize_int4`).  ``x`` (M, K) bfloat16 or float16 with a contiguous last dimension, rows a multiple of 8 elements
+    apart, 16-byte aligned; ``w_scale`` of the same type.  Sums in fp32, rounded once; a row of ``x`` that holds an infinity or a
+    NaN comes out as NaN.  No gradients.
+    """
+    return torch.ops.prime_moe.grouped_mm_int4(x, w, w_scale, offsets)
+
+
+def moe_layer(x: torch.Tensor, gate: torch.Tensor, w1: torch.Tensor, w2: torch.Tensor, top_k: int, bias: torch.Tensor = None):
+    """A whole layer of experts for up to 16 tokens: router, experts and weighted sum.  Returns ``(out, topk_ids, topk_weights)``.
+
+    What ``route(x @ gate.T, top_k, bias=bias)`` and a fused forward pass compute, with fp32 logits: ``topk_ids`` (T, top_k) int32,
+    the ``top_k`` largest of ``x @ gate.T + bias``, largest first, ties to the lower index; ``topk_weights`` (T, top_k) float32,
+    softmax over the selected logits; ``out`` (T, K) the sum of ``weight * (w2[e] @ (silu(g) * u))`` with ``g`` and ``u`` the two
+    halves of ``w1[e] @ x``.  ``x`` (T, K), ``gate`` (E, K), ``w1`` (E, 2H, K) with the gate rows first, ``w2`` (E, K, H): contiguous,
+    all bfloat16 or all float16, K and H multiples of 8, at most 512 experts; ``bias`` (E,) float32.  Sums in fp32, one rounding at
+    the end; the same bits every time.  No gradients.  More than 16 tokens: :func:`route` and :func:`fused_moe_bf16`.
+    """
+    return torch.ops.prime_moe.moe_layer(x, gate, w1, w2, top_k, bias)
+
+
+def moe_layer_int4(x: torch.Tensor, gate: torch.Tensor, w1: torch.Tensor, w1_scale: torch.Tensor, w2: torch.Tensor,
+                   w2_scale: torch.Tensor, top_k: int, bias: torch.Tensor = None):
+    """:func:`moe_layer` with experts of 4 bits: ``w1``, ``w1_scale`` and ``w2``, ``w2_scale`` from :func:`quantize_int4` or
+    :func:`pack_int4`, of (E, 2H, K) and (E, K, H) weights with one group size and scales of the type of ``x``.  K and H are
+    multiples of the group (and with it of 16)."""
+    return torch.ops.prime_moe.moe_layer_int4(x, gate, w1, w1_scale, w2, w2_scale, top_k, bias)
+
+
 __all__ = [
+    "dequantize_int4",
+    "grouped_mm_int4",
+    "moe_layer",
+    "moe_layer_int4",
+    "pack_int4",
+    "quantize_int4",
     "expert_offsets",
     "grouped_mm",
     "grouped_mm_int8",

@@ -35,6 +35,11 @@ SIGNATURES = {
     "pmoe_grouped_mm_wgrad": (_c_int, [_c_void_p] * 4 + [_c_int, ctypes.c_int64] + [_c_int] * 2 + [ctypes.c_int64] * 2 + [_c_int, _c_void_p]),
     "pmoe_grouped_mm_int8": (_c_int, [_c_void_p] * 6 + [_c_int, ctypes.c_int64] + [_c_int] * 2 + [ctypes.c_int64] * 3 + [_c_int, _c_void_p]),
     "pmoe_quantize_int8": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 2 + [ctypes.c_int64, _c_int, ctypes.c_int64, _c_void_p]),
+    "pmoe_grouped_mm_int4": (_c_int, [_c_void_p] * 5 + [_c_int, ctypes.c_int64] + [_c_int] * 3 + [ctypes.c_int64, _c_int, _c_void_p]),
+    "pmoe_quantize_int4": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 2 + [_c_int, ctypes.c_int64] + [_c_int] * 2 + [_c_void_p]),
+    "pmoe_dequantize_int4": (_c_int, [_c_void_p] * 3 + [_c_int, ctypes.c_int64] + [_c_int] * 2 + [_c_void_p]),
+    "pmoe_moe_layer_workspace_bytes": (_c_size_t, [_c_int] * 4),
+    "pmoe_moe_layer": (_c_int, [_c_void_p] * 7 + [_c_int] + [_c_void_p] * 3 + [_c_int] * 6 + [_c_void_p, _c_size_t, _c_void_p]),
     "pmoe_set_phase_mask": (None, [_c_int]),
     "pmoe_set_tiles_per_workgroup": (None, [_c_int]),
     "pmoe_set_compute_units": (None, [_c_int]),

@@ -19,7 +19,7 @@ OBJ_DIR = os.path.join(CSRC, "build")
 LIB_NAME = "libprime_moe_hip.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 SOURCES = ["api.hip", "moe_align.hip", "route.hip", "quantize_mx.hip", "fused_moe.hip", "fused_moe_bf16.hip",
-           "grouped_mm.hip", "grouped_int8.hip", "quantize_int8.hip"]
+           "grouped_mm.hip", "grouped_int8.hip", "quantize_int8.hip", "grouped_int4.hip", "quantize_int4.hip", "moe_layer.hip"]
 ARCH = "gfx950"
 EXT_SOURCE = "torch_ops.cpp"
 EXT_PATH = os.path.join(HERE, "_torch_ops.so")
