@@ -1,8 +1,9 @@
 // Products with weights of 4 bits (int4_tile.h): rows by their group's matrix, or by a single one.
 //
-// Bound by the stream of the touched groups' weights.  A workgroup takes one group and 16 U of its weight rows; its waves share
-// the contraction, each in one run of tiles, and add their sums in LDS in the order of the waves.  Rows of x come from the L2 straight
-// into registers, 16 (or 32) at a time; a group with more rows streams its weights again for every 32.
+// Bound by the stream of the touched groups' weights, 64 tokens on 256 experts of 4096 x 7168 by 345 us, 5.7 TB/s.  A workgroup takes one
+// group and 16 U of its weight rows at a time; its waves share the contraction, each in one run of tiles, and add their sums in LDS
+// in the order of the waves.  Rows of x come from the L2 straight into registers, 16 (or 32) at a time; a group with more rows
+// streams its weights again for every 32.
 #include <algorithm>
 
 #include "grouped_host.h"
@@ -13,7 +14,6 @@ namespace {
 using namespace pmoe;
 using namespace pmoe::int4;
 using gmm::RowsArgs;
-using gmm::few::Span;
 
 struct Int4Args {
     RowsArgs rows;      // x, w, out, offsets, n_groups, rows, cols, depth; w_group: bytes of a group's weights
@@ -26,7 +26,7 @@ struct Shared {
     f32x4 sum[WAVES][U * R][64];
 };
 
-template <class T, int GROUP, int U, int R, int WAVES>
+template <class T, int GROUP, int U, int R, int S, int WAVES>
 __device__ __forceinline__ void pass(const Int4Args &a, int group, int row0, int live, int strip0, int strips, Shared<U, 2, WAVES> &sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = gmm::uniform(tid >> 6), r = lane & 15, c = lane >> 4;
     const int tiles = tiles_of(a.rows.depth), t0 = wave * tiles / WAVES, t1 = (wave + 1) * tiles / WAVES;
@@ -40,7 +40,7 @@ __device__ __forceinline__ void pass(const Int4Args &a, int group, int row0, int
 #pragma unroll
     for (int t = 0; t < R; ++t) x[t] = a.rows.x + (row0 + min(16 * t + r, live - 1)) * a.rows.x_pitch;
     f32x4 acc[U][R] = {};
-    dots<T, GROUP, U, R, 2>(acc, w, s, x, t0, t1, a.rows.depth);
+    dots<T, GROUP, U, R, S>(acc, w, s, x, t0, t1, a.rows.depth);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -59,32 +59,108 @@ __device__ __forceinline__ void pass(const Int4Args &a, int group, int row0, int
     __syncthreads();  // the sums may be overwritten
 }
 
-template <class T, int GROUP, int U, int WAVES>
-__global__ __launch_bounds__(64 * WAVES) void grouped_mm_int4_kernel(Int4Args a, int strips, int jobs) {
-    __shared__ Shared<U, 2, WAVES> sh;
-    const int slot = (int)blockIdx.x / jobs, strip0 = ((int)blockIdx.x - slot * jobs) * U;
-    const Span s = gmm::few::find_span<0>(a.rows, slot);
-    if (s.zero) {
-        const int chunks = min(16 * U, a.rows.cols - 16 * strip0) / 8;
-        for (int64_t i = threadIdx.x; i < (int64_t)(s.end - s.begin) * chunks; i += 64 * WAVES)
-            *reinterpret_cast<uint4 *>(a.rows.out + (s.begin + i / chunks) * a.rows.out_pitch + strip0 * 32 + i % chunks * 16) = make_uint4(0, 0, 0, 0);
+// The groups that have rows, in their order: what a group's rows are follows Walk (a group begins at the furthest end in front of it).
+struct Spans {
+    int n, live_rows;
+    int group[gmm::kMaxGroups], begin[gmm::kMaxGroups + 1];
+    int scan[2][8];
+};
+template <int WAVES>
+__device__ __forceinline__ void find_spans(const RowsArgs &a, Spans &s) {
+    constexpr int PER = gmm::kMaxGroups / (64 * WAVES);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    if (a.offsets == nullptr) {
+        if (tid == 0) s.n = 1, s.live_rows = a.rows, s.group[0] = 0, s.begin[0] = 0, s.begin[1] = a.rows;
+        __syncthreads();
         return;
     }
-    for (int row0 = s.begin; row0 < s.end; row0 += 32) {
-        const int live = min(s.end - row0, 32);
-        if (live <= 16) pass<T, GROUP, U, 1, WAVES>(a, s.group, row0, live, strip0, strips, sh);
-        else pass<T, GROUP, U, 2, WAVES>(a, s.group, row0, live, strip0, strips, sh);
+    int end[PER], far = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int g = tid * PER + i;
+        far = max(far, g < a.n_groups ? gmm::group_end(a, g) : 0);
+        end[i] = far;
     }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int v = __shfl_up(far, d, 64);
+        if (lane >= d) far = max(far, v);
+    }
+    if (lane == 63) s.scan[0][wave] = far;
+    __syncthreads();
+    int before = __shfl_up(far, 1, 64);
+    if (lane == 0) before = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+        if (w < wave) before = max(before, s.scan[0][w]);
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        end[i] = max(end[i], before);
+        count += end[i] > (i == 0 ? before : end[i - 1]);
+    }
+    int incl = count;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int v = __shfl_up(incl, d, 64);
+        if (lane >= d) incl += v;
+    }
+    if (lane == 63) s.scan[1][wave] = incl;
+    __syncthreads();
+    int at = incl - count;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w)
+        if (w < wave) at += s.scan[1][w];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int begin = i == 0 ? before : end[i - 1];
+        if (end[i] > begin) s.group[at] = tid * PER + i, s.begin[at] = begin, s.begin[at + 1] = end[i], ++at;
+    }
+    if (tid == 64 * WAVES - 1) {
+        s.n = at;
+        s.live_rows = end[PER - 1];
+    }
+    __syncthreads();
 }
 
+// Resident: a workgroup takes every grid-th job, a group and U strips of its weights, then its part of the rows behind the last group.
+// (A workgroup per job spends more on starting, finding its group and filling its pipeline than on its weights.)
+template <class T, int GROUP, int U, int S, int WAVES, int PER_SIMD>
+__global__ __launch_bounds__(64 * WAVES, PER_SIMD) void grouped_mm_int4_kernel(Int4Args a, int strips, int jobs) {
+    __shared__ Shared<U, 2, WAVES> sh;
+    __shared__ Spans sp;
+    find_spans<WAVES>(a.rows, sp);
+    const int64_t total = (int64_t)sp.n * jobs;
+    for (int64_t job = blockIdx.x; job < total; job += gridDim.x) {
+        const int slot = (int)(job / jobs), strip0 = (int)(job - (int64_t)slot * jobs) * U;
+        const int group = gmm::uniform(sp.group[slot]), begin = gmm::uniform(sp.begin[slot]), end = gmm::uniform(sp.begin[slot + 1]);
+        for (int row0 = begin; row0 < end; row0 += 32) {
+            const int live = min(end - row0, 32);
+            if (live <= 16) pass<T, GROUP, U, 1, S, WAVES>(a, group, row0, live, strip0, strips, sh);
+            else pass<T, GROUP, U, 2, (S + 1) / 2, WAVES>(a, group, row0, live, strip0, strips, sh);
+        }
+    }
+    const int64_t from = sp.live_rows * a.rows.out_pitch / 16, to = a.rows.rows * a.rows.out_pitch / 16;
+    for (int64_t i = from + (int64_t)blockIdx.x * 64 * WAVES + threadIdx.x; i < to; i += (int64_t)gridDim.x * 64 * WAVES)
+        reinterpret_cast<uint4 *>(a.rows.out)[i] = make_uint4(0, 0, 0, 0);
+}
+
+template <class T, int GROUP, int U, int S, int WAVES, int PER_SIMD>
+int launch_as(const Int4Args &a, int64_t slots, hipStream_t stream) {
+    const int strips = a.rows.cols / 16, jobs = (strips + U - 1) / U;
+    const int64_t grid = std::min<int64_t>(jobs * slots, resident_grid() * (4 * PER_SIMD / WAVES));
+    hipLaunchKernelGGL((grouped_mm_int4_kernel<T, GROUP, U, S, WAVES, PER_SIMD>), dim3((uint32_t)grid), dim3(64 * WAVES), 0, stream, a, strips, jobs);
+    return check_launch("grouped_mm_int4 launch");
+}
 template <class T, int GROUP>
 int launch(const Int4Args &a, hipStream_t stream) {
-    constexpr int U = 1, WAVES = 8;
-    const int strips = a.rows.cols / 16, jobs = (strips + U - 1) / U;
-    const int64_t slots = std::min(a.rows.rows, a.rows.n_groups) + (a.rows.offsets != nullptr ? 1 : 0);
-    PMOE_REQUIRE(jobs * slots * (64 * WAVES) <= UINT32_MAX, "grouped_mm_int4: too many tiles");
-    hipLaunchKernelGGL((grouped_mm_int4_kernel<T, GROUP, U, WAVES>), dim3((uint32_t)(jobs * slots)), dim3(64 * WAVES), 0, stream, a, strips, jobs);
-    return check_launch("grouped_mm_int4 launch");
+    const int64_t slots = std::min(a.rows.rows, a.rows.n_groups), strips = a.rows.cols / 16;
+    // A wave with more strips reads x less often, which costs as many loads as four strips of weights; few strips are shared by
+    // more waves instead, so that all CUs have some.  Strips of one, two, four, us: 256 (a row through 4096 x 7168) 7.2, 9.0, 13;
+    // 1024 (8 of 128 experts of 2048 x 768) 6.8, 5.8, 7.2; 7900 (16 tokens on 128 experts of 1536 x 2048) 50, 38, 33.
+    if (strips * slots <= 2 * resident_grid()) return launch_as<T, GROUP, 1, 2, 8, 4>(a, slots, stream);
+    if (strips * slots <= 4 * resident_grid()) return launch_as<T, GROUP, 2, 1, 8, 4>(a, slots, stream);
+    return launch_as<T, GROUP, 4, 1, 4, 3>(a, slots, stream);
 }
 template <class T>
 int launch(const Int4Args &a, int group, hipStream_t stream) {

@@ -1,8 +1,7 @@
 // To 4 bits and back (layout: int4_tile.h).
 //
 // scale = the 16-bit number nearest to max(amax c, least) with c = 1 / 7 in fp32; q = the integer nearest to the exact quotient of
-// value and scale, ties to even, from -8 to 7: the remainder value - q scale, which an fma gives without rounding, corrects the first
-// guess value (1 / scale), which is off by one at most.  A group with an infinity, a NaN, or a scale beyond the 16-bit type
+// value and scale, ties to even, from -8 to 7.  A group with an infinity, a NaN, or a scale beyond the 16-bit type
 // gets the scale NaN and q = 0.
 //
 // Bound by memory.  A wave takes a tile: its loads are 64 contiguous bytes of 16 rows, whole lines over four of them, its stores 1 KB.
@@ -17,31 +16,56 @@ using namespace pmoe;
 using namespace pmoe::int4;
 
 struct F32 {};
+// Eight values of a lane, and the largest magnitude among them as the bits of a float: infinity and the NaNs are above all numbers.
 template <class FROM>
 struct Load {
     static constexpr int kBytes = 2;
-    static __device__ __forceinline__ void eight(const char *p, float (&v)[8]) {
+    static constexpr bool kShort = true;  // 11 bits of mantissa at most
+    static __device__ __forceinline__ uint32_t eight(const char *p, float (&v)[8]) {
+        typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
         const uint4 u = *reinterpret_cast<const uint4 *>(p);
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        u16x2 m = {0, 0};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[2 * i] = Num<FROM>::to_f32((uint16_t)w[i]), v[2 * i + 1] = Num<FROM>::to_f32((uint16_t)(w[i] >> 16));
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = Num<FROM>::to_f32((uint16_t)w[i]), v[2 * i + 1] = Num<FROM>::to_f32((uint16_t)(w[i] >> 16));
+            m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+        }
+        return __float_as_uint(Num<FROM>::to_f32(m[0] > m[1] ? m[0] : m[1]));
     }
 };
 template <>
 struct Load<F32> {
     static constexpr int kBytes = 4;
-    static __device__ __forceinline__ void eight(const char *p, float (&v)[8]) {
+    static constexpr bool kShort = false;
+    static __device__ __forceinline__ uint32_t eight(const char *p, float (&v)[8]) {
         const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
         v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        uint32_t m = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = max(m, __float_as_uint(v[k]) & 0x7fffffffu);
+        return m;
     }
 };
 
-__device__ __forceinline__ int nearest(float x, float scale, float inv) {
-    float q = rintf(x * inv);
-    const float rest = fmaf(-q, scale, x), twice = 2.0f * fabsf(rest);
-    const bool odd = ((int)q & 1) != 0;
-    if (twice > scale || (twice == scale && odd)) q += copysignf(1.0f, rest);
-    return (int)fminf(fmaxf(q, -8.0f), 7.0f);
+// The integer nearest to x / scale, ties to even, from -8 to 7; plus 8, in the lowest bits of kBias + it.
+// The quotient is corrected by its remainder, which an fma gives without rounding.  For 16-bit values that leaves the exact
+// quotient where it is half way between two integers, and nothing else is near: with up to 11 bits of mantissa in both, a
+// quotient that is not half an odd number is 2^-13 or more away from it.  A float's may be nearer than its last place: there the
+// remainder of the integer decides.
+constexpr uint32_t kBias = 0x4b400000u;  // bits of 1.5 2^23, whose last place is 1
+template <bool SHORT>
+__device__ __forceinline__ uint32_t nearest(float x, float scale, float inv) {
+    float q = x * inv;
+    if constexpr (SHORT) {
+        q = fmaf(fmaf(-q, scale, x), inv, q);
+    } else {
+        q = rintf(q);
+        const float rest = fmaf(-q, scale, x), twice = 2.0f * fabsf(rest);
+        const bool odd = ((int)q & 1) != 0;
+        if (twice > scale || (twice == scale && odd)) q += copysignf(1.0f, rest);
+    }
+    return __float_as_uint(__builtin_amdgcn_fmed3f(q, -8.0f, 7.0f) + 12582920.0f);
 }
 
 // Position of column k (0 .. 7) of a dword, in nibbles.
@@ -58,17 +82,16 @@ __global__ __launch_bounds__(256) void quantize_int4_kernel(const char *__restri
         const int col0 = (int)(tile - strip * tiles) * kTileCols;
         const char *p = src + ((strip * 16 + r) * cols + col0 + 8 * c) * Load<FROM>::kBytes;
         float v[4][8] = {};
+        uint32_t peaks[4] = {};
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (col0 + 32 * j < cols) Load<FROM>::eight(p + 32 * j * Load<FROM>::kBytes, v[j]);
+            if (col0 + 32 * j < cols) peaks[j] = Load<FROM>::eight(p + 32 * j * Load<FROM>::kBytes, v[j]);
         uint32_t out[4];
 #pragma unroll
         for (int g = 0; g < Sc::kCount; ++g) {
-            uint32_t peak = 0;  // largest magnitude as its bits: infinity and the NaNs are above all numbers
+            uint32_t peak = peaks[g * PER];
 #pragma unroll
-            for (int j = 0; j < PER; ++j)
-#pragma unroll
-                for (int k = 0; k < 8; ++k) peak = max(peak, __float_as_uint(v[g * PER + j][k]) & 0x7fffffffu);
+            for (int j = 1; j < PER; ++j) peak = max(peak, peaks[g * PER + j]);
             peak = max(peak, (uint32_t)__shfl_xor((int)peak, 16, 64));
             peak = max(peak, (uint32_t)__shfl_xor((int)peak, 32, 64));
             uint16_t s16 = Num<T>::from_f32(fmaxf(__uint_as_float(peak) * (1.0f / 7.0f), Num<T>::kLeastScale));
@@ -77,10 +100,13 @@ __global__ __launch_bounds__(256) void quantize_int4_kernel(const char *__restri
             const float scale = Num<T>::to_f32(s16), inv = 1.0f / scale;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-                uint32_t word = 0;
+                uint32_t word = 0, bias = 0;  // (the sum of the biases leaves in one subtraction)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) word |= (uint32_t)(fine ? nearest(v[g * PER + j][k], scale, inv) + 8 : 8) << (4 * nibble(k));
-                out[g * PER + j] = word;
+                for (int k = 0; k < 8; ++k) {
+                    word += nearest<Load<FROM>::kShort>(v[g * PER + j][k], scale, inv) << (4 * nibble(k));
+                    bias += kBias << (4 * nibble(k));
+                }
+                out[g * PER + j] = fine ? word - bias : 0x88888888u;
             }
             if (c == 0) reinterpret_cast<uint16_t *>(scales + tile * Sc::kBytes)[r * Sc::kCount + g] = inside ? s16 : 0;
         }
@@ -104,9 +130,15 @@ __global__ __launch_bounds__(256) void dequantize_int4_kernel(const char *__rest
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float s = Num<T>::to_f32(sc.v[j / (GROUP / 32)]);
+            // (24 + q) s - 24 s: both products are exact, and so is the difference
+            const i32x4 wide = Num<T>::wide(w[j]);
+            const float less = -24.0f * s;
             float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = (float)((int)(w[j] >> (4 * nibble(k)) & 15u) - 8) * s;
+            for (int k = 0; k < 4; ++k) {
+                v[2 * k] = fmaf(Num<T>::to_f32((uint16_t)wide[k]), s, less);
+                v[2 * k + 1] = fmaf(Num<T>::to_f32((uint16_t)((uint32_t)wide[k] >> 16)), s, less);
+            }
             const uint2 lo = gmm::Pack<T>::four(v[0], v[1], v[2], v[3]), hi = gmm::Pack<T>::four(v[4], v[5], v[6], v[7]);
             if (col0 + 32 * j < cols) *reinterpret_cast<uint4 *>(p + 64 * j) = make_uint4(lo.x, lo.y, hi.x, hi.y);
         }
