@@ -1,9 +1,8 @@
 // Products with weights of 4 bits (int4_tile.h): rows by their group's matrix, or by a single one.
 //
-// Bound by the stream of the touched groups' weights, 64 tokens on 256 experts of 4096 x 7168 by 345 us, 5.7 TB/s.  A workgroup takes one
+// Bound by the stream of the touched groups' weights, 64 tokens on 256 experts of 4096 x 7168 by 417 us, 4.8 TB/s (345 where x is constant).  A workgroup takes one
 // group and 16 U of its weight rows at a time; its waves share the contraction, each in one run of tiles, and add their sums in LDS
-// in the order of the waves.  Rows of x come from the L2 straight into registers, 16 (or 32) at a time; a group with more rows
-// streams its weights again for every 32.
+// in the order of the waves.  Rows of x come 16 (or 32) at a time; a group with more rows streams its weights again for them.
 #include <algorithm>
 
 #include "grouped_host.h"
@@ -21,26 +20,27 @@ struct Int4Args {
     int64_t scale_group;
 };
 
-template <int U, int R, int WAVES>
-struct Shared {
+template <int U, int R, int S, int WAVES>
+union Shared {
     f32x4 sum[WAVES][U * R][64];
+    char rows[WAVES][Rows<R, S>::kBytes];
 };
 
 template <class T, int GROUP, int U, int R, int S, int WAVES>
-__device__ __forceinline__ void pass(const Int4Args &a, int group, int row0, int live, int strip0, int strips, Shared<U, 2, WAVES> &sh) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = gmm::uniform(tid >> 6), r = lane & 15, c = lane >> 4;
+__device__ __forceinline__ void pass(const Int4Args &a, int group, int row0, int live, int strip0, int strips, Shared<U, R, S, WAVES> &sh) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = gmm::uniform(tid >> 6);
     const int tiles = tiles_of(a.rows.depth), t0 = wave * tiles / WAVES, t1 = (wave + 1) * tiles / WAVES;
-    const char *w[U], *s[U], *x[R];
+    const char *w[U], *s[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int64_t strip = min(strip0 + u, strips - 1);
         w[u] = a.rows.w + group * a.rows.w_group + strip * tiles * kTileBytes;
         s[u] = a.scale + group * a.scale_group + strip * tiles * TileScales<GROUP>::kBytes;
     }
-#pragma unroll
-    for (int t = 0; t < R; ++t) x[t] = a.rows.x + (row0 + min(16 * t + r, live - 1)) * a.rows.x_pitch;
+    const char *const x = a.rows.x + row0 * a.rows.x_pitch;
     f32x4 acc[U][R] = {};
-    dots<T, GROUP, U, R, S>(acc, w, s, x, t0, t1, a.rows.depth);
+    dots<T, GROUP, U, R, S>(acc, w, s, [&](int q) { return x + q * a.rows.x_pitch; }, live, t0, t1, a.rows.depth, sh.rows[wave]);
+    __syncthreads();  // the sums lie where the rows were
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -125,42 +125,42 @@ __device__ __forceinline__ void find_spans(const RowsArgs &a, Spans &s) {
 
 // Resident: a workgroup takes every grid-th job, a group and U strips of its weights, then its part of the rows behind the last group.
 // (A workgroup per job spends more on starting, finding its group and filling its pipeline than on its weights.)
-template <class T, int GROUP, int U, int S, int WAVES, int PER_SIMD>
+template <class T, int GROUP, int U, int R, int S, int WAVES, int PER_SIMD>
 __global__ __launch_bounds__(64 * WAVES, PER_SIMD) void grouped_mm_int4_kernel(Int4Args a, int strips, int jobs) {
-    __shared__ Shared<U, 2, WAVES> sh;
+    __shared__ __attribute__((aligned(1024))) Shared<U, R, S, WAVES> sh;
     __shared__ Spans sp;
     find_spans<WAVES>(a.rows, sp);
     const int64_t total = (int64_t)sp.n * jobs;
     for (int64_t job = blockIdx.x; job < total; job += gridDim.x) {
         const int slot = (int)(job / jobs), strip0 = (int)(job - (int64_t)slot * jobs) * U;
         const int group = gmm::uniform(sp.group[slot]), begin = gmm::uniform(sp.begin[slot]), end = gmm::uniform(sp.begin[slot + 1]);
-        for (int row0 = begin; row0 < end; row0 += 32) {
-            const int live = min(end - row0, 32);
-            if (live <= 16) pass<T, GROUP, U, 1, S, WAVES>(a, group, row0, live, strip0, strips, sh);
-            else pass<T, GROUP, U, 2, (S + 1) / 2, WAVES>(a, group, row0, live, strip0, strips, sh);
-        }
+        for (int row0 = begin; row0 < end; row0 += 16 * R) pass<T, GROUP, U, R, S, WAVES>(a, group, row0, min(end - row0, 16 * R), strip0, strips, sh);
     }
     const int64_t from = sp.live_rows * a.rows.out_pitch / 16, to = a.rows.rows * a.rows.out_pitch / 16;
     for (int64_t i = from + (int64_t)blockIdx.x * 64 * WAVES + threadIdx.x; i < to; i += (int64_t)gridDim.x * 64 * WAVES)
         reinterpret_cast<uint4 *>(a.rows.out)[i] = make_uint4(0, 0, 0, 0);
 }
 
-template <class T, int GROUP, int U, int S, int WAVES, int PER_SIMD>
+template <class T, int GROUP, int U, int R, int S, int WAVES, int PER_SIMD>
 int launch_as(const Int4Args &a, int64_t slots, hipStream_t stream) {
     const int strips = a.rows.cols / 16, jobs = (strips + U - 1) / U;
     const int64_t grid = std::min<int64_t>(jobs * slots, resident_grid() * (4 * PER_SIMD / WAVES));
-    hipLaunchKernelGGL((grouped_mm_int4_kernel<T, GROUP, U, S, WAVES, PER_SIMD>), dim3((uint32_t)grid), dim3(64 * WAVES), 0, stream, a, strips, jobs);
+    hipLaunchKernelGGL((grouped_mm_int4_kernel<T, GROUP, U, R, S, WAVES, PER_SIMD>), dim3((uint32_t)grid), dim3(64 * WAVES), 0, stream, a, strips, jobs);
     return check_launch("grouped_mm_int4 launch");
 }
 template <class T, int GROUP>
 int launch(const Int4Args &a, hipStream_t stream) {
     const int64_t slots = std::min(a.rows.rows, a.rows.n_groups), strips = a.rows.cols / 16;
-    // A wave with more strips reads x less often, which costs as many loads as four strips of weights; few strips are shared by
-    // more waves instead, so that all CUs have some.  Strips of one, two, four, us: 256 (a row through 4096 x 7168) 7.2, 9.0, 13;
-    // 1024 (8 of 128 experts of 2048 x 768) 6.8, 5.8, 7.2; 7900 (16 tokens on 128 experts of 1536 x 2048) 50, 38, 33.
-    if (strips * slots <= 2 * resident_grid()) return launch_as<T, GROUP, 1, 2, 8, 4>(a, slots, stream);
-    if (strips * slots <= 4 * resident_grid()) return launch_as<T, GROUP, 2, 1, 8, 4>(a, slots, stream);
-    return launch_as<T, GROUP, 4, 1, 4, 3>(a, slots, stream);
+    // Rows are taken 16 at a time, or 32 where the average group has more (27 rows x 28672 x 4096: 21 us instead of 30; the registers
+    // of 32 rows cost those with fewer half of their waves: 16 tokens on 128 experts of 1536 x 2048 47 us instead of 31).
+    // A wave with more strips reads x less often; few strips are shared by more waves instead, so that all CUs have some.  Strips
+    // of one, two, four, us: 256 (a row through 4096 x 7168) 7.8, 9.8, 13; 1024 (8 of 128 experts of 2048 x 768) 7.5, 6.2, 6.5; 7900 (16
+    // tokens on 128 experts of 1536 x 2048) 49, 38, 31.
+    const int64_t all = strips * slots, cus = resident_grid();
+    if (a.rows.rows > 16 * (int64_t)a.rows.n_groups) return all <= 2 * cus ? launch_as<T, GROUP, 1, 2, 1, 8, 2>(a, slots, stream) : launch_as<T, GROUP, 4, 2, 1, 4, 2>(a, slots, stream);
+    if (all <= 2 * cus) return launch_as<T, GROUP, 1, 1, 2, 8, 4>(a, slots, stream);
+    if (all <= 4 * cus) return launch_as<T, GROUP, 2, 1, 1, 8, 4>(a, slots, stream);
+    return launch_as<T, GROUP, 4, 1, 1, 4, 4>(a, slots, stream);
 }
 template <class T>
 int launch(const Int4Args &a, int group, hipStream_t stream) {

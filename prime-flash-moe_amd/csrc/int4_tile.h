@@ -80,48 +80,88 @@ struct TileScales {
     }
 };
 
-// S tiles of U strips and of the rows of x beside them, in registers.
-template <class T, int GROUP, int U, int R, int S>
-struct Batch {
-    using Sc = TileScales<GROUP>;
-    i32x4 w[S][U], x[S][R][4];
-    Sc sc[S][U];
+// Rows of x on their way to a wave: S tiles of up to 16 R rows, in LDS of the wave's own.  A load of the wave is 1 KB, four rows
+// of a tile, where the operands of its matrix instructions would be 64 bytes of 16 rows each, most of them the same row again: one
+// load per tile instead of four for up to four rows.  Row q of tile i is 256 bytes, its chunk of 16 bytes k in slot k ^ q % 16: the
+// reads of 16 rows cover all banks.
+template <int R, int S>
+struct Rows {
+    i32x4 v[S * R * 4];
+    // `x(q)`: begins row q; `n`: rows, from 1 to 16 R (both wave-uniform but for the lane's q).
+    template <class X>
+    __device__ __forceinline__ void load(X x, int n, int t, int t1, int k) {
+        const int lane = threadIdx.x & 63, sub = lane >> 4, e = (lane & 15) * 8;
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+            if (i == 0 || t + i < t1) {
+                const int col = (t + i) * kTileCols + e;
+#pragma unroll
+                for (int g = 0; g < R * 4; ++g)
+                    if (g == 0 || 4 * g < n) {
+                        v[i * R * 4 + g] = i32x4{0, 0, 0, 0};
+                        if (col < k) v[i * R * 4 + g] = *reinterpret_cast<const i32x4 *>(x(min(4 * g + sub, n - 1)) + (int64_t)col * 2);
+                    }
+            }
+    }
+    __device__ __forceinline__ void store(char *lds, int n, int t, int t1) const {
+        const int lane = threadIdx.x & 63, sub = lane >> 4;
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+            if (i == 0 || t + i < t1) {
+#pragma unroll
+                for (int g = 0; g < R * 4; ++g)
+                    if (g == 0 || 4 * g < n)
+                        *reinterpret_cast<i32x4 *>(lds + ((i * 16 * R + 4 * g + sub) * 256 + (((lane & 15) ^ (4 * g + sub)) & 15) * 16)) = v[i * R * 4 + g];
+            }
+    }
+    // Operand of row 16 q + r, columns 32 j + 8 c .. + 7 of tile i.
+    static __device__ __forceinline__ i32x4 read(const char *lds, int n, int i, int q, int j) {
+        const int lane = threadIdx.x & 63, row = min(16 * q + (lane & 15), n - 1);
+        return *reinterpret_cast<const i32x4 *>(lds + (i * 16 * R + row) * 256 + (((4 * j + (lane >> 4)) ^ row) & 15) * 16);
+    }
+    static constexpr int kBytes = S * R * 16 * 256;
+};
 
-    __device__ __forceinline__ void load(const char *const (&wp)[U], const char *const (&sp)[U], const char *const (&xp)[R], int t, int t1, int k) {
-        const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+// acc[u][q] += n rows of x times the weights of tiles t0 .. t1 - 1 of U strips (16 weight rows each), for one wave.  Lane l, r = l %
+// 16, c = l / 16: `w[u]`, `s[u]` begin strip u.  acc[u][q][i]: weight row r, row 16 q + 4 c + i of x (any of the n where there are fewer).
+// `k`: columns; nothing of x is read behind them.  `lds`: Rows<R, S>::kBytes of the wave's own.  S: tiles whose loads are in flight
+// together; what hides the rest of their latency is other waves.
+template <class T, int GROUP, int U, int R, int S, class X>
+__device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[U], const char *const (&s)[U], X x, int n, int t0, int t1, int k, char *lds) {
+    using Sc = TileScales<GROUP>;
+    constexpr int PER = GROUP / 32;
+    const int lane = threadIdx.x & 63, r = lane & 15;
+    const i32x4 minus = {(int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24};
+    for (int t = t0; t < t1; t += S) {
+        i32x4 wv[S][U];
+        Sc sc[S][U];
+        Rows<R, S> rows;
+        rows.load(x, n, t, t1, k);
 #pragma unroll
         for (int i = 0; i < S; ++i)
             if (i == 0 || t + i < t1) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
-                    w[i][u] = load_once16(wp[u] + (int64_t)(t + i) * kTileBytes + lane * 16);
-                    sc[i][u].load(sp[u] + (int64_t)(t + i) * Sc::kBytes, r);
+                    wv[i][u] = load_once16(w[u] + (int64_t)(t + i) * kTileBytes + lane * 16);
+                    sc[i][u].load(s[u] + (int64_t)(t + i) * Sc::kBytes, r);
                 }
-                const int left = k - (t + i) * kTileCols;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int q = 0; q < R; ++q) {
-                        x[i][q][j] = i32x4{0, 0, 0, 0};
-                        if (32 * j < left) x[i][q][j] = *reinterpret_cast<const i32x4 *>(xp[q] + (int64_t)(t + i) * 256 + j * 64 + c * 16);
-                    }
             }
-    }
-
-    __device__ __forceinline__ void multiply(f32x4 (&acc)[U][R], int t, int t1) const {
-        const i32x4 minus = {(int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24};
-        constexpr int PER = GROUP / 32;
+        rows.store(lds, n, t, t1);
 #pragma unroll
         for (int i = 0; i < S; ++i)
             if (i == 0 || t + i < t1) {
 #pragma unroll
                 for (int g = 0; g < Sc::kCount; ++g) {
+                    i32x4 xv[R][PER];
                     f32x4 less[R];  // -24 times the sums of the group's part of x
 #pragma unroll
                     for (int q = 0; q < R; ++q) {
                         less[q] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                        for (int j = g * PER; j < (g + 1) * PER; ++j) less[q] = gmm::few::Mini<T>::mfma(x[i][q][j], minus, less[q]);
+                        for (int j = 0; j < PER; ++j) {
+                            xv[q][j] = Rows<R, S>::read(lds, n, i, q, g * PER + j);
+                            less[q] = gmm::few::Mini<T>::mfma(xv[q][j], minus, less[q]);
+                        }
                     }
 #pragma unroll
                     for (int u = 0; u < U; ++u) {
@@ -129,10 +169,10 @@ struct Batch {
 #pragma unroll
                         for (int q = 0; q < R; ++q) sum[q] = less[q];
 #pragma unroll
-                        for (int j = g * PER; j < (g + 1) * PER; ++j) {
-                            const i32x4 b = Num<T>::wide((uint32_t)w[i][u][j]);
+                        for (int j = 0; j < PER; ++j) {
+                            const i32x4 b = Num<T>::wide((uint32_t)wv[i][u][g * PER + j]);
 #pragma unroll
-                            for (int q = 0; q < R; ++q) sum[q] = gmm::few::Mini<T>::mfma(x[i][q][j], b, sum[q]);
+                            for (int q = 0; q < R; ++q) sum[q] = gmm::few::Mini<T>::mfma(xv[q][j], b, sum[q]);
                         }
                         const float f = Num<T>::to_f32(sc[i][u].v[g]);
 #pragma unroll
@@ -142,22 +182,6 @@ struct Batch {
                     }
                 }
             }
-    }
-};
-
-// acc[u][t] += rows of x times the weights of tiles t0 .. t1 - 1 of U strips (16 weight rows each), for one wave.  Lane l, r = l %
-// 16, c = l / 16: `w[u]`, `s[u]` begin strip u; `x[t]` is row 16 t + r of x (any row that can be read, where there are fewer).
-// acc[u][t][i]: weight row r, row 16 t + 4 c + i of x.  `k`: columns, a multiple of 32; nothing of x is read behind them.
-// S: tiles whose loads are in flight together; what hides the
-// rest of their latency is other waves.  (Two batches by turns, the one loaded while the other is multiplied, take the registers of
-// half of the waves: 64 tokens on 256 experts of 4096 x 7168 370 us instead of 345.)
-template <class T, int GROUP, int U, int R, int S>
-__device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[U], const char *const (&s)[U], const char *const (&x)[R], int t0,
-                                     int t1, int k) {
-    Batch<T, GROUP, U, R, S> b;
-    for (int t = t0; t < t1; t += S) {
-        b.load(w, s, x, t, t1, k);
-        b.multiply(acc, t, t1);
     }
 }
 

@@ -176,15 +176,19 @@ __device__ __forceinline__ uint32_t split(float v) {
     return hi | (uint32_t)lo << 16;
 }
 
+using Rows = int4::Rows<1, 1>;
 struct UpSums {
     float part[kWaves][2][kMaxTokens][kUpCols];  // [part of the contraction][gate, up][row][column]
 };
 struct DownSums {
     float y[kWaves][kMaxTokens][16];  // [wave][token][column]
 };
-union Sums {
-    UpSums up;
-    DownSums down;
+struct Sums {
+    union {
+        UpSums up;
+        DownSums down;
+    };
+    char rows[kWaves][Rows::kBytes];  // rows of x or of the activation on their way to a wave
 };
 
 // What the 16 columns of an up job have in `parts` parts -> activation.
@@ -210,7 +214,8 @@ struct Wide {
     static constexpr int kDownCols = 8;
 
     // Waves: four groups of four columns (a column's gate and up row on 16 lanes) x two halves of the contraction.
-    static __device__ __forceinline__ void up(const Args &a, const Plan &p, UpSums &sums, int u, int strip) {
+    static __device__ __forceinline__ void up(const Args &a, const Plan &p, Sums &sh, int u, int strip) {
+        UpSums &sums = sh.up;
         const int lane = threadIdx.x & 63, wave = gmm::uniform(threadIdx.x >> 6), quad = wave & 3, half = wave >> 2, sub = lane >> 4;
         const int steps = (a.K + 127) / 128, s0 = half * steps / 2, s1 = (half + 1) * steps / 2;
         const int c = 4 * quad + sub, col = min(strip * kUpCols + c, a.H - 1);
@@ -236,12 +241,12 @@ struct Wide {
     }
 
     // sums[.][.] += expert u's share, steps part / parts, of 8 columns of out.
-    static __device__ __forceinline__ void down(const Args &a, const Plan &p, float (&y)[kMaxTokens][16], int u, int strip, int part, int parts) {
+    static __device__ __forceinline__ void down(const Args &a, const Plan &p, float (&y)[kMaxTokens][16], char *rows, int u, int strip, int part, int parts) {
         const int lane = threadIdx.x & 63, sub = lane >> 4;
         const int steps = (a.H + 127) / 128, s0 = part * steps / parts, s1 = (part + 1) * steps / parts;
         const uint32_t tokens = gmm::uniform(p.tokens[u]);
-        const char *rows = a.w2 + (int64_t)p.expert[u] * a.K * a.H * 2;
-        const char *const w[2] = {rows + (int64_t)(strip * 8 + sub) * a.H * 2, rows + (int64_t)(strip * 8 + 4 + sub) * a.H * 2};
+        const char *w2 = a.w2 + (int64_t)p.expert[u] * a.K * a.H * 2;
+        const char *const w[2] = {w2 + (int64_t)(strip * 8 + sub) * a.H * 2, w2 + (int64_t)(strip * 8 + 4 + sub) * a.H * 2};
         auto some = [&](auto n, int row0) {
             constexpr int N = decltype(n)::value;
             const int last = __popc(tokens) - 1;
@@ -277,8 +282,10 @@ struct Narrow {
     static constexpr int kDownCols = 16;
 
     // The waves share the contraction; a strip of gate rows and the matching one of up rows.
-    static __device__ __forceinline__ void up(const Args &a, const Plan &p, UpSums &sums, int u, int strip) {
+    static __device__ __forceinline__ void up(const Args &a, const Plan &p, Sums &sh, int u, int strip) {
+        UpSums &sums = sh.up;
         const int lane = threadIdx.x & 63, wave = gmm::uniform(threadIdx.x >> 6), r = lane & 15, c = lane >> 4;
+        char *const rows = sh.rows[wave];
         const int tiles = int4::tiles_of(a.K), t0 = wave * tiles / kWaves, t1 = (wave + 1) * tiles / kWaves, strips = a.H / 16;
         const uint32_t tokens = gmm::uniform(p.tokens[u]);
         const int last = __popc(tokens) - 1;
@@ -286,16 +293,16 @@ struct Narrow {
         const int64_t first = (int64_t)p.expert[u] * 2 * strips + strip;
         const char *const w[2] = {a.w1 + first * tiles * int4::kTileBytes, a.w1 + (first + strips) * tiles * int4::kTileBytes};
         const char *const s[2] = {a.w1_scale + first * tiles * SB, a.w1_scale + (first + strips) * tiles * SB};
-        const char *const x[1] = {a.x + (int64_t)token_of(tokens, min(r, last)) * a.K * 2};
         f32x4 acc[2][1] = {};
-        int4::dots<T, GROUP, 2, 1, 2>(acc, w, s, x, t0, t1, a.K);
+        int4::dots<T, GROUP, 2, 1, 1>(acc, w, s, [&](int q) { return a.x + (int64_t)token_of(tokens, q) * a.K * 2; }, last + 1, t0, t1, a.K, rows);
+        __syncthreads();  // the sums may lie where the rows were
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums.part[wave][0][4 * c + i][r] = acc[0][0][i], sums.part[wave][1][4 * c + i][r] = acc[1][0][i];
         __syncthreads();
         finish_up<T>(a, p, sums, u, strip * kUpCols, kWaves);
     }
 
-    static __device__ __forceinline__ void down(const Args &a, const Plan &p, float (&y)[kMaxTokens][16], int u, int strip, int part, int parts) {
+    static __device__ __forceinline__ void down(const Args &a, const Plan &p, float (&y)[kMaxTokens][16], char *rows, int u, int strip, int part, int parts) {
         const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
         const int tiles = int4::tiles_of(a.H), t0 = part * tiles / parts, t1 = (part + 1) * tiles / parts;
         const uint32_t tokens = gmm::uniform(p.tokens[u]);
@@ -306,10 +313,12 @@ struct Narrow {
         const char *const s[1] = {a.w2_scale + first * tiles * SB};
         // row m of the matrix instructions: value (m even) or rest of the expert's row m / 2
         for (int row0 = 0; row0 <= last; row0 += 8) {
-            const int mine = token_of(tokens, min(row0 + r / 2, last));
-            const char *const x[1] = {a.act + ((int64_t)(mine * a.top_k + p.slot[u][mine]) * 2 + (r & 1)) * a.act_pitch};
             f32x4 acc[1][1] = {};
-            int4::dots<T, GROUP, 1, 1, 2>(acc, w, s, x, t0, t1, a.H);
+            auto row = [&](int q) {
+                const int t = token_of(tokens, row0 + q / 2);
+                return a.act + ((int64_t)(t * a.top_k + p.slot[u][t]) * 2 + (q & 1)) * a.act_pitch;
+            };
+            int4::dots<T, GROUP, 1, 1, 1>(acc, w, s, row, 2 * min(last + 1 - row0, 8), t0, t1, a.H, rows);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int j = row0 + 2 * c + i;
@@ -325,13 +334,14 @@ struct Narrow {
 // kDownCols columns of out.  A wave takes experts wave, wave + 8, ...; of four experts or fewer two waves or more share the contraction
 // of each.  Its sums are its own; they are added up in the order of the waves.
 template <class W>
-__device__ __forceinline__ void down_job(const Args &a, const Plan &p, DownSums &sums, int strip) {
+__device__ __forceinline__ void down_job(const Args &a, const Plan &p, Sums &sh, int strip) {
+    DownSums &sums = sh.down;
     const int tid = threadIdx.x, wave = gmm::uniform(tid >> 6), lane = tid & 63;
     const int parts = p.n > 4 ? 1 : p.n > 2 ? 2 : p.n == 2 ? 4 : 8;
     float(&y)[kMaxTokens][16] = sums.y[wave];
 #pragma unroll
     for (int i = 0; i < kMaxTokens * 16 / 64; ++i) (&y[0][0])[i * 64 + lane] = 0.f;
-    for (int u = wave / parts; u < p.n; u += kWaves / parts) W::down(a, p, y, u, strip, wave & (parts - 1), parts);
+    for (int u = wave / parts; u < p.n; u += kWaves / parts) W::down(a, p, y, sh.rows[wave], u, strip, wave & (parts - 1), parts);
     __syncthreads();
     constexpr int C = W::kDownCols;
     if (tid < a.T * C) {

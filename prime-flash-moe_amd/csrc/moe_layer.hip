@@ -40,18 +40,18 @@ __global__ __launch_bounds__(256) void moe_layer_router_kernel(Args a) {
 template <class W>
 __global__ __launch_bounds__(kThreads) void moe_layer_up_kernel(Args a) {
     __shared__ Plan p;
-    __shared__ Sums sums;
+    __shared__ __attribute__((aligned(1024))) Sums sums;
     find_plan(a, p, blockIdx.x == 0);
     const int strips = (a.H + kUpCols - 1) / kUpCols, u = (int)blockIdx.x / strips;
-    if (u < p.n) W::up(a, p, sums.up, u, (int)blockIdx.x - u * strips);
+    if (u < p.n) W::up(a, p, sums, u, (int)blockIdx.x - u * strips);
 }
 
 template <class W>
 __global__ __launch_bounds__(kThreads) void moe_layer_down_kernel(Args a) {
     __shared__ Plan p;
-    __shared__ Sums sums;
+    __shared__ __attribute__((aligned(1024))) Sums sums;
     find_plan(a, p, false);
-    down_job<W>(a, p, sums.down, (int)blockIdx.x);
+    down_job<W>(a, p, sums, (int)blockIdx.x);
 }
 
 template <class W>
