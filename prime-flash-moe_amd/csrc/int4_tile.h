@@ -61,6 +61,25 @@ struct Num<F16> {
 
 __device__ __forceinline__ i32x4 load_once16(const char *p) { return __builtin_nontemporal_load(reinterpret_cast<const i32x4 *>(p)); }
 
+// 16 bytes as they stand in memory now, whatever the caches of the XCD hold.
+__device__ __forceinline__ i32x4 load_now(const char *p) {
+    const uint64_t *q = reinterpret_cast<const uint64_t *>(p);
+    const uint64_t lo = __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), hi = __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
+}
+
+// A piece of memory of up to 4 GB, wave-uniform: a load takes an offset per lane and one for the wave; behind `bytes` it reads zeros.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+__device__ __forceinline__ Buffer buffer(const char *p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(ring::uniform_ptr(p)), 0, (int)bytes, 0x00020000);  // (raw bytes, no stride)
+}
+__device__ __forceinline__ i32x4 load(Buffer b, uint32_t lane, uint32_t wave) { return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(b, lane, wave, 0)); }
+// The same with the non-temporal hint, for what no other workgroup reads.
+__device__ __forceinline__ i32x4 load_once(Buffer b, uint32_t lane, uint32_t wave) { return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(b, lane, wave, 2)); }
+
+// The same, as it stands in memory now, whatever the caches of the XCD hold.
+__device__ __forceinline__ i32x4 load_now(Buffer b, uint32_t lane, uint32_t wave) { return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(b, lane, wave, 16)); }
+
 // The scales of a lane's row in a tile.
 template <int GROUP>
 struct TileScales {
@@ -87,9 +106,9 @@ struct TileScales {
 template <int R, int S>
 struct Rows {
     i32x4 v[S * R * 4];
-    // `x(q)`: begins row q; `n`: rows, from 1 to 16 R (both wave-uniform but for the lane's q).
-    template <class X>
-    __device__ __forceinline__ void load(X x, int n, int t, int t1, int k) {
+    // `x(q)`: begins row q; `n`: rows, from 1 to 16 R (both wave-uniform but for the lane's q); get(address): 16 bytes.
+    template <class X, class Get>
+    __device__ __forceinline__ void load(X x, Get get, int n, int t, int t1, int k) {
         const int lane = threadIdx.x & 63, sub = lane >> 4, e = (lane & 15) * 8;
 #pragma unroll
         for (int i = 0; i < S; ++i)
@@ -99,9 +118,24 @@ struct Rows {
                 for (int g = 0; g < R * 4; ++g)
                     if (g == 0 || 4 * g < n) {
                         v[i * R * 4 + g] = i32x4{0, 0, 0, 0};
-                        if (col < k) v[i * R * 4 + g] = *reinterpret_cast<const i32x4 *>(x(min(4 * g + sub, n - 1)) + (int64_t)col * 2);
+                        if (col < k) v[i * R * 4 + g] = get(x(min(4 * g + sub, n - 1)) + (int64_t)col * 2);
                     }
             }
+    }
+    // The largest of the words that were loaded.
+    __device__ __forceinline__ uint32_t most(int n, int t, int t1) const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < S; ++i)
+            if (i == 0 || t + i < t1) {
+#pragma unroll
+                for (int g = 0; g < R * 4; ++g)
+                    if (g == 0 || 4 * g < n) {
+#pragma unroll
+                        for (int d = 0; d < 4; ++d) m = max(m, (uint32_t)v[i * R * 4 + g][d]);
+                    }
+            }
+        return m;
     }
     __device__ __forceinline__ void store(char *lds, int n, int t, int t1) const {
         const int lane = threadIdx.x & 63, sub = lane >> 4;
@@ -125,9 +159,13 @@ struct Rows {
 // acc[u][q] += n rows of x times the weights of tiles t0 .. t1 - 1 of U strips (16 weight rows each), for one wave.  Lane l, r = l %
 // 16, c = l / 16: `w[u]`, `s[u]` begin strip u.  acc[u][q][i]: weight row r, row 16 q + 4 c + i of x (any of the n where there are fewer).
 // `k`: columns; nothing of x is read behind them.  `lds`: Rows<R, S>::kBytes of the wave's own.  S: tiles whose loads are in flight
-// together; what hides the rest of their latency is other waves.
-template <class T, int GROUP, int U, int R, int S, class X>
-__device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[U], const char *const (&s)[U], X x, int n, int t0, int t1, int k, char *lds) {
+// together; what hides the rest of their latency is other waves.  wait(most): called with the largest word of what was loaded of x, for
+// rows that may not all be there yet: true until they are.
+struct NoWait {
+    static constexpr bool kWaits = false;
+};
+template <class T, int GROUP, int U, int R, int S, class X, class Wait = NoWait>
+__device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[U], const char *const (&s)[U], X x, int n, int t0, int t1, int k, char *lds, Wait wait = {}) {
     using Sc = TileScales<GROUP>;
     constexpr int PER = GROUP / 32;
     const int lane = threadIdx.x & 63, r = lane & 15;
@@ -136,7 +174,7 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
         i32x4 wv[S][U];
         Sc sc[S][U];
         Rows<R, S> rows;
-        rows.load(x, n, t, t1, k);
+        rows.load(x, [](const char *p) { return *reinterpret_cast<const i32x4 *>(p); }, n, t, t1, k);
 #pragma unroll
         for (int i = 0; i < S; ++i)
             if (i == 0 || t + i < t1) {
@@ -146,6 +184,8 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
                     sc[i][u].load(s[u] + (int64_t)(t + i) * Sc::kBytes, r);
                 }
             }
+        if constexpr (Wait::kWaits)
+            while (wait(rows.most(n, t, t1))) rows.load(x, [](const char *p) { return load_now(p); }, n, t, t1, k);
         rows.store(lds, n, t, t1);
 #pragma unroll
         for (int i = 0; i < S; ++i)

@@ -27,10 +27,20 @@ using int4::f32x4;
 using int4::Num;
 
 constexpr int kMaxTokens = 16, kMaxTopK = 32, kMaxPairs = kMaxTokens * kMaxTopK, kMaxExperts = 512;
-constexpr int kThreads = 512, kWaves = 8;
-constexpr int kUpCols = 16;  // activation columns of an up job
+constexpr int kThreads = 512, kWaves = 8, kWavesLog = 3;
+constexpr int kUpCols = 16;       // activation columns of an up job at most
+constexpr int kMaxShares = 4;     // workgroups that share a strip of out
+constexpr int kMaxShared = 1024;  // shares of all strips at most, if they are shared
+constexpr int64_t kMostTries = 1 << 24;  // of a wait, about a microsecond each: then the outputs are NaN
 
+// Queues of the up jobs, a line of 128 bytes each (an atomic of the device takes 11 ns per address).
+constexpr int kQueues = 8;  // as many as XCDs, which workgroups go round
+struct Sync {
+    int32_t ticket[kQueues][32];
+    int32_t arrived[kMaxShared / 2];  // strip of out: workgroups that have their share of a strip of out
+};
 struct Args {
+    Sync *sync;
     const char *x, *gate, *w1, *w1_scale, *w2, *w2_scale;
     const float *bias;
     char *out;
@@ -39,7 +49,11 @@ struct Args {
     float *logits;  // (T, E)
     char *act;      // [pair][2: value, rest][act_pitch bytes]
     int act_pitch;
+    float *shares;  // [strip of out][share][token][column]: sums of workgroups that share a strip
     int T, K, H, E, top_k;
+    int up_cols;    // columns of an up job, a multiple of 4
+    int n_shares;   // 1 << shares_log
+    int shares_log;
 };
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -66,54 +80,190 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
-// acc[q][n] += this lane's share of weight row w[q] times row x[n]: steps s0 .. s1 - 1 of 128 elements.  The pointers begin
-// the rows; `k`: their elements, a multiple of 8; nothing is read behind them.
-template <class T, int Q, int N, int S>
-__device__ __forceinline__ void row_dots(float (&acc)[Q][N], const char *const (&w)[Q], const char *const (&x)[N], int s0, int s1, int k) {
-    const int at = (threadIdx.x & 15) * 8;
-    for (int s = s0; s < s1; s += S) {
-        i32x4 wv[Q][S], xv[N][S];
+// What a word of the activation (two columns) holds until its up job has written it: two NaNs that no job writes.  So a word says by
+// itself whether it is there, and where a cached one says that it is not, memory is asked again: nothing else is needed between
+// the up jobs and the down jobs, no counter behind the stores, no cache to be emptied.
+constexpr uint32_t kAbsent = 0xffffffffu;
+struct Arrival {
+    static constexpr bool kWaits = true;
+    int *failed;  // LDS
+    int64_t tries = 0;
+    // Whether this wave has to load again.
+    __device__ __forceinline__ bool operator()(uint32_t most) {
+        if (__ballot(most == kAbsent) == 0) return false;
+        if (++tries > kMostTries || __hip_atomic_load(failed, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP) != 0) {
+            __hip_atomic_store(failed, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            return false;
+        }
+        __builtin_amdgcn_s_sleep(2);
+        return true;
+    }
+};
+
+// acc[q][n] += this lane's share of a weight row times row n of x: steps s0 .. s1 - 1 of 128 elements.  `w[q]` begins four weight rows,
+// `pitch` bytes apart, of which a lane has number lane / 16, `last` at most; row n begins at byte xo[n] of `x`, which holds `x_bytes`
+// (all wave-uniform).  `k`: elements of a row, a multiple of 8; nothing is read behind them.  Only the first `live` of the Q are there.  The weights of S steps are in flight together, the rows of SX.
+// wait: see int4::dots.
+template <class T, int Q, int N, int S, int SX, class Wait = int4::NoWait>
+__device__ __forceinline__ void row_dots(float (&acc)[Q][N], const char *const (&w)[Q], int pitch, const char *x, uint32_t x_bytes, const uint32_t (&xo)[N], int s0,
+                                         int s1, int k, int live = Q, int last = 3, Wait wait = {}) {
+    const int lane = threadIdx.x & 63;
+    const uint32_t own = (lane & 15) * 16, wo = (uint32_t)min(lane >> 4, last) * (uint32_t)pitch + own;
+    // (buffer loads take a step's offset from a scalar register, where pointers of their own per step fill the vector registers)
+    int4::Buffer wb[Q];
 #pragma unroll
-        for (int i = 0; i < S; ++i)
-            if (s + i < s1) {
-                const int e = (s + i) * 128 + at;
+    for (int q = 0; q < Q; ++q)
+        if (q < live) wb[q] = int4::buffer(w[q], 4u * (uint32_t)pitch);
+    const int4::Buffer xb = int4::buffer(x, x_bytes);
+    auto multiply = [&](const i32x4 (&wv)[Q], const i32x4 (&xv)[N]) {
 #pragma unroll
-                for (int q = 0; q < Q; ++q) {
-                    wv[q][i] = i32x4{0, 0, 0, 0};
-                    if (e < k) wv[q][i] = int4::load_once16(w[q] + (int64_t)e * 2);
-                }
+        for (int q = 0; q < Q; ++q)
+            if (q < live)
 #pragma unroll
                 for (int n = 0; n < N; ++n) {
-                    xv[n][i] = i32x4{0, 0, 0, 0};
-                    if (e < k) xv[n][i] = *reinterpret_cast<const i32x4 *>(x[n] + (int64_t)e * 2);
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) acc[q][n] = dot2<T>(wv[q][d], xv[n][d], acc[q][n]);
                 }
-            }
+    };
+    const int whole = min(s1, k / 128);
+    for (int s = s0; s < whole; s += S) {
+        i32x4 wv[S][Q];
 #pragma unroll
         for (int i = 0; i < S; ++i)
-            if (s + i < s1) {
+            if (s + i < whole) {
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+                    if (q < live) wv[i][q] = int4::load_once(wb[q], wo, (s + i) * 256);
+            }
+#pragma unroll
+        for (int i0 = 0; i0 < S; i0 += SX)
+            if (s + i0 < whole) {
+                i32x4 xv[SX][N];
+#pragma unroll
+                for (int i = 0; i < SX; ++i)
+                    if (s + i0 + i < whole) {
+#pragma unroll
+                        for (int n = 0; n < N; ++n) xv[i][n] = int4::load(xb, own, xo[n] + (s + i0 + i) * 256);
+                    }
+                if constexpr (Wait::kWaits)
+                    for (;;) {
+                        uint32_t most = 0;
+#pragma unroll
+                        for (int i = 0; i < SX; ++i)
+                            if (s + i0 + i < whole) {
+#pragma unroll
+                                for (int n = 0; n < N; ++n)
+#pragma unroll
+                                    for (int d = 0; d < 4; ++d) most = max(most, (uint32_t)xv[i][n][d]);
+                            }
+                        if (!wait(most)) break;
+#pragma unroll
+                        for (int i = 0; i < SX; ++i)
+                            if (s + i0 + i < whole) {
+#pragma unroll
+                                for (int n = 0; n < N; ++n) xv[i][n] = int4::load_now(xb, own, xo[n] + (s + i0 + i) * 256);
+                            }
+                    }
+#pragma unroll
+                for (int i = 0; i < SX; ++i)
+                    if (s + i0 + i < whole) multiply(wv[i0 + i], xv[i]);
+            }
+    }
+    if (s1 > k / 128 && s0 < s1 && (lane & 15) * 8 < k % 128) {  // a step in part (the last one)
+        i32x4 wv[Q], xv[N];
+#pragma unroll
+        for (int q = 0; q < Q; ++q)
+            if (q < live) wv[q] = int4::load_once(wb[q], wo, k / 128 * 256);
+#pragma unroll
+        for (int n = 0; n < N; ++n) xv[n] = int4::load(xb, own, xo[n] + k / 128 * 256);
+        if constexpr (Wait::kWaits)
+            for (;;) {
+                uint32_t most = 0;
 #pragma unroll
                 for (int n = 0; n < N; ++n)
 #pragma unroll
-                    for (int q = 0; q < Q; ++q)
+                    for (int d = 0; d < 4; ++d) most = max(most, (uint32_t)xv[n][d]);
+                if (!wait(most)) break;
 #pragma unroll
-                        for (int d = 0; d < 4; ++d) acc[q][n] = dot2<T>(wv[q][i][d], xv[n][i][d], acc[q][n]);
+                for (int n = 0; n < N; ++n) xv[n] = int4::load_now(xb, own, xo[n] + k / 128 * 256);
             }
+        multiply(wv, xv);
     }
 }
 
 // The touched experts and their tokens, by every workgroup for itself.
 struct Plan {
     int n;                              // touched experts
+    int job;                            // the workgroup's
+    int failed;                         // a wait was given up
     uint32_t touched[kMaxExperts / 32];
     uint16_t expert[kMaxPairs];
     uint32_t tokens[kMaxPairs];         // bit t: token t is the expert's
     uint8_t slot[kMaxPairs][kMaxTokens];  // which of the token's top_k the expert is
     float weight[kMaxPairs];            // of pair t top_k + r
     int16_t id[kMaxPairs];
+    __attribute__((aligned(16))) uint32_t key[kMaxExperts];
+    int32_t rank[kMaxExperts];
 };
 
+// One token: top-k by ranks.  A thread counts, for one expert, how many of a part of the logits are in front of it (rounds of a wave, one
+// winner after the other, take 0.7 us longer).  Every chosen expert is the token's, in the order of the ranks.
+__device__ __forceinline__ void plan_one(const Args &a, Plan &p, bool publish) {
+    const int tid = threadIdx.x, log = a.E <= 64 ? 6 : a.E <= 128 ? 7 : a.E <= 256 ? 8 : 9, stride = 1 << log;
+    const int parts_log = min(9 - log, log - 2), e = tid & (stride - 1), part = tid >> log;  // (a part is a multiple of four)
+    if (tid == 0) p.failed = 0, p.n = a.top_k;
+    if (tid < stride) {
+        uint32_t key = 0;
+        if (tid < a.E) {
+            float v = a.logits[tid];
+            if (a.bias != nullptr) v += a.bias[tid];
+            key = route::order_key(v);
+        }
+        p.key[tid] = key;
+        p.rank[tid] = 0;
+    }
+    __syncthreads();
+    if (part < 1 << parts_log && e < a.E) {
+        const uint32_t mine = p.key[e];
+        const int each = stride >> 2 >> parts_log;
+        int before = 0;
+#pragma unroll 2
+        for (int i = part * each; i < (part + 1) * each; ++i) {
+            const i32x4 k = reinterpret_cast<const i32x4 *>(p.key)[i];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) before += (uint32_t)k[j] > mine || ((uint32_t)k[j] == mine && 4 * i + j < e);
+        }
+        atomicAdd(&p.rank[e], before);
+    }
+    __syncthreads();
+    if (tid < a.E && p.rank[tid] < a.top_k) {
+        p.expert[p.rank[tid]] = (uint16_t)tid;
+        p.weight[p.rank[tid]] = route::key_value(p.key[tid]);
+    }
+    __syncthreads();
+    if (tid < 64) {  // softmax over the winners, the first of which is the largest; read behind a later barrier
+        const float v = tid < a.top_k ? p.weight[tid] : 0.f, most = __int_as_float(gmm::uniform(__float_as_int(v)));
+        const float ex = tid < a.top_k ? expf(v - most) : 0.f;
+        float sum = row_sum(ex);
+        sum += __shfl_xor(sum, 16, 64);
+        if (tid < a.top_k) {
+            p.weight[tid] = ex / sum;
+            if (publish) {
+                a.topk_ids[tid] = p.expert[tid];
+                a.topk_weights[tid] = ex / sum;
+            }
+        }
+    }
+}
+
+template <bool ONE>
 __device__ __forceinline__ void find_plan(const Args &a, Plan &p, bool publish) {
+    if constexpr (ONE) {
+        plan_one(a, p, publish);
+        return;
+    }
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, n_pairs = a.T * a.top_k;
+    if (tid == 0) p.failed = 0;
     if (tid < kMaxExperts / 32) p.touched[tid] = 0;
     if (tid < kMaxPairs) p.tokens[tid] = 0;
     for (int t = wave; t < a.T; t += kWaves) {
@@ -147,7 +297,7 @@ __device__ __forceinline__ void find_plan(const Args &a, Plan &p, bool publish) 
     if (wave == kWaves - 1) {
         int n = lane < kMaxExperts / 32 ? __popc(p.touched[lane]) : 0;
 #pragma unroll
-        for (int d = 32; d > 0; d /= 2) n += __shfl_xor(n, d, 64);
+        for (int d = 8; d > 0; d /= 2) n += __shfl_xor(n, d, 64);
         if (lane == 0) p.n = n;
     }
     __syncthreads();
@@ -159,20 +309,31 @@ __device__ __forceinline__ int token_of(uint32_t tokens, int j) {
     return __builtin_ctz(tokens);
 }
 
-// The rows of an expert one, two, four or eight at a time: f(integral N, first row).
-template <class F>
-__device__ __forceinline__ void by_rows(int n, F f) {
-    if (n == 1) f(std::integral_constant<int, 1>{}, 0);
-    else if (n == 2) f(std::integral_constant<int, 2>{}, 0);
-    else if (n <= 4) f(std::integral_constant<int, 4>{}, 0);
-    else
-        for (int j = 0; j < n; j += 8) f(std::integral_constant<int, 8>{}, j);
+// The tokens of an expert, the token of row j, and what number of its experts this is.  ONE: the layer has one token.
+template <bool ONE>
+__device__ __forceinline__ uint32_t tokens_of(const Plan &p, int u) {
+    return ONE ? 1u : (uint32_t)gmm::uniform((int)p.tokens[u]);
+}
+template <bool ONE>
+__device__ __forceinline__ int pair_of(const Args &a, const Plan &p, int u, int t) {
+    return ONE ? u : t * a.top_k + p.slot[u][t];
 }
 
-// Two 16-bit numbers that add up to v.
+// The rows of an expert one, two or four at a time: f(integral N, first row).
+template <bool ONE, class F>
+__device__ __forceinline__ void by_rows(int n, F f) {
+    if (ONE || n == 1) return f(std::integral_constant<int, 1>{}, 0);
+    if constexpr (!ONE) {
+        if (n == 2) return f(std::integral_constant<int, 2>{}, 0);
+        for (int j = 0; j < n; j += 4) f(std::integral_constant<int, 4>{}, j);
+    }
+}
+
+// Two 16-bit numbers that add up to v (of what is beyond the type the first alone; one NaN for all, see kAbsent).
 template <class T>
 __device__ __forceinline__ uint32_t split(float v) {
-    const uint16_t hi = Num<T>::from_f32(v), lo = Num<T>::from_f32(v - Num<T>::to_f32(hi));
+    const uint16_t hi = v != v ? Num<T>::kNan : Num<T>::from_f32(v);
+    const uint16_t lo = Num<T>::finite(hi) ? Num<T>::from_f32(v - Num<T>::to_f32(hi)) : 0;
     return hi | (uint32_t)lo << 16;
 }
 
@@ -191,19 +352,23 @@ struct Sums {
     char rows[kWaves][Rows::kBytes];  // rows of x or of the activation on their way to a wave
 };
 
-// What the 16 columns of an up job have in `parts` parts -> activation.
-template <class T>
-__device__ __forceinline__ void finish_up(const Args &a, const Plan &p, const UpSums &s, int u, int col0, int parts) {
-    const uint32_t tokens = p.tokens[u];
-    const int rows = __popc(tokens), c = threadIdx.x & 15, j = threadIdx.x >> 4;
-    if (j < rows && col0 + c < a.H) {
-        float gate = 0.f, up = 0.f;
-        for (int k = 0; k < parts; ++k) gate += s.part[k][0][j][c], up += s.part[k][1][j][c];
-        const int t = token_of(tokens, j);
-        const uint32_t v = split<T>(swiglu(gate, up));
-        char *at = a.act + (int64_t)(t * a.top_k + p.slot[u][t]) * 2 * a.act_pitch + (col0 + c) * 2;
-        *reinterpret_cast<uint16_t *>(at) = (uint16_t)v;
-        *reinterpret_cast<uint16_t *>(at + a.act_pitch) = (uint16_t)(v >> 16);
+// What the columns of an up job have from every wave -> activation, two columns a thread.  The stores go through to where all XCDs see
+// them.
+template <class T, bool ONE>
+__device__ __forceinline__ void finish_up(const Args &a, const Plan &p, const UpSums &s, int u, int col0) {
+    const uint32_t tokens = tokens_of<ONE>(p, u);
+    const int rows = __popc(tokens), c = (threadIdx.x & 7) * 2, j = threadIdx.x >> 3;
+    if (j < rows && c < a.up_cols && col0 + c < a.H) {
+        float gate[2] = {}, up[2] = {};
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) gate[i] += s.part[k][0][j][c + i], up[i] += s.part[k][1][j][c + i];
+        const int t = ONE ? 0 : token_of(tokens, j);
+        const uint32_t v0 = split<T>(swiglu(gate[0], up[0])), v1 = split<T>(swiglu(gate[1], up[1]));
+        char *at = a.act + (int64_t)pair_of<ONE>(a, p, u, t) * 2 * a.act_pitch + (col0 + c) * 2;
+        __hip_atomic_store(reinterpret_cast<uint32_t *>(at), (v0 & 0xffffu) | v1 << 16, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(reinterpret_cast<uint32_t *>(at + a.act_pitch), v0 >> 16 | (v1 & 0xffff0000u), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
@@ -213,65 +378,85 @@ struct Wide {
     using Type = T;
     static constexpr int kDownCols = 8;
 
-    // Waves: four groups of four columns (a column's gate and up row on 16 lanes) x two halves of the contraction.
+    // The waves share the contraction; each has the gate and up rows of all columns, so that a row of x is read for up to 32 of them.
+    template <bool ONE>
     static __device__ __forceinline__ void up(const Args &a, const Plan &p, Sums &sh, int u, int strip) {
-        UpSums &sums = sh.up;
-        const int lane = threadIdx.x & 63, wave = gmm::uniform(threadIdx.x >> 6), quad = wave & 3, half = wave >> 2, sub = lane >> 4;
-        const int steps = (a.K + 127) / 128, s0 = half * steps / 2, s1 = (half + 1) * steps / 2;
-        const int c = 4 * quad + sub, col = min(strip * kUpCols + c, a.H - 1);
-        const uint32_t tokens = gmm::uniform(p.tokens[u]);
-        const char *gate = a.w1 + ((int64_t)p.expert[u] * 2 * a.H + col) * a.K * 2;
-        const char *const w[2] = {gate, gate + (int64_t)a.H * a.K * 2};
-        by_rows(__popc(tokens), [&](auto n, int row0) {
+        const int lane = threadIdx.x & 63, wave = gmm::uniform(threadIdx.x >> 6), sub = lane >> 4, quads = a.up_cols / 4;
+        const int steps = (a.K + 127) / 128, s0 = wave * steps >> kWavesLog, s1 = (wave + 1) * steps >> kWavesLog;
+        const uint32_t tokens = tokens_of<ONE>(p, u);
+        const char *const gate = a.w1 + (int64_t)gmm::uniform(p.expert[u]) * 2 * a.H * a.K * 2;
+        const char *w[kUpCols / 2];
+#pragma unroll
+        for (int q = 0; q < kUpCols / 4; ++q) {
+            const int col = min(strip * a.up_cols + 4 * q, a.H - 4);  // (H is a multiple of 4: all four are inside or none)
+            w[2 * q] = gate + (int64_t)col * a.K * 2;
+            w[2 * q + 1] = gate + (int64_t)(a.H + col) * a.K * 2;
+        }
+        by_rows<ONE>(__popc(tokens), [&](auto n, int row0) {
             constexpr int N = decltype(n)::value;
             const int last = __popc(tokens) - 1;
-            const char *x[N];
-            float acc[2][N] = {};
+            uint32_t xo[N];
+            float acc[kUpCols / 2][N] = {};
 #pragma unroll
-            for (int j = 0; j < N; ++j) x[j] = a.x + (int64_t)token_of(tokens, min(row0 + j, last)) * a.K * 2;
-            row_dots<T, 2, N, (N <= 2 ? 8 : N == 4 ? 4 : 2)>(acc, w, x, s0, s1, a.K);
+            for (int j = 0; j < N; ++j) xo[j] = ONE ? 0 : (uint32_t)token_of(tokens, min(row0 + j, last)) * (uint32_t)a.K * 2;
+            row_dots<T, kUpCols / 2, N, (N <= 2 ? 2 : 1), (N <= 2 ? 2 : 1)>(acc, w, a.K * 2, a.x, (uint32_t)a.T * a.K * 2, xo, s0, s1, a.K, 2 * quads);
 #pragma unroll
-            for (int j = 0; j < N; ++j) {
-                const float g = row_sum(acc[0][j]), v = row_sum(acc[1][j]);
-                if ((lane & 15) == 0 && row0 + j <= last) sums.part[half][0][row0 + j][c] = g, sums.part[half][1][row0 + j][c] = v;
-            }
+            for (int q = 0; q < kUpCols / 4; ++q)
+                if (q < quads)
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const float g = row_sum(acc[2 * q][j]), v = row_sum(acc[2 * q + 1][j]);
+                        if ((lane & 15) == 0 && row0 + j <= last) sh.up.part[wave][0][row0 + j][4 * q + sub] = g, sh.up.part[wave][1][row0 + j][4 * q + sub] = v;
+                    }
         });
-        __syncthreads();
-        finish_up<T>(a, p, sums, u, strip * kUpCols, 2);
     }
 
-    // sums[.][.] += expert u's share, steps part / parts, of 8 columns of out.
-    static __device__ __forceinline__ void down(const Args &a, const Plan &p, float (&y)[kMaxTokens][16], char *rows, int u, int strip, int part, int parts) {
+    // Address of line `lane` of a wave's share of a down job (null: it has fewer).
+    static __device__ __forceinline__ const char *down_line(const Args &a, const Plan &p, int u, int strip, int part, int parts_log, int lane) {
+        const int steps = (a.H + 127) / 128, s0 = part * steps >> parts_log, lines = (((part + 1) * steps >> parts_log) - s0) * 2;
+        const int row = lane % 8, line = lane / 8, at = s0 * 256 + line * 128;
+        return line < lines && at < a.H * 2 ? down_weights(a, p, u, strip) + (int64_t)row * a.H * 2 + at : nullptr;
+    }
+    static __device__ __forceinline__ const char *down_weights(const Args &a, const Plan &p, int u, int strip) {
+        return a.w2 + ((int64_t)gmm::uniform(p.expert[u]) * a.K + strip * kDownCols) * a.H * 2;
+    }
+
+    // sums[.][.] += expert u's share, part `part` of 1 << parts_log of its contraction, of 8 columns of out.
+    template <bool ONE>
+    static __device__ __forceinline__ void down(const Args &a, Plan &p, float (&y)[kMaxTokens][16], char *rows, int u, int strip, int part, int parts_log) {
         const int lane = threadIdx.x & 63, sub = lane >> 4;
-        const int steps = (a.H + 127) / 128, s0 = part * steps / parts, s1 = (part + 1) * steps / parts;
-        const uint32_t tokens = gmm::uniform(p.tokens[u]);
-        const char *w2 = a.w2 + (int64_t)p.expert[u] * a.K * a.H * 2;
-        const char *const w[2] = {w2 + (int64_t)(strip * 8 + sub) * a.H * 2, w2 + (int64_t)(strip * 8 + 4 + sub) * a.H * 2};
+        const int steps = (a.H + 127) / 128, s0 = part * steps >> parts_log, s1 = (part + 1) * steps >> parts_log;
+        const uint32_t tokens = tokens_of<ONE>(p, u);
+        const char *const first = down_weights(a, p, u, strip);
+        const char *const w[2] = {first, first + (int64_t)4 * a.H * 2};
         auto some = [&](auto n, int row0) {
             constexpr int N = decltype(n)::value;
             const int last = __popc(tokens) - 1;
-            const char *x[2 * N];
+            uint32_t xo[2 * N];
             float acc[2][2 * N] = {};
-            int t[N];
+            int t[N], pair[N];
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                t[j] = token_of(tokens, min(row0 + j, last));
-                x[2 * j] = a.act + (int64_t)(t[j] * a.top_k + p.slot[u][t[j]]) * 2 * a.act_pitch;
-                x[2 * j + 1] = x[2 * j] + a.act_pitch;
+                t[j] = ONE ? 0 : token_of(tokens, min(row0 + j, last));
+                pair[j] = gmm::uniform(pair_of<ONE>(a, p, u, t[j]));
+                xo[2 * j] = (uint32_t)pair[j] * 2u * (uint32_t)a.act_pitch;
+                xo[2 * j + 1] = xo[2 * j] + a.act_pitch;
             }
-            row_dots<T, 2, 2 * N, (N <= 1 ? 8 : N == 2 ? 4 : 2)>(acc, w, x, s0, s1, a.H);
+            row_dots<T, 2, 2 * N, (N == 1 ? 6 : N == 2 ? 4 : 2), (N == 1 ? 3 : N == 2 ? 2 : 1)>(acc, w, a.H * 2, a.act, (uint32_t)(a.T * a.top_k) * 2u * (uint32_t)a.act_pitch, xo, s0, s1, a.H, 2, 3, Arrival{&p.failed});
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const float v0 = row_sum(acc[0][2 * j] + acc[0][2 * j + 1]), v1 = row_sum(acc[1][2 * j] + acc[1][2 * j + 1]);
-                const float wt = p.weight[t[j] * a.top_k + p.slot[u][t[j]]];
+                const float wt = p.weight[pair[j]];
                 if ((lane & 15) == 0 && row0 + j <= last) y[t[j]][sub] += wt * v0, y[t[j]][4 + sub] += wt * v1;
             }
         };
         const int n = __popc(tokens);
-        if (n == 1) some(std::integral_constant<int, 1>{}, 0);
-        else if (n == 2) some(std::integral_constant<int, 2>{}, 0);
-        else
-            for (int j = 0; j < n; j += 4) some(std::integral_constant<int, 4>{}, j);
+        if (ONE || n == 1) return some(std::integral_constant<int, 1>{}, 0);
+        if constexpr (!ONE) {
+            if (n == 2) some(std::integral_constant<int, 2>{}, 0);
+            else
+                for (int j = 0; j < n; j += 4) some(std::integral_constant<int, 4>{}, j);
+        }
     }
 };
 
@@ -282,75 +467,190 @@ struct Narrow {
     static constexpr int kDownCols = 16;
 
     // The waves share the contraction; a strip of gate rows and the matching one of up rows.
+    template <bool ONE>
     static __device__ __forceinline__ void up(const Args &a, const Plan &p, Sums &sh, int u, int strip) {
         UpSums &sums = sh.up;
         const int lane = threadIdx.x & 63, wave = gmm::uniform(threadIdx.x >> 6), r = lane & 15, c = lane >> 4;
         char *const rows = sh.rows[wave];
         const int tiles = int4::tiles_of(a.K), t0 = wave * tiles / kWaves, t1 = (wave + 1) * tiles / kWaves, strips = a.H / 16;
-        const uint32_t tokens = gmm::uniform(p.tokens[u]);
+        const uint32_t tokens = tokens_of<ONE>(p, u);
         const int last = __popc(tokens) - 1;
         constexpr int SB = int4::TileScales<GROUP>::kBytes;
-        const int64_t first = (int64_t)p.expert[u] * 2 * strips + strip;
+        const int64_t first = (int64_t)gmm::uniform(p.expert[u]) * 2 * strips + strip;
         const char *const w[2] = {a.w1 + first * tiles * int4::kTileBytes, a.w1 + (first + strips) * tiles * int4::kTileBytes};
         const char *const s[2] = {a.w1_scale + first * tiles * SB, a.w1_scale + (first + strips) * tiles * SB};
         f32x4 acc[2][1] = {};
-        int4::dots<T, GROUP, 2, 1, 1>(acc, w, s, [&](int q) { return a.x + (int64_t)token_of(tokens, q) * a.K * 2; }, last + 1, t0, t1, a.K, rows);
-        __syncthreads();  // the sums may lie where the rows were
+        int4::dots<T, GROUP, 2, 1, 1>(acc, w, s, [&](int q) { return a.x + (ONE ? 0 : (int64_t)token_of(tokens, q) * a.K * 2); }, last + 1, t0, t1, a.K, rows);
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums.part[wave][0][4 * c + i][r] = acc[0][0][i], sums.part[wave][1][4 * c + i][r] = acc[1][0][i];
-        __syncthreads();
-        finish_up<T>(a, p, sums, u, strip * kUpCols, kWaves);
     }
 
-    static __device__ __forceinline__ void down(const Args &a, const Plan &p, float (&y)[kMaxTokens][16], char *rows, int u, int strip, int part, int parts) {
+    static __device__ __forceinline__ const char *down_line(const Args &a, const Plan &p, int u, int strip, int part, int parts_log, int lane) {
+        const int tiles = int4::tiles_of(a.H), t0 = part * tiles >> parts_log, t1 = (part + 1) * tiles >> parts_log;
+        return lane < (t1 - t0) * (int4::kTileBytes / 128) ? down_weights(a, p, u, strip) + (int64_t)t0 * int4::kTileBytes + lane * 128 : nullptr;
+    }
+    static __device__ __forceinline__ const char *down_weights(const Args &a, const Plan &p, int u, int strip) {
+        return a.w2 + ((int64_t)gmm::uniform(p.expert[u]) * (a.K / 16) + strip) * int4::tiles_of(a.H) * int4::kTileBytes;
+    }
+
+    template <bool ONE>
+    static __device__ __forceinline__ void down(const Args &a, Plan &p, float (&y)[kMaxTokens][16], char *rows, int u, int strip, int part, int parts_log) {
         const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
-        const int tiles = int4::tiles_of(a.H), t0 = part * tiles / parts, t1 = (part + 1) * tiles / parts;
-        const uint32_t tokens = gmm::uniform(p.tokens[u]);
+        const int tiles = int4::tiles_of(a.H), t0 = part * tiles >> parts_log, t1 = (part + 1) * tiles >> parts_log;
+        const uint32_t tokens = tokens_of<ONE>(p, u);
         const int last = __popc(tokens) - 1;
         constexpr int SB = int4::TileScales<GROUP>::kBytes;
-        const int64_t first = (int64_t)p.expert[u] * (a.K / 16) + strip;
-        const char *const w[1] = {a.w2 + first * tiles * int4::kTileBytes};
+        const int64_t first = (int64_t)gmm::uniform(p.expert[u]) * (a.K / 16) + strip;
+        const char *const w[1] = {down_weights(a, p, u, strip)};
         const char *const s[1] = {a.w2_scale + first * tiles * SB};
         // row m of the matrix instructions: value (m even) or rest of the expert's row m / 2
         for (int row0 = 0; row0 <= last; row0 += 8) {
             f32x4 acc[1][1] = {};
             auto row = [&](int q) {
-                const int t = token_of(tokens, row0 + q / 2);
-                return a.act + ((int64_t)(t * a.top_k + p.slot[u][t]) * 2 + (q & 1)) * a.act_pitch;
+                const int t = ONE ? 0 : token_of(tokens, row0 + q / 2);
+                return a.act + ((int64_t)pair_of<ONE>(a, p, u, t) * 2 + (q & 1)) * a.act_pitch;
             };
-            int4::dots<T, GROUP, 1, 1, 1>(acc, w, s, row, 2 * min(last + 1 - row0, 8), t0, t1, a.H, rows);
+            int4::dots<T, GROUP, 1, 1, 1>(acc, w, s, row, 2 * min(last + 1 - row0, 8), t0, t1, a.H, rows, Arrival{&p.failed});
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int j = row0 + 2 * c + i;
                 if (j <= last) {
-                    const int t = token_of(tokens, j);
-                    y[t][r] += p.weight[t * a.top_k + p.slot[u][t]] * (acc[0][0][2 * i] + acc[0][0][2 * i + 1]);
+                    const int t = ONE ? 0 : token_of(tokens, j);
+                    y[t][r] += p.weight[pair_of<ONE>(a, p, u, t)] * (acc[0][0][2 * i] + acc[0][0][2 * i + 1]);
                 }
             }
         }
     }
 };
 
-// kDownCols columns of out.  A wave takes experts wave, wave + 8, ...; of four experts or fewer two waves or more share the contraction
-// of each.  Its sums are its own; they are added up in the order of the waves.
-template <class W>
-__device__ __forceinline__ void down_job(const Args &a, const Plan &p, Sums &sh, int strip) {
+__device__ __forceinline__ int load_device(const int32_t *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ int add_device(int32_t *p, int n) { return __hip_atomic_fetch_add(p, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// The same with the answer on its way: what stands behind it does not wait.  (An add would be gathered over the wave by the compiler, which
+// waits at once.)
+__device__ __forceinline__ int next_ticket(int32_t *p) { return (int)__builtin_amdgcn_atomic_inc32(reinterpret_cast<uint32_t *>(p), ~0u, __ATOMIC_RELAXED, "agent"); }
+
+// Who does what of a strip of out, kDownCols columns: the waves of all workgroups that share it take the experts by turns; where these are
+// fewer, several waves share the contraction of each.
+struct Turn {
+    int first, step;      // experts of this wave
+    int part, parts_log;  // of their contraction
+    __device__ __forceinline__ Turn(const Args &a, int n, int share) {
+        const int wave = gmm::uniform(threadIdx.x >> 6), all = kWaves * a.n_shares, me = share * kWaves + wave;
+        parts_log = 0;
+        while (n << (parts_log + 1) <= all) ++parts_log;
+        first = me >> parts_log;
+        step = all >> parts_log;
+        part = me & ((1 << parts_log) - 1);
+    }
+};
+
+// Job (strip, share).  A wave's sums are its own; they are added up in the order of the waves, and those of the workgroups that share
+// a strip, by the last of them to arrive, in the order of the shares.
+template <class W, bool ONE>
+__device__ __forceinline__ void down_job(const Args &a, Plan &p, Sums &sh, int job) {
     DownSums &sums = sh.down;
-    const int tid = threadIdx.x, wave = gmm::uniform(tid >> 6), lane = tid & 63;
-    const int parts = p.n > 4 ? 1 : p.n > 2 ? 2 : p.n == 2 ? 4 : 8;
+    const int tid = threadIdx.x, wave = gmm::uniform(tid >> 6), lane = tid & 63, strip = job >> a.shares_log, share = job & (a.n_shares - 1);
+    const Turn turn(a, p.n, share);
     float(&y)[kMaxTokens][16] = sums.y[wave];
 #pragma unroll
-    for (int i = 0; i < kMaxTokens * 16 / 64; ++i) (&y[0][0])[i * 64 + lane] = 0.f;
-    for (int u = wave / parts; u < p.n; u += kWaves / parts) W::down(a, p, y, sh.rows[wave], u, strip, wave & (parts - 1), parts);
+    for (int i = 0; i < (ONE ? 1 : kMaxTokens * 16 / 64); ++i) (&y[0][0])[i * 64 + lane] = 0.f;
+    for (int u = turn.first; u < p.n; u += turn.step) W::template down<ONE>(a, p, y, sh.rows[wave], u, strip, turn.part, turn.parts_log);
     __syncthreads();
     constexpr int C = W::kDownCols;
-    if (tid < a.T * C) {
-        const int t = tid / C, c = tid % C;
-        float v = 0.f;
+    const int t = tid / C, c = tid % C;
+    const bool mine = tid < a.T * C;
+    float v = 0.f;
+    if (mine) {
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) v += sums.y[k][t][c];
-        if (strip * C + c < a.K) reinterpret_cast<uint16_t *>(a.out)[(int64_t)t * a.K + strip * C + c] = Num<typename W::Type>::from_f32(v);
     }
+    bool last = true;
+    if (a.n_shares > 1) {
+        float *const all = a.shares + (int64_t)strip * a.n_shares * a.T * C;
+        if (mine) __hip_atomic_store(all + share * a.T * C + tid, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+        __syncthreads();
+        if (tid == 0) p.job = add_device(&a.sync->arrived[strip], 1);
+        __syncthreads();
+        last = p.job == a.n_shares - 1;
+        if (last && mine) {
+            v = 0.f;
+            for (int k = 0; k < a.n_shares; ++k) v += __hip_atomic_load(all + k * a.T * C + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
+    if (last && mine && strip * C + c < a.K)
+        reinterpret_cast<uint16_t *>(a.out)[(int64_t)t * a.K + strip * C + c] = Num<typename W::Type>::from_f32(p.failed ? __uint_as_float(0x7fc00000u) : v);
+    __syncthreads();  // the sums may be cleared again
+}
+
+// The up jobs, (touched expert, up_cols columns), job j in queue j % 8; a workgroup takes those of its own queue, `ticket` its first, and then
+// what other queues have left.  Returns when all have been taken: what a workgroup waits for then is with workgroups that run and do not
+// wait, so that a wait ends whatever else is on the device and however few workgroups fit on it.
+// Meanwhile the first weights of `down`, the workgroup's first down job (negative: it has none, and returns), are brought into the L2.
+template <class W, bool ONE>
+__device__ __forceinline__ void up_jobs(const Args &a, Plan &p, Sums &sh, int ticket, int down) {
+    const int tid = threadIdx.x, lane = tid & 63, home = blockIdx.x % kQueues;
+    const int strips = (a.H + a.up_cols - 1) / a.up_cols, jobs = p.n * strips;
+    bool own = true;
+    uint32_t ahead = 0;
+    for (;;) {
+        if (tid < 64) {
+            int job = -1;
+            if (own) {
+                const int j = gmm::uniform(ticket) * kQueues + home;
+                if (j < jobs) {
+                    job = j;
+                    if (lane == 0) ticket = next_ticket(&a.sync->ticket[home][0]);  // (on its way while the job runs)
+                }
+            } else {
+                for (;;) {  // lane q: queue q
+                    const uint64_t open = __ballot(lane < kQueues && load_device(&a.sync->ticket[lane % kQueues][0]) < (jobs - lane + kQueues - 1) / kQueues);
+                    if (open == 0) break;
+                    const int victim = __builtin_ctzll(open);
+                    int t = 0;
+                    if (lane == 0) t = add_device(&a.sync->ticket[victim][0], 1);
+                    const int j = gmm::uniform(t) * kQueues + victim;
+                    if (j < jobs) {
+                        job = j;
+                        break;
+                    }
+                }
+            }
+            if (lane == 0) p.job = job;
+        }
+        __syncthreads();
+        const int job = gmm::uniform(p.job);
+        if (job >= 0) {
+            const int u = job / strips;
+            W::template up<ONE>(a, p, sh, u, job - u * strips);
+            __syncthreads();
+            finish_up<typename W::Type, ONE>(a, p, sh.up, u, (job - u * strips) * a.up_cols);
+        } else if (own && down >= 0) {
+            own = false;
+            const Turn turn(a, p.n, down & (a.n_shares - 1));
+            const char *line = turn.first < p.n ? W::down_line(a, p, turn.first, down >> a.shares_log, turn.part, turn.parts_log, lane) : nullptr;
+            if (line != nullptr) ahead = *reinterpret_cast<const uint32_t *>(line);
+            __syncthreads();
+        } else {
+            break;
+        }
+    }
+    // (The last word of the last job: most others are there when it is, and lines that are not would be in the L2 for nothing.)
+    if (tid == 0 && down >= 0) {
+        const int u = p.n - 1, t = ONE ? 0 : __builtin_ctz(p.tokens[u]);
+        const int32_t *word = reinterpret_cast<const int32_t *>(a.act + (int64_t)pair_of<ONE>(a, p, u, t) * 2 * a.act_pitch + a.H * 2 - 4);
+#pragma unroll 1
+        for (int64_t tries = 0; (uint32_t)load_device(word) == kAbsent; ++tries) {
+            if (tries >= kMostTries) {
+                p.failed = 1;
+                break;
+            }
+            __builtin_amdgcn_s_sleep(2);
+        }
+    }
+    asm volatile("" : : "v"(ahead));
+    __syncthreads();
 }
 
 }  // namespace layer

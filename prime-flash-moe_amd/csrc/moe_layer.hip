@@ -7,59 +7,65 @@ namespace {
 using namespace pmoe;
 using namespace pmoe::layer;
 
-// logits[t][e], four experts per workgroup; its waves share the contraction.
+// logits[t][e]: four experts and up to eight tokens per workgroup, whose waves share the contraction.  Beside that, the queues begin and the
+// activation is marked as absent.
 template <class T>
-__global__ __launch_bounds__(256) void moe_layer_router_kernel(Args a) {
-    __shared__ float part[4][kMaxTokens][4];
-    const int lane = threadIdx.x & 63, wave = gmm::uniform(threadIdx.x >> 6), sub = lane >> 4;
-    const int steps = (a.K + 127) / 128, s0 = wave * steps / 4, s1 = (wave + 1) * steps / 4;
-    const char *const w[1] = {a.gate + (int64_t)min((int)blockIdx.x * 4 + sub, a.E - 1) * a.K * 2};
-    by_rows(a.T, [&](auto n, int row0) {
+__global__ __launch_bounds__(kThreads) void moe_layer_router_kernel(Args a) {
+    __shared__ float part[kWaves][8][4];
+    const int block = blockIdx.y * gridDim.x + blockIdx.x;
+    if (block == 0)
+        for (int i = threadIdx.x; i < (int)(sizeof(Sync) / 4); i += kThreads) reinterpret_cast<int32_t *>(a.sync)[i] = 0;
+    const int64_t words = (int64_t)a.T * a.top_k * 2 * a.act_pitch / 16;
+    for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < words; i += (int64_t)gridDim.x * gridDim.y * kThreads)
+        reinterpret_cast<i32x4 *>(a.act)[i] = i32x4{(int)kAbsent, (int)kAbsent, (int)kAbsent, (int)kAbsent};
+    const int lane = threadIdx.x & 63, wave = gmm::uniform(threadIdx.x >> 6), sub = lane >> 4, t0 = blockIdx.y * 8, rows = min(a.T - t0, 8);
+    const int steps = (a.K + 127) / 128, s0 = wave * steps / kWaves, s1 = (wave + 1) * steps / kWaves;
+    const char *const w[1] = {a.gate + (int64_t)blockIdx.x * 4 * a.K * 2};
+    auto some = [&](auto n) {
         constexpr int N = decltype(n)::value;
-        const char *x[N];
+        uint32_t xo[N];
         float acc[1][N] = {};
 #pragma unroll
-        for (int j = 0; j < N; ++j) x[j] = a.x + (int64_t)min(row0 + j, a.T - 1) * a.K * 2;
-        row_dots<T, 1, N, (N <= 4 ? 4 : 2)>(acc, w, x, s0, s1, a.K);
+        for (int j = 0; j < N; ++j) xo[j] = (uint32_t)(t0 + min(j, rows - 1)) * (uint32_t)a.K * 2;
+        row_dots<T, 1, N, (N <= 4 ? 8 : 4), (N <= 2 ? 8 : N == 4 ? 4 : 2)>(acc, w, a.K * 2, a.x, (uint32_t)a.T * a.K * 2, xo, s0, s1, a.K, 1, min(a.E - 1 - (int)blockIdx.x * 4, 3));
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const float v = row_sum(acc[0][j]);
-            if ((lane & 15) == 0 && row0 + j < a.T) part[wave][row0 + j][sub] = v;
+            if ((lane & 15) == 0) part[wave][j][sub] = v;
         }
-    });
+    };
+    if (rows == 1) some(std::integral_constant<int, 1>{});
+    else if (rows <= 4) some(std::integral_constant<int, 4>{});
+    else some(std::integral_constant<int, 8>{});
     __syncthreads();
     const int t = threadIdx.x >> 2, e = blockIdx.x * 4 + (threadIdx.x & 3);
-    if (t < a.T && e < a.E) {
+    if (t < rows && e < a.E) {
         float v = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v += part[k][t][threadIdx.x & 3];
-        a.logits[(int64_t)t * a.E + e] = v;
+        for (int k = 0; k < kWaves; ++k) v += part[k][t][threadIdx.x & 3];
+        a.logits[(int64_t)(t0 + t) * a.E + e] = v;
     }
 }
 
-template <class W>
-__global__ __launch_bounds__(kThreads) void moe_layer_up_kernel(Args a) {
+template <class W, bool ONE>
+__global__ __launch_bounds__(kThreads, 4) void moe_layer_kernel(Args a, int down_jobs) {
     __shared__ Plan p;
     __shared__ __attribute__((aligned(1024))) Sums sums;
-    find_plan(a, p, blockIdx.x == 0);
-    const int strips = (a.H + kUpCols - 1) / kUpCols, u = (int)blockIdx.x / strips;
-    if (u < p.n) W::up(a, p, sums, u, (int)blockIdx.x - u * strips);
+    int ticket = 0;
+    if (threadIdx.x == 0) ticket = next_ticket(&a.sync->ticket[blockIdx.x % kQueues][0]);
+    find_plan<ONE>(a, p, blockIdx.x == 0);
+    up_jobs<W, ONE>(a, p, sums, ticket, (int)blockIdx.x < down_jobs ? (int)blockIdx.x : -1);
+    for (int job = blockIdx.x; job < down_jobs; job += gridDim.x) down_job<W, ONE>(a, p, sums, job);
 }
 
 template <class W>
-__global__ __launch_bounds__(kThreads) void moe_layer_down_kernel(Args a) {
-    __shared__ Plan p;
-    __shared__ __attribute__((aligned(1024))) Sums sums;
-    find_plan(a, p, false);
-    down_job<W>(a, p, sums, (int)blockIdx.x);
-}
-
-template <class W>
-int launch(const Args &a, hipStream_t s) {
-    hipLaunchKernelGGL((moe_layer_router_kernel<typename W::Type>), dim3((a.E + 3) / 4), dim3(256), 0, s, a);
-    const int most = std::min(a.E, a.T * a.top_k);
-    hipLaunchKernelGGL((moe_layer_up_kernel<W>), dim3(most * ((a.H + kUpCols - 1) / kUpCols)), dim3(kThreads), 0, s, a);
-    hipLaunchKernelGGL((moe_layer_down_kernel<W>), dim3((a.K + W::kDownCols - 1) / W::kDownCols), dim3(kThreads), 0, s, a);
+int launch(Args a, hipStream_t s) {
+    hipLaunchKernelGGL((moe_layer_router_kernel<typename W::Type>), dim3((a.E + 3) / 4, (a.T + 7) / 8), dim3(kThreads), 0, s, a);
+    const int cus = resident_grid(), most = std::min(a.E, a.T * a.top_k), down_strips = (a.K + W::kDownCols - 1) / W::kDownCols;
+    const int64_t up_jobs = (int64_t)most * ((a.H + a.up_cols - 1) / a.up_cols), down_jobs = (int64_t)down_strips * a.n_shares;
+    const dim3 grid((uint32_t)std::min<int64_t>(std::max(up_jobs, down_jobs), 2 * cus)), block(kThreads);
+    if (a.T == 1) hipLaunchKernelGGL((moe_layer_kernel<W, true>), grid, block, 0, s, a, (int)down_jobs);
+    else hipLaunchKernelGGL((moe_layer_kernel<W, false>), grid, block, 0, s, a, (int)down_jobs);
     return check_launch("moe_layer launch");
 }
 template <class T>
@@ -67,14 +73,25 @@ int launch(const Args &a, int group, hipStream_t s) {
     return group == 0 ? launch<Wide<T>>(a, s) : group == 32 ? launch<Narrow<T, 32>>(a, s) : group == 64 ? launch<Narrow<T, 64>>(a, s) : launch<Narrow<T, 128>>(a, s);
 }
 
+// How the jobs of a layer are cut.
+void cut_jobs(Args &a, int group) {
+    const int64_t slots = 2 * resident_grid(), most = std::min(a.E, a.T * a.top_k), quads = most * ((a.H + 3) / 4);
+    const int64_t rounds = (quads + 4 * slots - 1) / (4 * slots);
+    a.up_cols = group != 0 ? 16 : 4 * (int)std::min<int64_t>(4, (quads + rounds * slots - 1) / (rounds * slots));
+    const int64_t strips = group != 0 ? a.K / 16 : (a.K + 7) / 8, bytes = most * 3 * a.H * a.K * 2 / (group != 0 ? 4 : 1);
+    a.shares_log = 0;
+    while (bytes > 128 << 20 && 1 << a.shares_log < kMaxShares && strips << a.shares_log < slots && strips << (a.shares_log + 1) <= kMaxShared) ++a.shares_log;
+    a.n_shares = 1 << a.shares_log;
+}
 size_t act_pitch(int H) { return align_up((size_t)H * 2, 128); }
 size_t logits_bytes(int T, int E) { return align_up((size_t)T * E * 4, 256); }
+static_assert(sizeof(Sync) % 256 == 0, "what follows is aligned");
 
 }  // namespace
 
 extern "C" size_t pmoe_moe_layer_workspace_bytes(int T, int H, int num_experts, int top_k) {
     if (T <= 0 || H <= 0 || num_experts <= 0 || top_k <= 0) return 0;
-    return logits_bytes(T, num_experts) + (size_t)T * top_k * 2 * act_pitch(H);
+    return sizeof(Sync) + logits_bytes(T, num_experts) + (size_t)kMaxShared * 16 * T * 4 + (size_t)T * top_k * 2 * act_pitch(H);
 }
 
 extern "C" int pmoe_moe_layer(const void *x, const void *gate, const float *bias, const void *w1, const void *w1_scale, const void *w2,
@@ -105,14 +122,17 @@ extern "C" int pmoe_moe_layer(const void *x, const void *gate, const float *bias
     a.out = static_cast<char *>(out);
     a.topk_ids = topk_ids;
     a.topk_weights = topk_weights;
-    a.logits = static_cast<float *>(workspace);
-    a.act = static_cast<char *>(workspace) + logits_bytes(T, num_experts);
+    a.sync = static_cast<Sync *>(workspace);
+    a.logits = reinterpret_cast<float *>(a.sync + 1);
+    a.shares = reinterpret_cast<float *>(reinterpret_cast<char *>(a.logits) + logits_bytes(T, num_experts));
+    a.act = reinterpret_cast<char *>(a.shares + (size_t)kMaxShared * 16 * T);
     a.act_pitch = (int)act_pitch(H);
     a.T = T;
     a.K = K;
     a.H = H;
     a.E = num_experts;
     a.top_k = top_k;
+    cut_jobs(a, group);
     hipStream_t s = static_cast<hipStream_t>(stream);
     return dtype == PMOE_DTYPE_BF16 ? launch<Bf16>(a, group, s) : launch<F16>(a, group, s);
 }
