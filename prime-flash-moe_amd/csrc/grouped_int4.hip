@@ -23,7 +23,7 @@ struct Int4Args {
 template <int U, int R, int S, int WAVES>
 union Shared {
     f32x4 sum[WAVES][U * R][64];
-    char rows[WAVES][Rows<R, S>::kBytes];
+    char rows[WAVES][Rows<16 * R, S>::kBytes];
 };
 
 template <class T, int GROUP, int U, int R, int S, int WAVES>

@@ -99,72 +99,67 @@ struct TileScales {
     }
 };
 
-// Rows of x on their way to a wave: S tiles of up to 16 R rows, in LDS of the wave's own.  A load of the wave is 1 KB, four rows
+// Rows of x on their way to a wave: S tiles of up to M rows, in LDS of the wave's own.  A load of the wave is 1 KB, four rows
 // of a tile, where the operands of its matrix instructions would be 64 bytes of 16 rows each, most of them the same row again: one
 // load per tile instead of four for up to four rows.  Row q of tile i is 256 bytes, its chunk of 16 bytes k in slot k ^ q % 16: the
 // reads of 16 rows cover all banks.
-template <int R, int S>
+template <int M, int S>
 struct Rows {
-    i32x4 v[S * R * 4];
-    // `x(q)`: begins row q; `n`: rows, from 1 to 16 R (both wave-uniform but for the lane's q); get(address): 16 bytes.
-    template <class X, class Get>
-    __device__ __forceinline__ void load(X x, Get get, int n, int t, int t1, int k) {
-        const int lane = threadIdx.x & 63, sub = lane >> 4, e = (lane & 15) * 8;
+    static_assert(M % 4 == 0, "four rows a load");
+    static constexpr int kBytes = S * M * 256;
+    i32x4 v[S][M / 4];
+    // f(tile, load) for what there is of `n` rows and tiles t .. t1 - 1.
+    template <class F>
+    static __device__ __forceinline__ void each(int n, int t, int t1, F f) {
 #pragma unroll
         for (int i = 0; i < S; ++i)
             if (i == 0 || t + i < t1) {
-                const int col = (t + i) * kTileCols + e;
 #pragma unroll
-                for (int g = 0; g < R * 4; ++g)
-                    if (g == 0 || 4 * g < n) {
-                        v[i * R * 4 + g] = i32x4{0, 0, 0, 0};
-                        if (col < k) v[i * R * 4 + g] = get(x(min(4 * g + sub, n - 1)) + (int64_t)col * 2);
-                    }
+                for (int g = 0; g < M / 4; ++g)
+                    if (g == 0 || 4 * g < n) f(i, g);
             }
+    }
+    // `x(q)`: begins row q; `n`: rows, from 1 to M (both wave-uniform but for the lane's q); get(address): 16 bytes.
+    template <class X, class Get>
+    __device__ __forceinline__ void load(X x, Get get, int n, int t, int t1, int k) {
+        const int lane = threadIdx.x & 63, sub = lane >> 4, e = (lane & 15) * 8;
+        each(n, t, t1, [&](int i, int g) {
+            const int col = (t + i) * kTileCols + e;
+            v[i][g] = i32x4{0, 0, 0, 0};
+            if (col < k) v[i][g] = get(x(min(4 * g + sub, n - 1)) + (int64_t)col * 2);
+        });
     }
     // The largest of the words that were loaded.
     __device__ __forceinline__ uint32_t most(int n, int t, int t1) const {
         uint32_t m = 0;
+        each(n, t, t1, [&](int i, int g) {
 #pragma unroll
-        for (int i = 0; i < S; ++i)
-            if (i == 0 || t + i < t1) {
-#pragma unroll
-                for (int g = 0; g < R * 4; ++g)
-                    if (g == 0 || 4 * g < n) {
-#pragma unroll
-                        for (int d = 0; d < 4; ++d) m = max(m, (uint32_t)v[i * R * 4 + g][d]);
-                    }
-            }
+            for (int d = 0; d < 4; ++d) m = max(m, (uint32_t)v[i][g][d]);
+        });
         return m;
     }
     __device__ __forceinline__ void store(char *lds, int n, int t, int t1) const {
         const int lane = threadIdx.x & 63, sub = lane >> 4;
-#pragma unroll
-        for (int i = 0; i < S; ++i)
-            if (i == 0 || t + i < t1) {
-#pragma unroll
-                for (int g = 0; g < R * 4; ++g)
-                    if (g == 0 || 4 * g < n)
-                        *reinterpret_cast<i32x4 *>(lds + ((i * 16 * R + 4 * g + sub) * 256 + (((lane & 15) ^ (4 * g + sub)) & 15) * 16)) = v[i * R * 4 + g];
-            }
+        each(n, t, t1, [&](int i, int g) {
+            *reinterpret_cast<i32x4 *>(lds + ((i * M + 4 * g + sub) * 256 + (((lane & 15) ^ (4 * g + sub)) & 15) * 16)) = v[i][g];
+        });
     }
     // Operand of row 16 q + r, columns 32 j + 8 c .. + 7 of tile i.
     static __device__ __forceinline__ i32x4 read(const char *lds, int n, int i, int q, int j) {
         const int lane = threadIdx.x & 63, row = min(16 * q + (lane & 15), n - 1);
-        return *reinterpret_cast<const i32x4 *>(lds + (i * 16 * R + row) * 256 + (((4 * j + (lane >> 4)) ^ row) & 15) * 16);
+        return *reinterpret_cast<const i32x4 *>(lds + (i * M + row) * 256 + (((4 * j + (lane >> 4)) ^ row) & 15) * 16);
     }
-    static constexpr int kBytes = S * R * 16 * 256;
 };
 
 // acc[u][q] += n rows of x times the weights of tiles t0 .. t1 - 1 of U strips (16 weight rows each), for one wave.  Lane l, r = l %
 // 16, c = l / 16: `w[u]`, `s[u]` begin strip u.  acc[u][q][i]: weight row r, row 16 q + 4 c + i of x (any of the n where there are fewer).
-// `k`: columns; nothing of x is read behind them.  `lds`: Rows<R, S>::kBytes of the wave's own.  S: tiles whose loads are in flight
+// `k`: columns; nothing of x is read behind them.  M: rows at most, `lds`: Rows<M, S>::kBytes of the wave's own.  S: tiles whose loads are in flight
 // together; what hides the rest of their latency is other waves.  wait(most): called with the largest word of what was loaded of x, for
 // rows that may not all be there yet: true until they are.
 struct NoWait {
     static constexpr bool kWaits = false;
 };
-template <class T, int GROUP, int U, int R, int S, class X, class Wait = NoWait>
+template <class T, int GROUP, int U, int R, int S, int M = 16 * R, class X, class Wait = NoWait>
 __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[U], const char *const (&s)[U], X x, int n, int t0, int t1, int k, char *lds, Wait wait = {}) {
     using Sc = TileScales<GROUP>;
     constexpr int PER = GROUP / 32;
@@ -173,7 +168,7 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
     for (int t = t0; t < t1; t += S) {
         i32x4 wv[S][U];
         Sc sc[S][U];
-        Rows<R, S> rows;
+        Rows<M, S> rows;
         rows.load(x, [](const char *p) { return *reinterpret_cast<const i32x4 *>(p); }, n, t, t1, k);
 #pragma unroll
         for (int i = 0; i < S; ++i)
@@ -199,7 +194,7 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
                         less[q] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                         for (int j = 0; j < PER; ++j) {
-                            xv[q][j] = Rows<R, S>::read(lds, n, i, q, g * PER + j);
+                            xv[q][j] = Rows<M, S>::read(lds, n, i, q, g * PER + j);
                             less[q] = gmm::few::Mini<T>::mfma(xv[q][j], minus, less[q]);
                         }
                     }

@@ -37,6 +37,7 @@ constexpr int64_t kMostTries = 1 << 24;  // of a wait, about a microsecond each:
 constexpr int kQueues = 8;  // as many as XCDs, which workgroups go round
 struct Sync {
     int32_t ticket[kQueues][32];
+    int32_t down[64];                 // down jobs taken behind the first one of every workgroup
     int32_t arrived[kMaxShared / 2];  // strip of out: workgroups that have their share of a strip of out
 };
 struct Args {
@@ -196,6 +197,7 @@ struct Plan {
     int n;                              // touched experts
     int job;                            // the workgroup's
     int failed;                         // a wait was given up
+    int next;                           // down job
     uint32_t touched[kMaxExperts / 32];
     uint16_t expert[kMaxPairs];
     uint32_t tokens[kMaxPairs];         // bit t: token t is the expert's
@@ -329,6 +331,16 @@ __device__ __forceinline__ void by_rows(int n, F f) {
     }
 }
 
+// How many rows at most a wave's piece of LDS is laid out for (4, 8 or 16; the fewer, the more tiles are on their way at a time).
+template <bool ONE, class F>
+__device__ __forceinline__ void by_height(int n, F f) {
+    if (ONE || n <= 4) return f(std::integral_constant<int, 4>{});
+    if constexpr (!ONE) {
+        if (n <= 8) f(std::integral_constant<int, 8>{});
+        else f(std::integral_constant<int, 16>{});
+    }
+}
+
 // Two 16-bit numbers that add up to v (of what is beyond the type the first alone; one NaN for all, see kAbsent).
 template <class T>
 __device__ __forceinline__ uint32_t split(float v) {
@@ -337,7 +349,6 @@ __device__ __forceinline__ uint32_t split(float v) {
     return hi | (uint32_t)lo << 16;
 }
 
-using Rows = int4::Rows<1, 1>;
 struct UpSums {
     float part[kWaves][2][kMaxTokens][kUpCols];  // [part of the contraction][gate, up][row][column]
 };
@@ -349,7 +360,7 @@ struct Sums {
         UpSums up;
         DownSums down;
     };
-    char rows[kWaves][Rows::kBytes];  // rows of x or of the activation on their way to a wave
+    char rows[kWaves][4096];  // rows of x or of the activation on their way to a wave (int4::Rows: 16 of a tile, 8 of two, 4 of four)
 };
 
 // What the columns of an up job have from every wave -> activation, two columns a thread.  The stores go through to where all XCDs see
@@ -372,8 +383,8 @@ __device__ __forceinline__ void finish_up(const Args &a, const Plan &p, const Up
     }
 }
 
-// Weights of 16 bits.
-template <class T>
+// Weights of 16 bits.  QUADS: of four columns, that an up job has at most.
+template <class T, int QUADS>
 struct Wide {
     using Type = T;
     static constexpr int kDownCols = 8;
@@ -385,9 +396,9 @@ struct Wide {
         const int steps = (a.K + 127) / 128, s0 = wave * steps >> kWavesLog, s1 = (wave + 1) * steps >> kWavesLog;
         const uint32_t tokens = tokens_of<ONE>(p, u);
         const char *const gate = a.w1 + (int64_t)gmm::uniform(p.expert[u]) * 2 * a.H * a.K * 2;
-        const char *w[kUpCols / 2];
+        const char *w[2 * QUADS];
 #pragma unroll
-        for (int q = 0; q < kUpCols / 4; ++q) {
+        for (int q = 0; q < QUADS; ++q) {
             const int col = min(strip * a.up_cols + 4 * q, a.H - 4);  // (H is a multiple of 4: all four are inside or none)
             w[2 * q] = gate + (int64_t)col * a.K * 2;
             w[2 * q + 1] = gate + (int64_t)(a.H + col) * a.K * 2;
@@ -396,12 +407,13 @@ struct Wide {
             constexpr int N = decltype(n)::value;
             const int last = __popc(tokens) - 1;
             uint32_t xo[N];
-            float acc[kUpCols / 2][N] = {};
+            float acc[2 * QUADS][N] = {};
 #pragma unroll
             for (int j = 0; j < N; ++j) xo[j] = ONE ? 0 : (uint32_t)token_of(tokens, min(row0 + j, last)) * (uint32_t)a.K * 2;
-            row_dots<T, kUpCols / 2, N, (N <= 2 ? 2 : 1), (N <= 2 ? 2 : 1)>(acc, w, a.K * 2, a.x, (uint32_t)a.T * a.K * 2, xo, s0, s1, a.K, 2 * quads);
+            constexpr int S = QUADS == 1 ? (N == 1 ? 8 : N == 2 ? 6 : 4) : N <= 2 ? 2 : 1, SX = QUADS == 1 ? (N == 1 ? 8 : N == 2 ? 3 : 2) : S;
+            row_dots<T, 2 * QUADS, N, S, SX>(acc, w, a.K * 2, a.x, (uint32_t)a.T * a.K * 2, xo, s0, s1, a.K, 2 * quads);
 #pragma unroll
-            for (int q = 0; q < kUpCols / 4; ++q)
+            for (int q = 0; q < QUADS; ++q)
                 if (q < quads)
 #pragma unroll
                     for (int j = 0; j < N; ++j) {
@@ -480,7 +492,8 @@ struct Narrow {
         const char *const w[2] = {a.w1 + first * tiles * int4::kTileBytes, a.w1 + (first + strips) * tiles * int4::kTileBytes};
         const char *const s[2] = {a.w1_scale + first * tiles * SB, a.w1_scale + (first + strips) * tiles * SB};
         f32x4 acc[2][1] = {};
-        int4::dots<T, GROUP, 2, 1, 1>(acc, w, s, [&](int q) { return a.x + (ONE ? 0 : (int64_t)token_of(tokens, q) * a.K * 2); }, last + 1, t0, t1, a.K, rows);
+        auto row = [&](int q) { return a.x + (ONE ? 0 : (int64_t)token_of(tokens, q) * a.K * 2); };
+        by_height<ONE>(last + 1, [&](auto m) { int4::dots<T, GROUP, 2, 1, (decltype(m)::value == 4 ? 2 : 16 / decltype(m)::value), decltype(m)::value>(acc, w, s, row, last + 1, t0, t1, a.K, rows); });
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums.part[wave][0][4 * c + i][r] = acc[0][0][i], sums.part[wave][1][4 * c + i][r] = acc[1][0][i];
     }
@@ -510,7 +523,8 @@ struct Narrow {
                 const int t = ONE ? 0 : token_of(tokens, row0 + q / 2);
                 return a.act + ((int64_t)pair_of<ONE>(a, p, u, t) * 2 + (q & 1)) * a.act_pitch;
             };
-            int4::dots<T, GROUP, 1, 1, 1>(acc, w, s, row, 2 * min(last + 1 - row0, 8), t0, t1, a.H, rows, Arrival{&p.failed});
+            const int n = 2 * min(last + 1 - row0, 8);
+            by_height<ONE>(n, [&](auto m) { int4::dots<T, GROUP, 1, 1, 16 / decltype(m)::value, decltype(m)::value>(acc, w, s, row, n, t0, t1, a.H, rows, Arrival{&p.failed}); });
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int j = row0 + 2 * c + i;
@@ -581,7 +595,6 @@ __device__ __forceinline__ void down_job(const Args &a, Plan &p, Sums &sh, int j
     }
     if (last && mine && strip * C + c < a.K)
         reinterpret_cast<uint16_t *>(a.out)[(int64_t)t * a.K + strip * C + c] = Num<typename W::Type>::from_f32(p.failed ? __uint_as_float(0x7fc00000u) : v);
-    __syncthreads();  // the sums may be cleared again
 }
 
 // The up jobs, (touched expert, up_cols columns), job j in queue j % 8; a workgroup takes those of its own queue, `ticket` its first, and then

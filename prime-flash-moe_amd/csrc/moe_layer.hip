@@ -7,19 +7,14 @@ namespace {
 using namespace pmoe;
 using namespace pmoe::layer;
 
-// logits[t][e]: four experts and up to eight tokens per workgroup, whose waves share the contraction.  Beside that, the queues begin and the
+// logits[t][e]: four experts and up to four tokens per workgroup, whose waves share the contraction.  Beside that, the queues begin and the
 // activation is marked as absent.
+constexpr int kRouterTokens = 4;
 template <class T>
 __global__ __launch_bounds__(kThreads) void moe_layer_router_kernel(Args a) {
-    __shared__ float part[kWaves][8][4];
-    const int block = blockIdx.y * gridDim.x + blockIdx.x;
-    if (block == 0)
-        for (int i = threadIdx.x; i < (int)(sizeof(Sync) / 4); i += kThreads) reinterpret_cast<int32_t *>(a.sync)[i] = 0;
-    const int64_t words = (int64_t)a.T * a.top_k * 2 * a.act_pitch / 16;
-    for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < words; i += (int64_t)gridDim.x * gridDim.y * kThreads)
-        reinterpret_cast<i32x4 *>(a.act)[i] = i32x4{(int)kAbsent, (int)kAbsent, (int)kAbsent, (int)kAbsent};
-    const int lane = threadIdx.x & 63, wave = gmm::uniform(threadIdx.x >> 6), sub = lane >> 4, t0 = blockIdx.y * 8, rows = min(a.T - t0, 8);
-    const int steps = (a.K + 127) / 128, s0 = wave * steps / kWaves, s1 = (wave + 1) * steps / kWaves;
+    __shared__ float part[kWaves][kRouterTokens][4];
+    const int lane = threadIdx.x & 63, wave = gmm::uniform(threadIdx.x >> 6), sub = lane >> 4, t0 = blockIdx.y * kRouterTokens, rows = min(a.T - t0, kRouterTokens);
+    const int steps = (a.K + 127) / 128, s0 = wave * steps >> kWavesLog, s1 = (wave + 1) * steps >> kWavesLog;
     const char *const w[1] = {a.gate + (int64_t)blockIdx.x * 4 * a.K * 2};
     auto some = [&](auto n) {
         constexpr int N = decltype(n)::value;
@@ -27,7 +22,7 @@ __global__ __launch_bounds__(kThreads) void moe_layer_router_kernel(Args a) {
         float acc[1][N] = {};
 #pragma unroll
         for (int j = 0; j < N; ++j) xo[j] = (uint32_t)(t0 + min(j, rows - 1)) * (uint32_t)a.K * 2;
-        row_dots<T, 1, N, (N <= 4 ? 8 : 4), (N <= 2 ? 8 : N == 4 ? 4 : 2)>(acc, w, a.K * 2, a.x, (uint32_t)a.T * a.K * 2, xo, s0, s1, a.K, 1, min(a.E - 1 - (int)blockIdx.x * 4, 3));
+        row_dots<T, 1, N, 4, 4>(acc, w, a.K * 2, a.x, (uint32_t)a.T * a.K * 2, xo, s0, s1, a.K, 1, min(a.E - 1 - (int)blockIdx.x * 4, 3));
 #pragma unroll
         for (int j = 0; j < N; ++j) {
             const float v = row_sum(acc[0][j]);
@@ -35,8 +30,14 @@ __global__ __launch_bounds__(kThreads) void moe_layer_router_kernel(Args a) {
         }
     };
     if (rows == 1) some(std::integral_constant<int, 1>{});
-    else if (rows <= 4) some(std::integral_constant<int, 4>{});
-    else some(std::integral_constant<int, 8>{});
+    else some(std::integral_constant<int, kRouterTokens>{});
+    const int block = blockIdx.y * gridDim.x + blockIdx.x;
+    if (block == 0)
+        for (int i = threadIdx.x; i < (int)(sizeof(Sync) / 4); i += kThreads) reinterpret_cast<int32_t *>(a.sync)[i] = 0;
+    const int64_t words = (int64_t)a.T * a.top_k * 2 * a.act_pitch / 16;
+#pragma unroll 1
+    for (int64_t i = (int64_t)block * kThreads + threadIdx.x; i < words; i += (int64_t)gridDim.x * gridDim.y * kThreads)
+        reinterpret_cast<i32x4 *>(a.act)[i] = i32x4{(int)kAbsent, (int)kAbsent, (int)kAbsent, (int)kAbsent};
     __syncthreads();
     const int t = threadIdx.x >> 2, e = blockIdx.x * 4 + (threadIdx.x & 3);
     if (t < rows && e < a.E) {
@@ -55,12 +56,20 @@ __global__ __launch_bounds__(kThreads, 4) void moe_layer_kernel(Args a, int down
     if (threadIdx.x == 0) ticket = next_ticket(&a.sync->ticket[blockIdx.x % kQueues][0]);
     find_plan<ONE>(a, p, blockIdx.x == 0);
     up_jobs<W, ONE>(a, p, sums, ticket, (int)blockIdx.x < down_jobs ? (int)blockIdx.x : -1);
-    for (int job = blockIdx.x; job < down_jobs; job += gridDim.x) down_job<W, ONE>(a, p, sums, job);
+    const bool more = down_jobs > (int)gridDim.x;
+    for (int job = blockIdx.x; job < down_jobs;) {
+        if (more && threadIdx.x == 0) ticket = next_ticket(a.sync->down);
+        down_job<W, ONE>(a, p, sums, job);
+        if (!more) break;
+        if (threadIdx.x == 0) p.next = (int)gridDim.x + ticket;
+        __syncthreads();  // the sums may be cleared again
+        job = gmm::uniform(p.next);
+    }
 }
 
 template <class W>
 int launch(Args a, hipStream_t s) {
-    hipLaunchKernelGGL((moe_layer_router_kernel<typename W::Type>), dim3((a.E + 3) / 4, (a.T + 7) / 8), dim3(kThreads), 0, s, a);
+    hipLaunchKernelGGL((moe_layer_router_kernel<typename W::Type>), dim3((a.E + 3) / 4, (a.T + kRouterTokens - 1) / kRouterTokens), dim3(kThreads), 0, s, a);
     const int cus = resident_grid(), most = std::min(a.E, a.T * a.top_k), down_strips = (a.K + W::kDownCols - 1) / W::kDownCols;
     const int64_t up_jobs = (int64_t)most * ((a.H + a.up_cols - 1) / a.up_cols), down_jobs = (int64_t)down_strips * a.n_shares;
     const dim3 grid((uint32_t)std::min<int64_t>(std::max(up_jobs, down_jobs), 2 * cus)), block(kThreads);
@@ -70,14 +79,16 @@ int launch(Args a, hipStream_t s) {
 }
 template <class T>
 int launch(const Args &a, int group, hipStream_t s) {
-    return group == 0 ? launch<Wide<T>>(a, s) : group == 32 ? launch<Narrow<T, 32>>(a, s) : group == 64 ? launch<Narrow<T, 64>>(a, s) : launch<Narrow<T, 128>>(a, s);
+    return group == 0 ? (a.up_cols == 4 ? launch<Wide<T, 1>>(a, s) : launch<Wide<T, 4>>(a, s)) : group == 32 ? launch<Narrow<T, 32>>(a, s) : group == 64 ? launch<Narrow<T, 64>>(a, s) : launch<Narrow<T, 128>>(a, s);
 }
 
 // How the jobs of a layer are cut.
 void cut_jobs(Args &a, int group) {
     const int64_t slots = 2 * resident_grid(), most = std::min(a.E, a.T * a.top_k), quads = most * ((a.H + 3) / 4);
-    const int64_t rounds = (quads + 4 * slots - 1) / (4 * slots);
-    a.up_cols = group != 0 ? 16 : 4 * (int)std::min<int64_t>(4, (quads + rounds * slots - 1) / (rounds * slots));
+    // One round of the grid where they are so few, otherwise jobs of 128 KB or the next thing below: where a job is large, what some
+    // workgroups have left at the end is.
+    const int64_t most_cols = quads <= 4 * slots ? (quads + slots - 1) / slots : std::max<int64_t>(1, (128 << 10) / (16 * a.K));
+    a.up_cols = group != 0 ? 16 : 4 * (int)std::min<int64_t>(4, most_cols);
     const int64_t strips = group != 0 ? a.K / 16 : (a.K + 7) / 8, bytes = most * 3 * a.H * a.K * 2 / (group != 0 ? 4 : 1);
     a.shares_log = 0;
     while (bytes > 128 << 20 && 1 << a.shares_log < kMaxShares && strips << a.shares_log < slots && strips << (a.shares_log + 1) <= kMaxShared) ++a.shares_log;
