@@ -29,16 +29,14 @@ using int4::Num;
 constexpr int kMaxTokens = 16, kMaxTopK = 32, kMaxPairs = kMaxTokens * kMaxTopK, kMaxExperts = 512;
 constexpr int kThreads = 512, kWaves = 8, kWavesLog = 3;
 constexpr int kUpCols = 16;       // activation columns of an up job at most
-constexpr int kMaxShares = 4;     // workgroups that share a strip of out
-constexpr int kMaxShared = 1024;  // shares of all strips at most, if they are shared
+constexpr int kMaxGroups = 512;   // workgroups at most
 constexpr int64_t kMostTries = 1 << 24;  // of a wait, about a microsecond each: then the outputs are NaN
 
 // Queues of the up jobs, a line of 128 bytes each (an atomic of the device takes 11 ns per address).
 constexpr int kQueues = 8;  // as many as XCDs, which workgroups go round
 struct Sync {
     int32_t ticket[kQueues][32];
-    int32_t down[64];                 // down jobs taken behind the first one of every workgroup
-    int32_t arrived[kMaxShared / 2];  // strip of out: workgroups that have their share of a strip of out
+    int32_t arrived[kMaxGroups];  // of the strip of out that begins with this workgroup: steps of its contraction that are done
 };
 struct Args {
     Sync *sync;
@@ -50,11 +48,11 @@ struct Args {
     float *logits;  // (T, E)
     char *act;      // [pair][2: value, rest][act_pitch bytes]
     int act_pitch;
-    float *shares;  // [strip of out][share][token][column]: sums of workgroups that share a strip
+    float *shares;  // [workgroup][2: of its first strip, of its last one][token][column]: sums of workgroups that share a strip of out
     int T, K, H, E, top_k;
     int up_cols;    // columns of an up job, a multiple of 4
-    int n_shares;   // 1 << shares_log
-    int shares_log;
+    int down_groups;  // workgroups of the down projection
+    int split;        // whether they share strips of out
 };
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
@@ -197,7 +195,6 @@ struct Plan {
     int n;                              // touched experts
     int job;                            // the workgroup's
     int failed;                         // a wait was given up
-    int next;                           // down job
     uint32_t touched[kMaxExperts / 32];
     uint16_t expert[kMaxPairs];
     uint32_t tokens[kMaxPairs];         // bit t: token t is the expert's
@@ -423,21 +420,20 @@ struct Wide {
         });
     }
 
-    // Address of line `lane` of a wave's share of a down job (null: it has fewer).
-    static __device__ __forceinline__ const char *down_line(const Args &a, const Plan &p, int u, int strip, int part, int parts_log, int lane) {
-        const int steps = (a.H + 127) / 128, s0 = part * steps >> parts_log, lines = (((part + 1) * steps >> parts_log) - s0) * 2;
+    static __device__ __forceinline__ int down_steps(const Args &a) { return (a.H + 127) / 128; }
+    // Address of line `lane` of steps s0 .. s1 - 1 of a strip of out (null: there are fewer).
+    static __device__ __forceinline__ const char *down_line(const Args &a, const Plan &p, int u, int strip, int s0, int s1, int lane) {
         const int row = lane % 8, line = lane / 8, at = s0 * 256 + line * 128;
-        return line < lines && at < a.H * 2 ? down_weights(a, p, u, strip) + (int64_t)row * a.H * 2 + at : nullptr;
+        return line < (s1 - s0) * 2 && at < a.H * 2 ? down_weights(a, p, u, strip) + (int64_t)row * a.H * 2 + at : nullptr;
     }
     static __device__ __forceinline__ const char *down_weights(const Args &a, const Plan &p, int u, int strip) {
         return a.w2 + ((int64_t)gmm::uniform(p.expert[u]) * a.K + strip * kDownCols) * a.H * 2;
     }
 
-    // sums[.][.] += expert u's share, part `part` of 1 << parts_log of its contraction, of 8 columns of out.
+    // y[.][.] += steps s0 .. s1 - 1 of expert u's share of a strip of out.
     template <bool ONE>
-    static __device__ __forceinline__ void down(const Args &a, Plan &p, float (&y)[kMaxTokens][16], char *rows, int u, int strip, int part, int parts_log) {
+    static __device__ __forceinline__ void down(const Args &a, Plan &p, float (&y)[kMaxTokens][16], char *rows, int u, int strip, int s0, int s1) {
         const int lane = threadIdx.x & 63, sub = lane >> 4;
-        const int steps = (a.H + 127) / 128, s0 = part * steps >> parts_log, s1 = (part + 1) * steps >> parts_log;
         const uint32_t tokens = tokens_of<ONE>(p, u);
         const char *const first = down_weights(a, p, u, strip);
         const char *const w[2] = {first, first + (int64_t)4 * a.H * 2};
@@ -498,18 +494,18 @@ struct Narrow {
         for (int i = 0; i < 4; ++i) sums.part[wave][0][4 * c + i][r] = acc[0][0][i], sums.part[wave][1][4 * c + i][r] = acc[1][0][i];
     }
 
-    static __device__ __forceinline__ const char *down_line(const Args &a, const Plan &p, int u, int strip, int part, int parts_log, int lane) {
-        const int tiles = int4::tiles_of(a.H), t0 = part * tiles >> parts_log, t1 = (part + 1) * tiles >> parts_log;
-        return lane < (t1 - t0) * (int4::kTileBytes / 128) ? down_weights(a, p, u, strip) + (int64_t)t0 * int4::kTileBytes + lane * 128 : nullptr;
+    static __device__ __forceinline__ int down_steps(const Args &a) { return int4::tiles_of(a.H); }
+    static __device__ __forceinline__ const char *down_line(const Args &a, const Plan &p, int u, int strip, int s0, int s1, int lane) {
+        return lane < (s1 - s0) * (int4::kTileBytes / 128) ? down_weights(a, p, u, strip) + (int64_t)s0 * int4::kTileBytes + lane * 128 : nullptr;
     }
     static __device__ __forceinline__ const char *down_weights(const Args &a, const Plan &p, int u, int strip) {
         return a.w2 + ((int64_t)gmm::uniform(p.expert[u]) * (a.K / 16) + strip) * int4::tiles_of(a.H) * int4::kTileBytes;
     }
 
     template <bool ONE>
-    static __device__ __forceinline__ void down(const Args &a, Plan &p, float (&y)[kMaxTokens][16], char *rows, int u, int strip, int part, int parts_log) {
+    static __device__ __forceinline__ void down(const Args &a, Plan &p, float (&y)[kMaxTokens][16], char *rows, int u, int strip, int s0, int s1) {
         const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
-        const int tiles = int4::tiles_of(a.H), t0 = part * tiles >> parts_log, t1 = (part + 1) * tiles >> parts_log;
+        const int tiles = int4::tiles_of(a.H);
         const uint32_t tokens = tokens_of<ONE>(p, u);
         const int last = __popc(tokens) - 1;
         constexpr int SB = int4::TileScales<GROUP>::kBytes;
@@ -524,7 +520,7 @@ struct Narrow {
                 return a.act + ((int64_t)pair_of<ONE>(a, p, u, t) * 2 + (q & 1)) * a.act_pitch;
             };
             const int n = 2 * min(last + 1 - row0, 8);
-            by_height<ONE>(n, [&](auto m) { int4::dots<T, GROUP, 1, 1, 16 / decltype(m)::value, decltype(m)::value>(acc, w, s, row, n, t0, t1, a.H, rows, Arrival{&p.failed}); });
+            by_height<ONE>(n, [&](auto m) { int4::dots<T, GROUP, 1, 1, 16 / decltype(m)::value, decltype(m)::value>(acc, w, s, row, n, s0, s1, a.H, rows, Arrival{&p.failed}); });
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int j = row0 + 2 * c + i;
@@ -544,65 +540,82 @@ __device__ __forceinline__ int add_device(int32_t *p, int n) { return __hip_atom
 // waits at once.)
 __device__ __forceinline__ int next_ticket(int32_t *p) { return (int)__builtin_amdgcn_atomic_inc32(reinterpret_cast<uint32_t *>(p), ~0u, __ATOMIC_RELAXED, "agent"); }
 
-// Who does what of a strip of out, kDownCols columns: the waves of all workgroups that share it take the experts by turns; where these are
-// fewer, several waves share the contraction of each.
-struct Turn {
-    int first, step;      // experts of this wave
-    int part, parts_log;  // of their contraction
-    __device__ __forceinline__ Turn(const Args &a, int n, int share) {
-        const int wave = gmm::uniform(threadIdx.x >> 6), all = kWaves * a.n_shares, me = share * kWaves + wave;
-        parts_log = 0;
-        while (n << (parts_log + 1) <= all) ++parts_log;
-        first = me >> parts_log;
-        step = all >> parts_log;
-        part = me & ((1 << parts_log) - 1);
-    }
+// Who does what of the down projection.  A strip of out, kDownCols columns, is n `down_steps` steps: those of the touched experts, one
+// behind the other.  All strips in a row are cut into `down_groups` pieces of one length (or of whole strips), and what a workgroup has of a
+// strip into one for each wave, wherever that is in an expert: no wave has more than one step more than others, whatever the numbers of strips
+// and experts.
+struct Place {
+    int strip, step;  // of the strip
+};
+template <class W>
+__device__ __forceinline__ Place place_of(const Args &a, int group, int all) {
+    const uint32_t strips = (a.K + W::kDownCols - 1) / W::kDownCols, at = (uint32_t)group * strips, g = (uint32_t)a.down_groups, strip = at / g;
+    return {(int)strip, a.split ? (int)((at - strip * g) * (uint32_t)all / g) : 0};
+}
+// The steps of a strip that are between two places.
+struct Steps {
+    int from, to;
+    __device__ __forceinline__ Steps(Place p0, Place p1, int strip, int all) : from(strip == p0.strip ? p0.step : 0), to(strip == p1.strip ? p1.step : all) {}
 };
 
-// Job (strip, share).  A wave's sums are its own; they are added up in the order of the waves, and those of the workgroups that share
-// a strip, by the last of them to arrive, in the order of the shares.
+// A workgroup's share of a strip.  A wave's sums are its own; they are added up in the order of the waves, and those of the workgroups that
+// share a strip, by the last of them to arrive, in the order of the workgroups.
 template <class W, bool ONE>
-__device__ __forceinline__ void down_job(const Args &a, Plan &p, Sums &sh, int job) {
+__device__ __forceinline__ void down_job(const Args &a, Plan &p, Sums &sh, int strip, Steps mine, int each, int all) {
     DownSums &sums = sh.down;
-    const int tid = threadIdx.x, wave = gmm::uniform(tid >> 6), lane = tid & 63, strip = job >> a.shares_log, share = job & (a.n_shares - 1);
-    const Turn turn(a, p.n, share);
+    const int tid = threadIdx.x, wave = gmm::uniform(tid >> 6), lane = tid & 63;
     float(&y)[kMaxTokens][16] = sums.y[wave];
 #pragma unroll
     for (int i = 0; i < (ONE ? 1 : kMaxTokens * 16 / 64); ++i) (&y[0][0])[i * 64 + lane] = 0.f;
-    for (int u = turn.first; u < p.n; u += turn.step) W::template down<ONE>(a, p, y, sh.rows[wave], u, strip, turn.part, turn.parts_log);
+    const int n = mine.to - mine.from, end = mine.from + ((wave + 1) * n >> kWavesLog);
+    int at = mine.from + (wave * n >> kWavesLog), u = at / each, s0 = at - u * each;
+    while (at < end) {
+        const int s1 = min(each, s0 + end - at);
+        W::template down<ONE>(a, p, y, sh.rows[wave], u, strip, s0, s1);
+        at += s1 - s0, ++u, s0 = 0;
+    }
     __syncthreads();
     constexpr int C = W::kDownCols;
     const int t = tid / C, c = tid % C;
-    const bool mine = tid < a.T * C;
+    const bool has = tid < a.T * C;
     float v = 0.f;
-    if (mine) {
+    if (has) {
 #pragma unroll
         for (int k = 0; k < kWaves; ++k) v += sums.y[k][t][c];
     }
     bool last = true;
-    if (a.n_shares > 1) {
-        float *const all = a.shares + (int64_t)strip * a.n_shares * a.T * C;
-        if (mine) __hip_atomic_store(all + share * a.T * C + tid, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (n < all) {
+        // (what begins a strip is its workgroup's last share, everything else the first)
+        const int64_t size = a.T * C;
+        if (has) __hip_atomic_store(a.shares + (2 * (int)blockIdx.x + (mine.from == 0)) * size + tid, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
         __syncthreads();
-        if (tid == 0) p.job = add_device(&a.sync->arrived[strip], 1);
+        const int strips = (a.K + C - 1) / C, g0 = (int)((uint32_t)strip * (uint32_t)a.down_groups / (uint32_t)strips);
+        if (tid == 0) p.job = add_device(&a.sync->arrived[g0], n) + n;
         __syncthreads();
-        last = p.job == a.n_shares - 1;
-        if (last && mine) {
+        last = p.job == all;
+        if (last && has) {
             v = 0.f;
-            for (int k = 0; k < a.n_shares; ++k) v += __hip_atomic_load(all + k * a.T * C + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            Place from = place_of<W>(a, g0, all);
+            for (int g = g0; g < a.down_groups && from.strip <= strip; ++g) {
+                const Place to = place_of<W>(a, g + 1, all);
+                const Steps s(from, to, strip, all);
+                if (s.from < s.to) v += __hip_atomic_load(a.shares + (2 * g + (s.from == 0)) * size + tid, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                from = to;
+            }
         }
     }
-    if (last && mine && strip * C + c < a.K)
+    if (last && has && strip * C + c < a.K)
         reinterpret_cast<uint16_t *>(a.out)[(int64_t)t * a.K + strip * C + c] = Num<typename W::Type>::from_f32(p.failed ? __uint_as_float(0x7fc00000u) : v);
+    __syncthreads();  // the sums may be cleared again
 }
 
 // The up jobs, (touched expert, up_cols columns), job j in queue j % 8; a workgroup takes those of its own queue, `ticket` its first, and then
 // what other queues have left.  Returns when all have been taken: what a workgroup waits for then is with workgroups that run and do not
 // wait, so that a wait ends whatever else is on the device and however few workgroups fit on it.
-// Meanwhile the first weights of `down`, the workgroup's first down job (negative: it has none, and returns), are brought into the L2.
+// Meanwhile the first weights of the workgroup's part of the down projection, if it has one, are brought into the L2.
 template <class W, bool ONE>
-__device__ __forceinline__ void up_jobs(const Args &a, Plan &p, Sums &sh, int ticket, int down) {
+__device__ __forceinline__ void up_jobs(const Args &a, Plan &p, Sums &sh, int ticket, Place down, Steps mine, int each, bool down_too) {
     const int tid = threadIdx.x, lane = tid & 63, home = blockIdx.x % kQueues;
     const int strips = (a.H + a.up_cols - 1) / a.up_cols, jobs = p.n * strips;
     bool own = true;
@@ -639,10 +652,11 @@ __device__ __forceinline__ void up_jobs(const Args &a, Plan &p, Sums &sh, int ti
             W::template up<ONE>(a, p, sh, u, job - u * strips);
             __syncthreads();
             finish_up<typename W::Type, ONE>(a, p, sh.up, u, (job - u * strips) * a.up_cols);
-        } else if (own && down >= 0) {
+        } else if (own && down_too) {
             own = false;
-            const Turn turn(a, p.n, down & (a.n_shares - 1));
-            const char *line = turn.first < p.n ? W::down_line(a, p, turn.first, down >> a.shares_log, turn.part, turn.parts_log, lane) : nullptr;
+            const int wave = gmm::uniform(tid >> 6), n = mine.to - mine.from, at = mine.from + (wave * n >> kWavesLog), end = mine.from + ((wave + 1) * n >> kWavesLog);
+            const int eu = at / each, s0 = at - eu * each;
+            const char *line = at < end ? W::down_line(a, p, eu, down.strip, s0, min(each, s0 + end - at), lane) : nullptr;
             if (line != nullptr) ahead = *reinterpret_cast<const uint32_t *>(line);
             __syncthreads();
         } else {
@@ -650,7 +664,7 @@ __device__ __forceinline__ void up_jobs(const Args &a, Plan &p, Sums &sh, int ti
         }
     }
     // (The last word of the last job: most others are there when it is, and lines that are not would be in the L2 for nothing.)
-    if (tid == 0 && down >= 0) {
+    if (tid == 0 && down_too) {
         const int u = p.n - 1, t = ONE ? 0 : __builtin_ctz(p.tokens[u]);
         const int32_t *word = reinterpret_cast<const int32_t *>(a.act + (int64_t)pair_of<ONE>(a, p, u, t) * 2 * a.act_pitch + a.H * 2 - 4);
 #pragma unroll 1

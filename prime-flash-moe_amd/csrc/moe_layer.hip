@@ -7,6 +7,9 @@ namespace {
 using namespace pmoe;
 using namespace pmoe::layer;
 
+// Workgroups that run at a time.
+int slots() { return std::min(2 * resident_grid(), kMaxGroups); }
+
 // logits[t][e]: four experts and up to four tokens per workgroup, whose waves share the contraction.  Beside that, the queues begin and the
 // activation is marked as absent.
 constexpr int kRouterTokens = 4;
@@ -49,32 +52,30 @@ __global__ __launch_bounds__(kThreads) void moe_layer_router_kernel(Args a) {
 }
 
 template <class W, bool ONE>
-__global__ __launch_bounds__(kThreads, 4) void moe_layer_kernel(Args a, int down_jobs) {
+__global__ __launch_bounds__(kThreads, 4) void moe_layer_kernel(Args a) {
     __shared__ Plan p;
     __shared__ __attribute__((aligned(1024))) Sums sums;
     int ticket = 0;
     if (threadIdx.x == 0) ticket = next_ticket(&a.sync->ticket[blockIdx.x % kQueues][0]);
     find_plan<ONE>(a, p, blockIdx.x == 0);
-    up_jobs<W, ONE>(a, p, sums, ticket, (int)blockIdx.x < down_jobs ? (int)blockIdx.x : -1);
-    const bool more = down_jobs > (int)gridDim.x;
-    for (int job = blockIdx.x; job < down_jobs;) {
-        if (more && threadIdx.x == 0) ticket = next_ticket(a.sync->down);
-        down_job<W, ONE>(a, p, sums, job);
-        if (!more) break;
-        if (threadIdx.x == 0) p.next = (int)gridDim.x + ticket;
-        __syncthreads();  // the sums may be cleared again
-        job = gmm::uniform(p.next);
+    const int each = W::down_steps(a), all = gmm::uniform(p.n) * each;
+    const Place from = place_of<W>(a, blockIdx.x, all), to = place_of<W>(a, blockIdx.x + 1, all);
+    const bool down_too = (int)blockIdx.x < a.down_groups;
+    up_jobs<W, ONE>(a, p, sums, ticket, from, Steps(from, to, from.strip, all), each, down_too);
+    if (!down_too) return;
+    for (int strip = from.strip; strip <= to.strip; ++strip) {
+        const Steps mine(from, to, strip, all);
+        if (mine.from < mine.to) down_job<W, ONE>(a, p, sums, strip, mine, each, all);
     }
 }
 
 template <class W>
 int launch(Args a, hipStream_t s) {
     hipLaunchKernelGGL((moe_layer_router_kernel<typename W::Type>), dim3((a.E + 3) / 4, (a.T + kRouterTokens - 1) / kRouterTokens), dim3(kThreads), 0, s, a);
-    const int cus = resident_grid(), most = std::min(a.E, a.T * a.top_k), down_strips = (a.K + W::kDownCols - 1) / W::kDownCols;
-    const int64_t up_jobs = (int64_t)most * ((a.H + a.up_cols - 1) / a.up_cols), down_jobs = (int64_t)down_strips * a.n_shares;
-    const dim3 grid((uint32_t)std::min<int64_t>(std::max(up_jobs, down_jobs), 2 * cus)), block(kThreads);
-    if (a.T == 1) hipLaunchKernelGGL((moe_layer_kernel<W, true>), grid, block, 0, s, a, (int)down_jobs);
-    else hipLaunchKernelGGL((moe_layer_kernel<W, false>), grid, block, 0, s, a, (int)down_jobs);
+    const int64_t up_jobs = (int64_t)std::min(a.E, a.T * a.top_k) * ((a.H + a.up_cols - 1) / a.up_cols);
+    const dim3 grid((uint32_t)std::min<int64_t>(std::max<int64_t>(up_jobs, a.down_groups), slots())), block(kThreads);
+    if (a.T == 1) hipLaunchKernelGGL((moe_layer_kernel<W, true>), grid, block, 0, s, a);
+    else hipLaunchKernelGGL((moe_layer_kernel<W, false>), grid, block, 0, s, a);
     return check_launch("moe_layer launch");
 }
 template <class T>
@@ -84,15 +85,11 @@ int launch(const Args &a, int group, hipStream_t s) {
 
 // How the jobs of a layer are cut.
 void cut_jobs(Args &a, int group) {
-    const int64_t slots = 2 * resident_grid(), most = std::min(a.E, a.T * a.top_k), quads = most * ((a.H + 3) / 4);
-    // One round of the grid where they are so few, otherwise jobs of 128 KB or the next thing below: where a job is large, what some
-    // workgroups have left at the end is.
-    const int64_t most_cols = quads <= 4 * slots ? (quads + slots - 1) / slots : std::max<int64_t>(1, (128 << 10) / (16 * a.K));
-    a.up_cols = group != 0 ? 16 : 4 * (int)std::min<int64_t>(4, most_cols);
+    const int64_t most = std::min(a.E, a.T * a.top_k), quads = most * ((a.H + 3) / 4);
+    a.up_cols = group != 0 ? 16 : 4 * (int)std::min<int64_t>(4, (quads + slots() - 1) / slots());
     const int64_t strips = group != 0 ? a.K / 16 : (a.K + 7) / 8, bytes = most * 3 * a.H * a.K * 2 / (group != 0 ? 4 : 1);
-    a.shares_log = 0;
-    while (bytes > 128 << 20 && 1 << a.shares_log < kMaxShares && strips << a.shares_log < slots && strips << (a.shares_log + 1) <= kMaxShared) ++a.shares_log;
-    a.n_shares = 1 << a.shares_log;
+    a.split = bytes > 128 << 20;
+    a.down_groups = (int)std::min<int64_t>(slots(), a.split ? strips * most : strips);
 }
 size_t act_pitch(int H) { return align_up((size_t)H * 2, 128); }
 size_t logits_bytes(int T, int E) { return align_up((size_t)T * E * 4, 256); }
@@ -102,7 +99,7 @@ static_assert(sizeof(Sync) % 256 == 0, "what follows is aligned");
 
 extern "C" size_t pmoe_moe_layer_workspace_bytes(int T, int H, int num_experts, int top_k) {
     if (T <= 0 || H <= 0 || num_experts <= 0 || top_k <= 0) return 0;
-    return sizeof(Sync) + logits_bytes(T, num_experts) + (size_t)kMaxShared * 16 * T * 4 + (size_t)T * top_k * 2 * act_pitch(H);
+    return sizeof(Sync) + logits_bytes(T, num_experts) + (size_t)2 * kMaxGroups * 16 * T * 4 + (size_t)T * top_k * 2 * act_pitch(H);
 }
 
 extern "C" int pmoe_moe_layer(const void *x, const void *gate, const float *bias, const void *w1, const void *w1_scale, const void *w2,
@@ -136,7 +133,7 @@ extern "C" int pmoe_moe_layer(const void *x, const void *gate, const float *bias
     a.sync = static_cast<Sync *>(workspace);
     a.logits = reinterpret_cast<float *>(a.sync + 1);
     a.shares = reinterpret_cast<float *>(reinterpret_cast<char *>(a.logits) + logits_bytes(T, num_experts));
-    a.act = reinterpret_cast<char *>(a.shares + (size_t)kMaxShared * 16 * T);
+    a.act = reinterpret_cast<char *>(a.shares + (size_t)2 * kMaxGroups * 16 * T);
     a.act_pitch = (int)act_pitch(H);
     a.T = T;
     a.K = K;
