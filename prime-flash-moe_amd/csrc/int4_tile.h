@@ -61,13 +61,6 @@ struct Num<F16> {
 
 __device__ __forceinline__ i32x4 load_once16(const char *p) { return __builtin_nontemporal_load(reinterpret_cast<const i32x4 *>(p)); }
 
-// 16 bytes as they stand in memory now, whatever the caches of the XCD hold.
-__device__ __forceinline__ i32x4 load_now(const char *p) {
-    const uint64_t *q = reinterpret_cast<const uint64_t *>(p);
-    const uint64_t lo = __hip_atomic_load(q, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT), hi = __hip_atomic_load(q + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    return i32x4{(int)lo, (int)(lo >> 32), (int)hi, (int)(hi >> 32)};
-}
-
 // A piece of memory of up to 4 GB, wave-uniform: a load takes an offset per lane and one for the wave; behind `bytes` it reads zeros.
 typedef __amdgpu_buffer_rsrc_t Buffer;
 __device__ __forceinline__ Buffer buffer(const char *p, uint32_t bytes) {
@@ -119,14 +112,17 @@ struct Rows {
                     if (g == 0 || 4 * g < n) f(i, g);
             }
     }
-    // `x(q)`: begins row q; `n`: rows, from 1 to M (both wave-uniform but for the lane's q); get(address): 16 bytes.
-    template <class X, class Get>
-    __device__ __forceinline__ void load(X x, Get get, int n, int t, int t1, int k) {
-        const int lane = threadIdx.x & 63, sub = lane >> 4, e = (lane & 15) * 8;
+    // `at[g]`: where this lane's 16 bytes of row 4 g + lane / 16 are in tile 0; `n`: rows, from 1 to M; `k`: columns; get(at, what to add): 16
+    // bytes.
+    template <class Get>
+    __device__ __forceinline__ void load(Get get, const uint32_t (&at)[M / 4], int n, int t, int t1, int k) {
         each(n, t, t1, [&](int i, int g) {
-            const int col = (t + i) * kTileCols + e;
-            v[i][g] = i32x4{0, 0, 0, 0};
-            if (col < k) v[i][g] = get(x(min(4 * g + sub, n - 1)) + (int64_t)col * 2);
+            if ((t + i + 1) * kTileCols <= k) {
+                v[i][g] = get(at[g], (t + i) * (kTileCols * 2));
+            } else {
+                v[i][g] = i32x4{0, 0, 0, 0};
+                if ((t + i) * kTileCols + (int)(threadIdx.x & 15) * 8 < k) v[i][g] = get(at[g], (t + i) * (kTileCols * 2));
+            }
         });
     }
     // The largest of the words that were loaded.
@@ -152,24 +148,28 @@ struct Rows {
 };
 
 // acc[u][q] += n rows of x times the weights of tiles t0 .. t1 - 1 of U strips (16 weight rows each), for one wave.  Lane l, r = l %
-// 16, c = l / 16: `w[u]`, `s[u]` begin strip u.  acc[u][q][i]: weight row r, row 16 q + 4 c + i of x (any of the n where there are fewer).
+// 16, c = l / 16: `w[u]`, `s[u]` begin strip u, row q of x is row(q) bytes behind `x`.  acc[u][q][i]: weight row r, row 16 q + 4 c + i of x (any of the n where there are fewer).
 // `k`: columns; nothing of x is read behind them.  M: rows at most, `lds`: Rows<M, S>::kBytes of the wave's own.  S: tiles whose loads are in flight
 // together; what hides the rest of their latency is other waves.  wait(most): called with the largest word of what was loaded of x, for
 // rows that may not all be there yet: true until they are.
 struct NoWait {
     static constexpr bool kWaits = false;
 };
-template <class T, int GROUP, int U, int R, int S, int M = 16 * R, class X, class Wait = NoWait>
-__device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[U], const char *const (&s)[U], X x, int n, int t0, int t1, int k, char *lds, Wait wait = {}) {
+template <class T, int GROUP, int U, int R, int S, int M = 16 * R, class Row, class Wait = NoWait>
+__device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[U], const char *const (&s)[U], const char *x, Row row, int n, int t0, int t1, int k, char *lds, Wait wait = {}) {
     using Sc = TileScales<GROUP>;
     constexpr int PER = GROUP / 32;
     const int lane = threadIdx.x & 63, r = lane & 15;
+    const Buffer xb = buffer(x, ~0u);
+    uint32_t at[M / 4];
+#pragma unroll
+    for (int g = 0; g < M / 4; ++g) at[g] = row(min(4 * g + (lane >> 4), n - 1)) + r * 16;
     const i32x4 minus = {(int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24};
     for (int t = t0; t < t1; t += S) {
         i32x4 wv[S][U];
         Sc sc[S][U];
         Rows<M, S> rows;
-        rows.load(x, [](const char *p) { return *reinterpret_cast<const i32x4 *>(p); }, n, t, t1, k);
+        rows.load([&](uint32_t l, uint32_t w) { return load(xb, l, w); }, at, n, t, t1, k);
 #pragma unroll
         for (int i = 0; i < S; ++i)
             if (i == 0 || t + i < t1) {
@@ -180,7 +180,7 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
                 }
             }
         if constexpr (Wait::kWaits)
-            while (wait(rows.most(n, t, t1))) rows.load(x, [](const char *p) { return load_now(p); }, n, t, t1, k);
+            while (wait(rows.most(n, t, t1))) rows.load([&](uint32_t l, uint32_t w) { return load_now(xb, l, w); }, at, n, t, t1, k);
         rows.store(lds, n, t, t1);
 #pragma unroll
         for (int i = 0; i < S; ++i)

@@ -488,8 +488,8 @@ struct Narrow {
         const char *const w[2] = {a.w1 + first * tiles * int4::kTileBytes, a.w1 + (first + strips) * tiles * int4::kTileBytes};
         const char *const s[2] = {a.w1_scale + first * tiles * SB, a.w1_scale + (first + strips) * tiles * SB};
         f32x4 acc[2][1] = {};
-        auto row = [&](int q) { return a.x + (ONE ? 0 : (int64_t)token_of(tokens, q) * a.K * 2); };
-        by_height<ONE>(last + 1, [&](auto m) { int4::dots<T, GROUP, 2, 1, (decltype(m)::value == 4 ? 2 : 16 / decltype(m)::value), decltype(m)::value>(acc, w, s, row, last + 1, t0, t1, a.K, rows); });
+        auto row = [&](int q) { return ONE ? 0u : (uint32_t)token_of(tokens, q) * (uint32_t)a.K * 2; };
+        by_height<ONE>(last + 1, [&](auto m) { int4::dots<T, GROUP, 2, 1, (decltype(m)::value == 4 ? 2 : 16 / decltype(m)::value), decltype(m)::value>(acc, w, s, a.x, row, last + 1, t0, t1, a.K, rows); });
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums.part[wave][0][4 * c + i][r] = acc[0][0][i], sums.part[wave][1][4 * c + i][r] = acc[1][0][i];
     }
@@ -517,10 +517,10 @@ struct Narrow {
             f32x4 acc[1][1] = {};
             auto row = [&](int q) {
                 const int t = ONE ? 0 : token_of(tokens, row0 + q / 2);
-                return a.act + ((int64_t)pair_of<ONE>(a, p, u, t) * 2 + (q & 1)) * a.act_pitch;
+                return ((uint32_t)pair_of<ONE>(a, p, u, t) * 2 + (q & 1)) * (uint32_t)a.act_pitch;
             };
             const int n = 2 * min(last + 1 - row0, 8);
-            by_height<ONE>(n, [&](auto m) { int4::dots<T, GROUP, 1, 1, 16 / decltype(m)::value, decltype(m)::value>(acc, w, s, row, n, s0, s1, a.H, rows, Arrival{&p.failed}); });
+            by_height<ONE>(n, [&](auto m) { int4::dots<T, GROUP, 1, 1, 16 / decltype(m)::value, decltype(m)::value>(acc, w, s, a.act, row, n, s0, s1, a.H, rows, Arrival{&p.failed}); });
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int j = row0 + 2 * c + i;
