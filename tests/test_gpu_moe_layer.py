@@ -233,3 +233,55 @@ def test_decoding_as_it_is_used(device):
         assert torch.equal(one[1][0], batch[1][t])
         layer_of_4_bits(x[t:t + 1], gate, packed, top_k, bias, 32, K, H).check(*one)
     assert prime_moe.moe_layer(x[:0], gate, w1, w2, top_k)[0].shape == (0, K)
+
+
+@pytest.fixture(params=[1, 7, 0])
+def compute_units(request):
+    """Grids of two workgroups, of 14, and of the whole card."""
+    from prime_moe import _native
+    _native.load().pmoe_set_compute_units(request.param)
+    yield request.param
+    _native.load().pmoe_set_compute_units(0)
+
+
+@pytest.mark.parametrize("kind", ["wide", "narrow"])
+@pytest.mark.parametrize("T", [1, 6, 16])
+def test_workgroups_that_have_many_jobs(device, compute_units, kind, T):
+    import prime_moe
+    K, H, E, top_k = (264, 72, 6, 3) if kind == "wide" else (352, 160, 6, 3)
+    gen, x, gate, bias = inputs(T, K, H, E, BF16, device, 40 + T)
+    if kind == "wide":
+        w1, w2 = wide(gen, H, K, E, BF16, device)
+        Layer(x, gate, w1, w2, top_k, bias).check(*prime_moe.moe_layer(x, gate, w1, w2, top_k, bias))
+    else:
+        packed = narrow(gen, H, K, E, BF16, 32, device)
+        q = [prime_moe.pack_int4(*p) for p in packed]
+        layer_of_4_bits(x, gate, packed, top_k, bias, 32, K, H).check(*prime_moe.moe_layer_int4(x, gate, *q[0], *q[1], top_k, bias))
+
+
+@pytest.mark.parametrize("T", [1, 5])
+@pytest.mark.parametrize("kind", ["wide", "narrow"])
+def test_workgroups_that_share_columns_of_the_output(device, compute_units, kind, T):
+    """More than 128 MB of touched weights, strips and experts in numbers that no grid divides; twice, for the same bits."""
+    import prime_moe
+    dtype = F16 if kind == "wide" else BF16
+    K, H, E, top_k = (2056, 2728, 6, 6) if kind == "wide" else (4128, 2080, 11, 11)
+    _, x, gate, bias = inputs(T, K, H, E, dtype, device, 50 + T)
+    gen = torch.Generator(device=device).manual_seed(T)
+    rand = lambda *s, **k: torch.randn(s, generator=gen, device=device, dtype=torch.float32)
+    if kind == "wide":
+        w1, w2 = (rand(E, 2 * H, K) * K ** -0.5).to(dtype), (rand(E, K, H) * H ** -0.5).to(dtype)
+        assert E * 3 * K * H * 2 > 128 << 20
+        run = lambda: prime_moe.moe_layer(x, gate, w1, w2, top_k, bias)
+        ref = Layer(x, gate, w1, w2, top_k, bias)
+    else:
+        packed = [(torch.randint(-8, 8, (E, n, k), generator=gen, device=device, dtype=torch.int8), ((rand(E, n, k // 32).abs() + 0.5) * 0.1 * k ** -0.5).to(dtype))
+                  for n, k in ((2 * H, K), (K, H))]
+        assert E * 3 * K * H // 2 > 128 << 20
+        q = [prime_moe.pack_int4(*p) for p in packed]
+        run = lambda: prime_moe.moe_layer_int4(x, gate, *q[0], *q[1], top_k, bias)
+        ref = layer_of_4_bits(x, gate, packed, top_k, bias, 32, K, H)
+    first = run()
+    ref.check(*first)
+    for a, b in zip(first, run()):
+        assert torch.equal(a, b)
