@@ -28,7 +28,7 @@ using int4::Num;
 
 constexpr int kMaxTokens = 16, kMaxTopK = 32, kMaxPairs = kMaxTokens * kMaxTopK, kMaxExperts = 512;
 constexpr int kThreads = 512, kWaves = 8, kWavesLog = 3;
-constexpr int kUpCols = 16;       // activation columns of an up job at most
+constexpr int kUpCols = 16;       // activation columns that waves share the contraction of, at most
 constexpr int kMaxGroups = 512;   // workgroups at most
 constexpr int64_t kMostTries = 1 << 24;  // of a wait, about a microsecond each: then the outputs are NaN
 
@@ -50,7 +50,8 @@ struct Args {
     int act_pitch;
     float *shares;  // [workgroup][2: of its first strip, of its last one][token][column]: sums of workgroups that share a strip of out
     int T, K, H, E, top_k;
-    int up_cols;    // columns of an up job, a multiple of 4
+    int up_cols;    // columns of an up job: 4, 8, 12 or 16, or 16 << up_log (weights of 4 bits)
+    int up_log;     // 8 >> up_log waves share the contraction of 16 columns
     int down_groups;  // workgroups of the down projection
     int split;        // whether they share strips of out
 };
@@ -361,17 +362,19 @@ struct Sums {
 };
 
 // What the columns of an up job have from every wave -> activation, two columns a thread.  The stores go through to where all XCDs see
-// them.
-template <class T, bool ONE>
+// them.  LOG: see Args::up_log.
+template <class T, bool ONE, int LOG>
 __device__ __forceinline__ void finish_up(const Args &a, const Plan &p, const UpSums &s, int u, int col0) {
+    constexpr int WAVES = kWaves >> LOG;
     const uint32_t tokens = tokens_of<ONE>(p, u);
-    const int rows = __popc(tokens), c = (threadIdx.x & 7) * 2, j = threadIdx.x >> 3;
-    if (j < rows && c < a.up_cols && col0 + c < a.H) {
+    const int rows = __popc(tokens), c = (threadIdx.x & 7) * 2, j = threadIdx.x >> 3 & 15, strip = threadIdx.x >> 7;
+    col0 += strip * kUpCols;
+    if (strip < 1 << LOG && j < rows && strip * kUpCols + c < a.up_cols && col0 + c < a.H) {
         float gate[2] = {}, up[2] = {};
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k)
+        for (int k = 0; k < WAVES; ++k)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) gate[i] += s.part[k][0][j][c + i], up[i] += s.part[k][1][j][c + i];
+            for (int i = 0; i < 2; ++i) gate[i] += s.part[strip * WAVES + k][0][j][c + i], up[i] += s.part[strip * WAVES + k][1][j][c + i];
         const int t = ONE ? 0 : token_of(tokens, j);
         const uint32_t v0 = split<T>(swiglu(gate[0], up[0])), v1 = split<T>(swiglu(gate[1], up[1]));
         char *at = a.act + (int64_t)pair_of<ONE>(a, p, u, t) * 2 * a.act_pitch + (col0 + c) * 2;
@@ -384,7 +387,7 @@ __device__ __forceinline__ void finish_up(const Args &a, const Plan &p, const Up
 template <class T, int QUADS>
 struct Wide {
     using Type = T;
-    static constexpr int kDownCols = 8;
+    static constexpr int kDownCols = 8, kMaxUpLog = 0;
 
     // The waves share the contraction; each has the gate and up rows of all columns, so that a row of x is read for up to 32 of them.
     template <bool ONE>
@@ -472,15 +475,17 @@ struct Wide {
 template <class T, int GROUP>
 struct Narrow {
     using Type = T;
-    static constexpr int kDownCols = 16;
+    static constexpr int kDownCols = 16, kMaxUpLog = 2;
 
-    // The waves share the contraction; a strip of gate rows and the matching one of up rows.
+    // 8 >> up_log waves share the contraction of a strip of gate rows and the matching one of up rows.
     template <bool ONE>
-    static __device__ __forceinline__ void up(const Args &a, const Plan &p, Sums &sh, int u, int strip) {
+    static __device__ __forceinline__ void up(const Args &a, const Plan &p, Sums &sh, int u, int job) {
         UpSums &sums = sh.up;
         const int lane = threadIdx.x & 63, wave = gmm::uniform(threadIdx.x >> 6), r = lane & 15, c = lane >> 4;
         char *const rows = sh.rows[wave];
-        const int tiles = int4::tiles_of(a.K), t0 = wave * tiles / kWaves, t1 = (wave + 1) * tiles / kWaves, strips = a.H / 16;
+        const int tiles = int4::tiles_of(a.K), log = kWavesLog - a.up_log, part = wave & ((1 << log) - 1), t0 = part * tiles >> log, t1 = (part + 1) * tiles >> log;
+        const int strips = a.H / 16, strip = (job << a.up_log) + (wave >> log);
+        if (strip >= strips) return;
         const uint32_t tokens = tokens_of<ONE>(p, u);
         const int last = __popc(tokens) - 1;
         constexpr int SB = int4::TileScales<GROUP>::kBytes;
@@ -489,7 +494,10 @@ struct Narrow {
         const char *const s[2] = {a.w1_scale + first * tiles * SB, a.w1_scale + (first + strips) * tiles * SB};
         f32x4 acc[2][1] = {};
         auto row = [&](int q) { return ONE ? 0u : (uint32_t)token_of(tokens, q) * (uint32_t)a.K * 2; };
-        by_height<ONE>(last + 1, [&](auto m) { int4::dots<T, GROUP, 2, 1, (decltype(m)::value == 4 ? 2 : 16 / decltype(m)::value), decltype(m)::value>(acc, w, s, a.x, row, last + 1, t0, t1, a.K, rows); });
+        by_height<ONE>(last + 1, [&](auto m) {
+            constexpr int M = decltype(m)::value, S = M == 4 || (M == 8 && GROUP > 32) ? 2 : 1;  // (what registers there are)
+            int4::dots<T, GROUP, 2, 1, S, M>(acc, w, s, a.x, row, last + 1, t0, t1, a.K, rows);
+        });
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums.part[wave][0][4 * c + i][r] = acc[0][0][i], sums.part[wave][1][4 * c + i][r] = acc[1][0][i];
     }
@@ -520,7 +528,10 @@ struct Narrow {
                 return ((uint32_t)pair_of<ONE>(a, p, u, t) * 2 + (q & 1)) * (uint32_t)a.act_pitch;
             };
             const int n = 2 * min(last + 1 - row0, 8);
-            by_height<ONE>(n, [&](auto m) { int4::dots<T, GROUP, 1, 1, 16 / decltype(m)::value, decltype(m)::value>(acc, w, s, a.act, row, n, s0, s1, a.H, rows, Arrival{&p.failed}); });
+            by_height<ONE>(n, [&](auto m) {
+                constexpr int M = decltype(m)::value, S = 16 / M;
+                int4::dots<T, GROUP, 1, 1, S, M>(acc, w, s, a.act, row, n, s0, s1, a.H, rows, Arrival{&p.failed});
+            });
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int j = row0 + 2 * c + i;
@@ -651,7 +662,10 @@ __device__ __forceinline__ void up_jobs(const Args &a, Plan &p, Sums &sh, int ti
             const int u = job / strips;
             W::template up<ONE>(a, p, sh, u, job - u * strips);
             __syncthreads();
-            finish_up<typename W::Type, ONE>(a, p, sh.up, u, (job - u * strips) * a.up_cols);
+            const int col0 = (job - u * strips) * a.up_cols;
+            if (W::kMaxUpLog == 0 || a.up_log == 0) finish_up<typename W::Type, ONE, 0>(a, p, sh.up, u, col0);
+            else if (a.up_log == 1) finish_up<typename W::Type, ONE, (W::kMaxUpLog > 0)>(a, p, sh.up, u, col0);
+            else finish_up<typename W::Type, ONE, W::kMaxUpLog>(a, p, sh.up, u, col0);
         } else if (own && down_too) {
             own = false;
             const int wave = gmm::uniform(tid >> 6), n = mine.to - mine.from, at = mine.from + (wave * n >> kWavesLog), end = mine.from + ((wave + 1) * n >> kWavesLog);

@@ -85,10 +85,23 @@ int launch(const Args &a, int group, hipStream_t s) {
 
 // How the jobs of a layer are cut.
 void cut_jobs(Args &a, int group) {
-    const int64_t most = std::min(a.E, a.T * a.top_k), quads = most * ((a.H + 3) / 4);
-    a.up_cols = group != 0 ? 16 : 4 * (int)std::min<int64_t>(4, (quads + slots() - 1) / slots());
-    const int64_t strips = group != 0 ? a.K / 16 : (a.K + 7) / 8, bytes = most * 3 * a.H * a.K * 2 / (group != 0 ? 4 : 1);
-    a.split = bytes > 128 << 20;
+    const int64_t most = std::min(a.E, a.T * a.top_k), rows = group != 0 ? 16 : 4, jobs = most * ((a.H + rows - 1) / rows);
+    if (group != 0) {
+        // As many columns as leave every workgroup a job: fewer jobs of a wave's longer reads.  16, 32, 64 columns, us: 12288 jobs of 16
+        // (16 tokens on 256 experts of 7168 x 2048) 514, 496, 489; 3936 (16 on 128 of 2048 x 768) 64, 59, 58; 1024 (one on the 256) 55,
+        // 53, 68; 384 (one on the 128) 17, 18, 21.
+        while (a.up_log < Narrow<Bf16, 128>::kMaxUpLog && jobs >> (a.up_log + 1) >= slots()) ++a.up_log;
+        a.up_cols = 16 << a.up_log;
+    } else {
+        // One round of the grid where jobs of up to 16 columns do that, otherwise the 16: a row of x is read less often.  (One token on 128
+        // experts of 2048 x 768, 12 columns: 22.6 us, 25.5 with 4; 16 tokens 138, 166 with 4.)
+        a.up_cols = 4 * (int)std::min<int64_t>(4, (jobs + slots() - 1) / slots());
+    }
+    // Strips of out are shared where that takes enough steps from the wave that has the most: joining takes two microseconds.  Shared, not
+    // shared, us: 4 bits, 16 tokens on 128 experts of 2048 x 768 62, 79, three 31, 34, one (4 steps) 19.4, 17.0; 16 bits, 16 tokens 138,
+    // 143, four (12 steps) 64.2, 63.2.
+    const int64_t strips = group != 0 ? a.K / 16 : (a.K + 7) / 8, steps = most * ((a.H + 127) / 128);
+    a.split = ((strips + slots() - 1) / slots() * steps - strips * steps / slots()) / kWaves >= (group != 0 ? 8 : 16);
     a.down_groups = (int)std::min<int64_t>(slots(), a.split ? strips * most : strips);
 }
 size_t act_pitch(int H) { return align_up((size_t)H * 2, 128); }
