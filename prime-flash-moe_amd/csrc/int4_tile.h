@@ -30,14 +30,24 @@ constexpr int kTileRows = 16, kTileCols = 128, kTileBytes = 1024;
 
 __host__ __device__ inline int tiles_of(int k) { return (k + kTileCols - 1) / kTileCols; }
 
+// The two constants of the way to 16 bits, one in a scalar and one in a vector register, which the compiler is not told the values of: an
+// and-or has no room for a constant of 32 bits, and for known ones it makes an and and an or, half as many instructions again.
+struct Masks {
+    uint32_t mask, sixteen;
+    __device__ __forceinline__ Masks(uint32_t m, uint32_t s) : mask(m), sixteen(s) {
+        asm("" : "+s"(mask));
+        asm("" : "+v"(sixteen));
+    }
+};
+
 template <class T>
 struct Num;
 template <>
 struct Num<Bf16> {
     static constexpr uint32_t kMinus24 = 0xc1c0c1c0u;
-    static __device__ __forceinline__ i32x4 wide(uint32_t w) {
-        constexpr uint32_t M = 0x00780078u, B = 0x41804180u;
-        return i32x4{(int)((w << 3 & M) | B), (int)((w >> 1 & M) | B), (int)((w >> 5 & M) | B), (int)((w >> 9 & M) | B)};
+    static constexpr uint32_t kMask = 0x00780078u, kSixteen = 0x41804180u;
+    static __device__ __forceinline__ i32x4 wide(uint32_t w, Masks m) {
+        return i32x4{(int)((w << 3 & m.mask) | m.sixteen), (int)((w >> 1 & m.mask) | m.sixteen), (int)((w >> 5 & m.mask) | m.sixteen), (int)((w >> 9 & m.mask) | m.sixteen)};
     }
     static __device__ __forceinline__ float to_f32(uint16_t v) { return __uint_as_float((uint32_t)v << 16); }
     static __device__ __forceinline__ uint16_t from_f32(float v) { return (uint16_t)pack2_bf16(v, 0.f); }
@@ -48,9 +58,9 @@ struct Num<Bf16> {
 template <>
 struct Num<F16> {
     static constexpr uint32_t kMinus24 = 0xce00ce00u;
-    static __device__ __forceinline__ i32x4 wide(uint32_t w) {
-        constexpr uint32_t M = 0x03c003c0u, B = 0x4c004c00u;
-        return i32x4{(int)((w << 6 & M) | B), (int)((w << 2 & M) | B), (int)((w >> 2 & M) | B), (int)((w >> 6 & M) | B)};
+    static constexpr uint32_t kMask = 0x03c003c0u, kSixteen = 0x4c004c00u;
+    static __device__ __forceinline__ i32x4 wide(uint32_t w, Masks m) {
+        return i32x4{(int)((w << 6 & m.mask) | m.sixteen), (int)((w << 2 & m.mask) | m.sixteen), (int)((w >> 2 & m.mask) | m.sixteen), (int)((w >> 6 & m.mask) | m.sixteen)};
     }
     static __device__ __forceinline__ float to_f32(uint16_t v) { return (float)__builtin_bit_cast(_Float16, v); }
     static __device__ __forceinline__ uint16_t from_f32(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
@@ -164,6 +174,7 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
     uint32_t at[M / 4];
 #pragma unroll
     for (int g = 0; g < M / 4; ++g) at[g] = row(min(4 * g + (lane >> 4), n - 1)) + r * 16;
+    const Masks masks(Num<T>::kMask, Num<T>::kSixteen);
     const i32x4 minus = {(int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24};
     for (int t = t0; t < t1; t += S) {
         i32x4 wv[S][U];
@@ -205,7 +216,7 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
                         for (int q = 0; q < R; ++q) sum[q] = less[q];
 #pragma unroll
                         for (int j = 0; j < PER; ++j) {
-                            const i32x4 b = Num<T>::wide((uint32_t)wv[i][u][g * PER + j]);
+                            const i32x4 b = Num<T>::wide((uint32_t)wv[i][u][g * PER + j], masks);
 #pragma unroll
                             for (int q = 0; q < R; ++q) sum[q] = gmm::few::Mini<T>::mfma(xv[q][j], b, sum[q]);
                         }

@@ -140,6 +140,7 @@ __global__ __launch_bounds__(256) void dequantize_int4_kernel(const char *__rest
     using Sc = TileScales<GROUP>;
     __shared__ __attribute__((aligned(16))) char lds[4][4096];  // a tile of each wave's own: chunk k of row r in slot k ^ r
     const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+    const Masks masks(Num<T>::kMask, Num<T>::kSixteen);
     for (int64_t tile = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); tile < n_tiles; tile += (int64_t)gridDim.x * 4) {
         const int64_t strip = tile / tiles;
         const int col0 = (int)(tile - strip * tiles) * kTileCols;
@@ -152,7 +153,7 @@ __global__ __launch_bounds__(256) void dequantize_int4_kernel(const char *__rest
         for (int j = 0; j < 4; ++j) {
             const float s = Num<T>::to_f32(sc.v[j / (GROUP / 32)]);
             // (24 + q) s - 24 s: both products are exact, and so is the difference
-            const i32x4 wide = Num<T>::wide(w[j]);
+            const i32x4 wide = Num<T>::wide(w[j], masks);
             const float less = -24.0f * s;
             float v[8];
 #pragma unroll
