@@ -1,6 +1,7 @@
 // Products with weights of 4 bits (int4_tile.h): rows by their group's matrix, or by a single one.
 //
-// Bound by the stream of the touched groups' weights, 64 tokens on 256 experts of 4096 x 7168 by 417 us, 4.8 TB/s (345 where x is constant).  A workgroup takes one
+// Bound by the stream of the touched groups' weights, 64 tokens on half of 256 experts of 4096 x 7168 by 387 us, 5.2 TB/s, with the vector
+// units busy for half of the time (the way to 16 bits).  A workgroup takes one
 // group and 16 U of its weight rows at a time; its waves share the contraction, each in one run of tiles, and add their sums in LDS
 // in the order of the waves.  Rows of x come 16 (or 32) at a time; a group with more rows streams its weights again for them.
 #include <algorithm>
@@ -151,15 +152,18 @@ int launch_as(const Int4Args &a, int64_t slots, hipStream_t stream) {
 template <class T, int GROUP>
 int launch(const Int4Args &a, hipStream_t stream) {
     const int64_t slots = std::min(a.rows.rows, a.rows.n_groups), strips = a.rows.cols / 16;
-    // Rows are taken 16 at a time, or 32 where the average group has more (27 rows x 28672 x 4096: 21 us instead of 30; the registers
-    // of 32 rows cost those with fewer half of their waves: 16 tokens on 128 experts of 1536 x 2048 47 us instead of 31).
+    // Rows are taken 16 at a time, or 32 where there are more, or on average nearly as many as that in a group, so that some have more (27 rows x
+    // 28672 x 4096: 22 us instead of 30; 16 on average of 8 groups 125 instead of 137, 14 the same).  The registers of 32 rows cost
+    // those with fewer half of their waves: 12 on average 123 us instead of 104, 4 (128 experts of 1536 x 2048) 51 instead of 41.
     // A wave with more strips reads x less often; few strips are shared by more waves instead, so that all CUs have some.  Strips
-    // of one, two, four, us: 256 (a row through 4096 x 7168) 7.8, 9.8, 13; 1024 (8 of 128 experts of 2048 x 768) 7.5, 6.2, 6.5; 7900 (16
-    // tokens on 128 experts of 1536 x 2048) 49, 38, 31.
+    // of one, two, four, us: 256 (a row through 4096 x 7168) 7.8, 9.8, 18; 1024 (8 of 128 experts of 2048 x 768) 8.0, 6.5, 7.8; 1536 (16
+    // of 128 of 1536 x 2048) 11.8, 10.2, 11.1; 1792 (a row through 28672 x 4096) 16.8, 17.2, 15.6; 7900 (16 tokens on 128 of 1536 x 2048) 37, 30,
+    // 26.
     const int64_t all = strips * slots, cus = resident_grid();
-    if (a.rows.rows > 16 * (int64_t)a.rows.n_groups) return all <= 2 * cus ? launch_as<T, GROUP, 1, 2, 1, 8, 2>(a, slots, stream) : launch_as<T, GROUP, 4, 2, 1, 4, 2>(a, slots, stream);
+    if (a.rows.rows > (a.rows.offsets != nullptr ? 14 : 16) * (int64_t)a.rows.n_groups)
+        return all <= 2 * cus ? launch_as<T, GROUP, 1, 2, 1, 8, 2>(a, slots, stream) : launch_as<T, GROUP, 4, 2, 1, 4, 2>(a, slots, stream);
     if (all <= 2 * cus) return launch_as<T, GROUP, 1, 1, 2, 8, 4>(a, slots, stream);
-    if (all <= 4 * cus) return launch_as<T, GROUP, 2, 1, 1, 8, 4>(a, slots, stream);
+    if (all <= 6 * cus) return launch_as<T, GROUP, 2, 1, 1, 8, 4>(a, slots, stream);
     return launch_as<T, GROUP, 4, 1, 1, 4, 4>(a, slots, stream);
 }
 template <class T>
