@@ -258,3 +258,28 @@ def test_int4_experts_and_their_unpacked_form_agree(device):
         # (the unpacked weights are rounded to bfloat16: 2^-9 of a magnitude of 8 scales)
         y = prime_moe.grouped_mm(rows, prime_moe.dequantize_int4(q, s), offsets)
         assert ((y.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 8 * 2.0 ** -9 * 1.01 * m + 1e-6).all()
+
+
+def test_weights_behind_4_gb(device):
+    """The last of many matrices, and the last rows of a matrix of more than 2^32 values: products, quantiser, inverse."""
+    import prime_moe
+    E, N, K, group = 260, 8192, 4096, 128
+    gen = torch.Generator().manual_seed(3)
+    values, scale = operands((1, N, K), group, BF16, gen, device)
+    x = torch.randn((3, K), generator=gen).to(BF16).to(device)
+    q, s = prime_moe.pack_int4(values, scale)
+    many_q = torch.zeros((E, *q.shape[1:]), dtype=torch.uint8, device=device)
+    many_s = torch.zeros((E, *s.shape[1:]), dtype=BF16, device=device)
+    assert many_q.numel() > 1 << 32
+    many_q[-1], many_s[-1] = q[0], s[0]
+    ends = torch.tensor([0] * (E - 1) + [3], dtype=torch.int32, device=device)
+    R.check(prime_moe.grouped_mm_int4(x, many_q, many_s, ends), *R.mm(x, values, scale, [3]), K, group)
+    del many_q, many_s
+    w = torch.zeros((132, N, K), dtype=BF16, device=device)
+    assert w.numel() > 1 << 32
+    w[-1] = torch.randn((N, K), generator=gen).to(BF16).to(device)
+    q, s = prime_moe.quantize_int4(w, group)
+    one = prime_moe.quantize_int4(w[-1], group)
+    assert torch.equal(q[-1], one[0]) and torch.equal(s[-1], one[1])
+    back = prime_moe.dequantize_int4(q, s)
+    assert torch.equal(back[-1], prime_moe.dequantize_int4(*one)) and (back[0] == 0).all()

@@ -285,3 +285,59 @@ def test_workgroups_that_share_columns_of_the_output(device, compute_units, kind
     ref.check(*first)
     for a, b in zip(first, run()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("kind", ["wide", "narrow"])
+def test_experts_behind_4_gb(device, kind):
+    import prime_moe
+    T, top_k = 3, 2
+    K, H, E = (4096, 2048, 140) if kind == "wide" else (4096, 4096, 260)
+    gen, x, gate, bias = inputs(T, K, H, E, BF16, device, 70)
+    bias[:-2] -= 1e4  # the last two experts are everybody's
+    def all_experts(two):
+        whole = torch.zeros((E, *two.shape[1:]), dtype=two.dtype, device=device)
+        whole[-2:] = two
+        return whole
+    if kind == "wide":
+        w1, w2 = wide(gen, H, K, 2, BF16, device)
+        whole = [all_experts(t) for t in (w1, w2)]
+        ref = Layer(x, gate[-2:], w1, w2, top_k, bias[-2:])
+        out, ids, weights = prime_moe.moe_layer(x, gate, *whole, top_k, bias)
+    else:
+        packed = narrow(gen, H, K, 2, BF16, 128, device)
+        whole = [all_experts(t) for p in packed for t in prime_moe.pack_int4(*p)]
+        ref = layer_of_4_bits(x, gate[-2:], packed, top_k, bias[-2:], 128, K, H)
+        out, ids, weights = prime_moe.moe_layer_int4(x, gate, *whole, top_k, bias)
+    assert whole[0].numel() * whole[0].element_size() > 1 << 32
+    ref.check(out, ids - (E - 2), weights)
+
+
+@pytest.mark.parametrize("kind", ["wide", "narrow"])
+def test_calls_of_several_threads(device, kind):
+    """Calls of several host threads on streams of their own, each with rows of a longer batch."""
+    import threading
+
+    import prime_moe
+    K, H, E, top_k = 512, 256, 16, 4
+    gen, x, gate, bias = inputs(12, K, H, E, F16, device, 71)
+    w = wide(gen, H, K, E, F16, device) if kind == "wide" else [t for p in narrow(gen, H, K, E, F16, 32, device) for t in prime_moe.pack_int4(*p)]
+    run = lambda v: (prime_moe.moe_layer if kind == "wide" else prime_moe.moe_layer_int4)(v, gate, *w, top_k, bias)
+    want = [run(x[4 * i:4 * i + 4]) for i in range(3)]
+    torch.cuda.synchronize()
+    got = [[] for _ in range(3)]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(20):
+                got[i].append(run(x[4 * i:4 * i + 4]))
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for i in range(3):
+        assert len(got[i]) == 20
+        for r in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
