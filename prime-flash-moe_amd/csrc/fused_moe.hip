@@ -146,13 +146,6 @@ __device__ __forceinline__ void store_y_direct(const YDst &d, const f32x16 (&acc
             }
         }
 }
-// LDS written by some lanes of a wave is read by others of the same wave: LDS operations of a wave are executed in
-// order, only the compiler has to keep them so.
-__device__ __forceinline__ void wave_lds_order() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
 // Larger tiles: a wave rounds a fragment (token rows 32 t .. of its group) of its 64 columns to bf16, transposes it through a
 // scratch of its own, 16 rows at a time, and stores whole 128-byte lines.  `pair` = the pair ids of the fragment's rows (rows
 // without one are skipped).  Before, the groups' 128 x 256 tiles went through 132 KB of LDS: on two full blocks the first slabs of

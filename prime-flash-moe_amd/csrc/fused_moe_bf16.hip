@@ -402,14 +402,6 @@ __device__ __forceinline__ void epilogue_with_links(Epilogue epilogue, Link link
     for (int l = FG + 1; l < kLinks; ++l) link(l);
 }
 
-// LDS written by some lanes of a wave is read by others of the same wave: LDS operations of a wave are executed in
-// order, only the compiler has to keep them so.
-__device__ __forceinline__ void wave_lds_order() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // Up kernel tile: token fragments f0 .. f0 + 2 FG - 1 x activation columns [128 wt, 128 wt + 128) of expert e,
 // contraction slabs [slab0, slab0 + n_slabs).  LDS weight rows 0..127 are gate rows, 128..255 the matching up
 // rows; wave v of a group owns gate/up rows 32v..32v+31, so gate and up of one activation element sit in the

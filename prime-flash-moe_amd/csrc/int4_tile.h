@@ -192,7 +192,9 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
             }
         if constexpr (Wait::kWaits)
             while (wait(rows.most(n, t, t1))) rows.load([&](uint32_t l, uint32_t w) { return load_now(xb, l, w); }, at, n, t, t1, k);
+        wave_lds_order();  // (the reads of the tiles before are done)
         rows.store(lds, n, t, t1);
+        wave_lds_order();
 #pragma unroll
         for (int i = 0; i < S; ++i)
             if (i == 0 || t + i < t1) {

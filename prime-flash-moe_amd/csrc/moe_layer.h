@@ -585,11 +585,13 @@ __device__ __forceinline__ void down_job(const Args &a, Plan &p, Sums &sh, int s
     float(&y)[kMaxTokens][16] = sums.y[wave];
 #pragma unroll
     for (int i = 0; i < (ONE ? 1 : kMaxTokens * 16 / 64); ++i) (&y[0][0])[i * 64 + lane] = 0.f;
+    wave_lds_order();
     const int n = mine.to - mine.from, end = mine.from + ((wave + 1) * n >> kWavesLog);
     int at = mine.from + (wave * n >> kWavesLog), u = at / each, s0 = at - u * each;
     while (at < end) {
         const int s1 = min(each, s0 + end - at);
         W::template down<ONE>(a, p, y, sh.rows[wave], u, strip, s0, s1);
+        wave_lds_order();  // (the next expert's tokens may be other lanes')
         at += s1 - s0, ++u, s0 = 0;
     }
     __syncthreads();

@@ -15,6 +15,14 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+// LDS written by some lanes of a wave is read by others of the same wave: LDS operations of a wave are executed in
+// order, only the compiler has to keep them so.
+__device__ __forceinline__ void wave_lds_order() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 constexpr int kBlockRows = 128;  // sorted rows per block (= block_m)
 constexpr int kWRows = 256;      // weight rows per tile
 

@@ -93,10 +93,12 @@ __global__ __launch_bounds__(256) void quantize_int4_kernel(const char *__restri
                 in[i][k] = i32x4{0, 0, 0, 0};
                 if (col0 + 8 * r < cols) in[i][k] = p[(int64_t)i * cols / 2 * W + k];
             }
+        wave_lds_order();
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int k = 0; k < W; ++k) mine[k][(4 * i + c) * 16 + (r ^ (4 * i + c))] = in[i][k];
+        wave_lds_order();
         float v[4][8];
         uint32_t peaks[4];
 #pragma unroll
@@ -149,6 +151,7 @@ __global__ __launch_bounds__(256) void dequantize_int4_kernel(const char *__rest
         Sc sc;
         sc.load(scales + tile * Sc::kBytes, r);
         char *const mine = lds[threadIdx.x >> 6];
+        wave_lds_order();
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float s = Num<T>::to_f32(sc.v[j / (GROUP / 32)]);
@@ -164,6 +167,7 @@ __global__ __launch_bounds__(256) void dequantize_int4_kernel(const char *__rest
             const uint2 lo = gmm::Pack<T>::four(v[0], v[1], v[2], v[3]), hi = gmm::Pack<T>::four(v[4], v[5], v[6], v[7]);
             *reinterpret_cast<uint4 *>(mine + r * 256 + ((4 * j + c) ^ r) * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
         }
+        wave_lds_order();
         // (out by 256 bytes of four rows a store)
         const int col = col0 + (lane & 15) * 8;
         char *p = out + ((strip * 16 + c) * cols + col) * 2;
