@@ -155,14 +155,13 @@ __global__ __launch_bounds__(256) void dequantize_int4_kernel(const char *__rest
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float s = Num<T>::to_f32(sc.v[j / (GROUP / 32)]);
-            // (24 + q) s - 24 s: both products are exact, and so is the difference
+            // (24 is taken off before the product: the difference is exact, where 24 s may be beyond fp32 and q s is not)
             const i32x4 wide = Num<T>::wide(w[j], masks);
-            const float less = -24.0f * s;
             float v[8];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                v[2 * k] = fmaf(Num<T>::to_f32((uint16_t)wide[k]), s, less);
-                v[2 * k + 1] = fmaf(Num<T>::to_f32((uint16_t)((uint32_t)wide[k] >> 16)), s, less);
+                v[2 * k] = (Num<T>::to_f32((uint16_t)wide[k]) - 24.0f) * s;
+                v[2 * k + 1] = (Num<T>::to_f32((uint16_t)((uint32_t)wide[k] >> 16)) - 24.0f) * s;
             }
             const uint2 lo = gmm::Pack<T>::four(v[0], v[1], v[2], v[3]), hi = gmm::Pack<T>::four(v[4], v[5], v[6], v[7]);
             *reinterpret_cast<uint4 *>(mine + r * 256 + ((4 * j + c) ^ r) * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
