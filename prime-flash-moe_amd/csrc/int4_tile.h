@@ -15,6 +15,11 @@
 // and-ors; conversions to fp32 and back would be twenty instructions, which is more than there is time for at the rate of the memory:
 // 21 weights a cycle and CU.
 //
+// bf16 reaches as far as fp32, and 24 times a sum of 128 of it further.  So bf16 weights are 2^-12 (24 + q), from 2^-8 in place of 16.0: no
+// sum of a group passes 24 x 128 x 2^-12 = 0.75 of the largest |x|, and the 2^12 come back in the wave's sum, where all rows of weights
+// have been scaled.  Powers of two change no bit of what stays above 2^-126; the products of the least numbers are subnormal, which
+// the matrix instructions keep.
+//
 // Sums of a group are scaled in fp32, by four multiply-adds per 128 / group tiles.
 #pragma once
 #include "grouped_few.h"
@@ -44,8 +49,10 @@ template <class T>
 struct Num;
 template <>
 struct Num<Bf16> {
-    static constexpr uint32_t kMinus24 = 0xc1c0c1c0u;
     static constexpr uint32_t kMask = 0x00780078u, kSixteen = 0x41804180u;
+    // of a product: 16 and -24, both over kUnit
+    static constexpr uint32_t kBase = 0x3b803b80u, kMinus24 = 0xbbc0bbc0u;
+    static constexpr float kUnit = 0x1p12f;
     static __device__ __forceinline__ i32x4 wide(uint32_t w, Masks m) {
         return i32x4{(int)((w << 3 & m.mask) | m.sixteen), (int)((w >> 1 & m.mask) | m.sixteen), (int)((w >> 5 & m.mask) | m.sixteen), (int)((w >> 9 & m.mask) | m.sixteen)};
     }
@@ -57,8 +64,9 @@ struct Num<Bf16> {
 };
 template <>
 struct Num<F16> {
-    static constexpr uint32_t kMinus24 = 0xce00ce00u;
     static constexpr uint32_t kMask = 0x03c003c0u, kSixteen = 0x4c004c00u;
+    static constexpr uint32_t kBase = kSixteen, kMinus24 = 0xce00ce00u;
+    static constexpr float kUnit = 1.0f;
     static __device__ __forceinline__ i32x4 wide(uint32_t w, Masks m) {
         return i32x4{(int)((w << 6 & m.mask) | m.sixteen), (int)((w << 2 & m.mask) | m.sixteen), (int)((w >> 2 & m.mask) | m.sixteen), (int)((w >> 6 & m.mask) | m.sixteen)};
     }
@@ -157,7 +165,7 @@ struct Rows {
     }
 };
 
-// acc[u][q] += n rows of x times the weights of tiles t0 .. t1 - 1 of U strips (16 weight rows each), for one wave.  Lane l, r = l %
+// acc[u][q] = n rows of x times the weights of tiles t0 .. t1 - 1 of U strips (16 weight rows each), for one wave.  Lane l, r = l %
 // 16, c = l / 16: `w[u]`, `s[u]` begin strip u, row q of x is row(q) bytes behind `x`.  acc[u][q][i]: weight row r, row 16 q + 4 c + i of x (any of the n where there are fewer).
 // `k`: columns; nothing of x is read behind them.  M: rows at most, `lds`: Rows<M, S>::kBytes of the wave's own.  S: tiles whose loads are in flight
 // together; what hides the rest of their latency is other waves.  wait(most): called with the largest word of what was loaded of x, for
@@ -174,8 +182,12 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
     uint32_t at[M / 4];
 #pragma unroll
     for (int g = 0; g < M / 4; ++g) at[g] = row(min(4 * g + (lane >> 4), n - 1)) + r * 16;
-    const Masks masks(Num<T>::kMask, Num<T>::kSixteen);
+    const Masks masks(Num<T>::kMask, Num<T>::kBase);
     const i32x4 minus = {(int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24};
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int q = 0; q < R; ++q) acc[u][q] = f32x4{0.f, 0.f, 0.f, 0.f};
     for (int t = t0; t < t1; t += S) {
         i32x4 wv[S][U];
         Sc sc[S][U];
@@ -231,6 +243,13 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
                 }
             }
     }
+    if constexpr (Num<T>::kUnit != 1.0f)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int q = 0; q < R; ++q)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[u][q][e] *= Num<T>::kUnit;
 }
 
 }  // namespace int4

@@ -499,7 +499,7 @@ struct Narrow {
         const int64_t first = (int64_t)gmm::uniform(p.expert[u]) * 2 * strips + strip;
         const char *const w[2] = {a.w1 + first * tiles * int4::kTileBytes, a.w1 + (first + strips) * tiles * int4::kTileBytes};
         const char *const s[2] = {a.w1_scale + first * tiles * SB, a.w1_scale + (first + strips) * tiles * SB};
-        f32x4 acc[2][1] = {};
+        f32x4 acc[2][1];
         auto row = [&](int q) { return ONE ? 0u : (uint32_t)token_of(tokens, q) * (uint32_t)a.K * 2; };
         by_height<ONE>(last + 1, [&](auto m) {
             constexpr int M = decltype(m)::value, S = M == 4 || (M == 8 && GROUP > 32) ? 2 : 1;  // (what registers there are)
@@ -529,7 +529,7 @@ struct Narrow {
         const char *const s[1] = {a.w2_scale + first * tiles * SB};
         // row m of the matrix instructions: value (m even) or rest of the expert's row m / 2
         for (int row0 = 0; row0 <= last; row0 += 8) {
-            f32x4 acc[1][1] = {};
+            f32x4 acc[1][1];
             auto row = [&](int q) {
                 const int t = ONE ? 0 : token_of(tokens, row0 + q / 2);
                 return ((uint32_t)pair_of<ONE>(a, p, u, t) * 2 + (q & 1)) * (uint32_t)a.act_pitch;
