@@ -40,7 +40,7 @@ __device__ __forceinline__ void pass(const Int4Args &a, int group, int row0, int
     }
     const char *const x = a.rows.x + row0 * a.rows.x_pitch;
     f32x4 acc[U][R];
-    dots<T, GROUP, U, R, S>(acc, w, s, x, [&](int q) { return (uint32_t)q * (uint32_t)a.rows.x_pitch; }, live, t0, t1, a.rows.depth, sh.rows[wave]);
+    dots<T, T, GROUP, U, R, S>(acc, w, s, x, [&](int q) { return (uint32_t)q * (uint32_t)a.rows.x_pitch; }, live, t0, t1, a.rows.depth, sh.rows[wave]);
     __syncthreads();  // the sums lie where the rows were
 #pragma unroll
     for (int u = 0; u < U; ++u)

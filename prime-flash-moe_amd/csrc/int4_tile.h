@@ -168,12 +168,12 @@ struct Rows {
 // acc[u][q] = n rows of x times the weights of tiles t0 .. t1 - 1 of U strips (16 weight rows each), for one wave.  Lane l, r = l %
 // 16, c = l / 16: `w[u]`, `s[u]` begin strip u, row q of x is row(q) bytes behind `x`.  acc[u][q][i]: weight row r, row 16 q + 4 c + i of x (any of the n where there are fewer).
 // `k`: columns; nothing of x is read behind them.  M: rows at most, `lds`: Rows<M, S>::kBytes of the wave's own.  S: tiles whose loads are in flight
-// together; what hides the rest of their latency is other waves.  wait(most): called with the largest word of what was loaded of x, for
+// together; what hides the rest of their latency is other waves.  X: type of the rows, T: of the scales.  wait(most): called with the largest word of what was loaded of x, for
 // rows that may not all be there yet: true until they are.
 struct NoWait {
     static constexpr bool kWaits = false;
 };
-template <class T, int GROUP, int U, int R, int S, int M = 16 * R, class Row, class Wait = NoWait>
+template <class X, class T, int GROUP, int U, int R, int S, int M = 16 * R, class Row, class Wait = NoWait>
 __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[U], const char *const (&s)[U], const char *x, Row row, int n, int t0, int t1, int k, char *lds, Wait wait = {}) {
     using Sc = TileScales<GROUP>;
     constexpr int PER = GROUP / 32;
@@ -182,8 +182,8 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
     uint32_t at[M / 4];
 #pragma unroll
     for (int g = 0; g < M / 4; ++g) at[g] = row(min(4 * g + (lane >> 4), n - 1)) + r * 16;
-    const Masks masks(Num<T>::kMask, Num<T>::kBase);
-    const i32x4 minus = {(int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24, (int)Num<T>::kMinus24};
+    const Masks masks(Num<X>::kMask, Num<X>::kBase);
+    const i32x4 minus = {(int)Num<X>::kMinus24, (int)Num<X>::kMinus24, (int)Num<X>::kMinus24, (int)Num<X>::kMinus24};
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -220,7 +220,7 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
 #pragma unroll
                         for (int j = 0; j < PER; ++j) {
                             xv[q][j] = Rows<M, S>::read(lds, n, i, q, g * PER + j);
-                            less[q] = gmm::few::Mini<T>::mfma(xv[q][j], minus, less[q]);
+                            less[q] = gmm::few::Mini<X>::mfma(xv[q][j], minus, less[q]);
                         }
                     }
 #pragma unroll
@@ -230,9 +230,9 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
                         for (int q = 0; q < R; ++q) sum[q] = less[q];
 #pragma unroll
                         for (int j = 0; j < PER; ++j) {
-                            const i32x4 b = Num<T>::wide((uint32_t)wv[i][u][g * PER + j], masks);
+                            const i32x4 b = Num<X>::wide((uint32_t)wv[i][u][g * PER + j], masks);
 #pragma unroll
-                            for (int q = 0; q < R; ++q) sum[q] = gmm::few::Mini<T>::mfma(xv[q][j], b, sum[q]);
+                            for (int q = 0; q < R; ++q) sum[q] = gmm::few::Mini<X>::mfma(xv[q][j], b, sum[q]);
                         }
                         const float f = Num<T>::to_f32(sc[i][u].v[g]);
 #pragma unroll
@@ -243,13 +243,13 @@ __device__ __forceinline__ void dots(f32x4 (&acc)[U][R], const char *const (&w)[
                 }
             }
     }
-    if constexpr (Num<T>::kUnit != 1.0f)
+    if constexpr (Num<X>::kUnit != 1.0f)
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int q = 0; q < R; ++q)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc[u][q][e] *= Num<T>::kUnit;
+                for (int e = 0; e < 4; ++e) acc[u][q][e] *= Num<X>::kUnit;
 }
 
 }  // namespace int4

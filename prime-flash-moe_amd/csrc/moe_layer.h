@@ -15,9 +15,12 @@
 // contiguous bytes, straight into registers, and a lane multiplies its eight with those of up to eight tokens by dot products
 // of two elements with fp32 sums.  (No matrix instruction wants its operands in whole lines of 128 bytes.)  Weights of 4 bits: int4_tile.h.
 //
-// The activation is kept as the sum of two 16-bit numbers, the rounded value and the rounded rest, of which the down
-// projection multiplies both: 16 bits or more of mantissa at two dot products (or two rows of a matrix instruction that has rows to
-// spare) instead of one, so that the output is rounded once.
+// The activation keeps the range of fp32 and 16 bits of mantissa or more, so that the output is rounded once, in 32 bits a value.  With fp16
+// weights of 16 bits it is fp32: an instruction multiplies half of a register of fp16 with fp32, as many of them as dot products of two halves.
+// Otherwise it is the sum of two bf16 numbers, the rounded value and the rounded rest, of which the down projection
+// multiplies both, at two dot products (or two rows of a matrix instruction that has rows to spare) instead of one; integers of 4 bits are
+// whole in bf16 whatever the layer's type is.  (Two fp16 numbers end at 65504, where activations of fp16 layers do not, and lose the rest's bits
+// below 2^-9.)
 #pragma once
 #include "int4_tile.h"
 #include "route_topk.h"
@@ -50,7 +53,7 @@ struct Args {
     int32_t *topk_ids;
     float *topk_weights;
     float *logits;  // (T, E)
-    char *act;      // [pair][2: value, rest][act_pitch bytes]
+    char *act;      // [pair][2][act_pitch bytes]: values, rests; or whole ones: columns 8 c .. + 3, columns 8 c + 4 .. + 7 behind byte 16 c
     int act_pitch;
     float *shares;  // [workgroup][2: of its first strip, of its last one][token][column]: sums of workgroups that share a strip of out
     int T, K, H, E, top_k;
@@ -84,7 +87,7 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
-// What a word of the activation (two columns) holds until its up job has written it: two NaNs that no job writes.  So a word says by
+// What a word of the activation holds until its up job has written it: a NaN, or two, that no job writes.  So a word says by
 // itself whether it is there, and where a cached one says that it is not, memory is asked again: nothing else is needed between
 // the up jobs and the down jobs, no counter behind the stores, no cache to be emptied.
 constexpr uint32_t kAbsent = 0xffffffffu;
@@ -107,8 +110,9 @@ struct Arrival {
 // acc[q][n] += this lane's share of a weight row times row n of x: steps s0 .. s1 - 1 of 128 elements.  `w[q]` begins four weight rows,
 // `pitch` bytes apart, of which a lane has number lane / 16, `last` at most; row n begins at byte xo[n] of `x`, which holds `x_bytes`
 // (all wave-uniform).  `k`: elements of a row, a multiple of 8; nothing is read behind them.  Only the first `live` of the Q are there.  The
-// weights of S steps are in flight together, of x SX steps of NX rows.  wait: see int4::dots.
-template <class T, int Q, int N, int S, int SX, int NX = N, class Wait = int4::NoWait>
+// weights of S steps are in flight together, of x SX steps of NX rows.  WHOLE: two rows of x are one of fp32, the first four of every eight
+// columns and the others (T is F16).  wait: see int4::dots.
+template <class T, int Q, int N, int S, int SX, int NX = N, bool WHOLE = false, class Wait = int4::NoWait>
 __device__ __forceinline__ void row_dots(float (&acc)[Q][N], const char *const (&w)[Q], int pitch, const char *x, uint32_t x_bytes, const uint32_t (&xo)[N], int s0,
                                          int s1, int k, int live = Q, int last = 3, Wait wait = {}) {
     const int lane = threadIdx.x & 63;
@@ -120,6 +124,21 @@ __device__ __forceinline__ void row_dots(float (&acc)[Q][N], const char *const (
         if (q < live) wb[q] = int4::buffer(w[q], 4u * (uint32_t)pitch);
     const int4::Buffer xb = int4::buffer(x, x_bytes);
     auto multiply = [&](const i32x4 (&wv)[Q], const i32x4 (&xv)[NX], int n0) {
+        if constexpr (WHOLE) {
+            // (by columns, so that no sum waits for the one before it)
+#pragma unroll
+            for (int d = 0; d < 4; ++d)
+#pragma unroll
+                for (int q = 0; q < Q; ++q)
+                    if (q < live)
+#pragma unroll
+                        for (int n = 0; n < NX; ++n) {
+                            const int word = wv[q][n % 2 * 2 + d / 2];  // (a value: of an element of a vector the cast would take the first)
+                            const f16x2 pair = __builtin_bit_cast(f16x2, word);
+                            acc[q][n0 + n] = fmaf((float)pair[d % 2], __int_as_float(xv[n][d]), acc[q][n0 + n]);
+                        }
+            return;
+        }
 #pragma unroll
         for (int q = 0; q < Q; ++q)
             if (q < live)
@@ -352,11 +371,13 @@ __device__ __forceinline__ void by_height(int n, F f) {
     }
 }
 
-// Two 16-bit numbers that add up to v (of what is beyond the type the first alone; one NaN for all, see kAbsent).
-template <class T>
+// Two bf16 numbers that add up to v (infinity and NaN the first alone; one NaN for all, see kAbsent).  What would round to infinity has the
+// largest number in front of its rest.
 __device__ __forceinline__ uint32_t split(float v) {
-    const uint16_t hi = v != v ? Num<T>::kNan : Num<T>::from_f32(v);
-    const uint16_t lo = Num<T>::finite(hi) ? Num<T>::from_f32(v - Num<T>::to_f32(hi)) : 0;
+    using N = Num<Bf16>;
+    uint16_t hi = v != v ? N::kNan : N::from_f32(v);
+    if (!N::finite(hi) && fabsf(v) <= 0x1.fffffep127f) --hi;
+    const uint16_t lo = N::finite(hi) ? N::from_f32(v - N::to_f32(hi)) : 0;
     return hi | (uint32_t)lo << 16;
 }
 
@@ -376,7 +397,7 @@ struct Sums {
 
 // What the columns of an up job have from every wave -> activation, two columns a thread.  The stores go through to where all XCDs see
 // them.  LOG: see Args::up_log.
-template <class T, bool ONE, int LOG>
+template <class W, bool ONE, int LOG>
 __device__ __forceinline__ void finish_up(const Args &a, const Plan &p, const UpSums &s, int u, int col0) {
     constexpr int WAVES = kWaves >> LOG;
     const uint32_t tokens = tokens_of<ONE>(p, u);
@@ -389,10 +410,19 @@ __device__ __forceinline__ void finish_up(const Args &a, const Plan &p, const Up
 #pragma unroll
             for (int i = 0; i < 2; ++i) gate[i] += s.part[strip * WAVES + k][0][j][c + i], up[i] += s.part[strip * WAVES + k][1][j][c + i];
         const int t = ONE ? 0 : token_of(tokens, j);
-        const uint32_t v0 = split<T>(swiglu(gate[0], up[0])), v1 = split<T>(swiglu(gate[1], up[1]));
-        char *at = a.act + (int64_t)pair_of<ONE>(a, p, u, t) * 2 * a.act_pitch + (col0 + c) * 2;
-        __hip_atomic_store(reinterpret_cast<uint32_t *>(at), (v0 & 0xffffu) | v1 << 16, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(reinterpret_cast<uint32_t *>(at + a.act_pitch), v0 >> 16 | (v1 & 0xffff0000u), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const float v[2] = {swiglu(gate[0], up[0]), swiglu(gate[1], up[1])};
+        char *const row = a.act + (int64_t)pair_of<ONE>(a, p, u, t) * 2 * a.act_pitch;
+        const int col = col0 + c;
+        if constexpr (W::kWhole) {
+            uint32_t *const at = reinterpret_cast<uint32_t *>(row + (col & 4 ? a.act_pitch : 0) + col / 8 * 16 + col % 4 * 4);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) __hip_atomic_store(at + i, v[i] != v[i] ? 0x7fc00000u : __float_as_uint(v[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        } else {
+            const uint32_t v0 = split(v[0]), v1 = split(v[1]);
+            char *const at = row + col * 2;
+            __hip_atomic_store(reinterpret_cast<uint32_t *>(at), (v0 & 0xffffu) | v1 << 16, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(reinterpret_cast<uint32_t *>(at + a.act_pitch), v0 >> 16 | (v1 & 0xffff0000u), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
     }
 }
 
@@ -401,6 +431,7 @@ template <class T, int QUADS>
 struct Wide {
     using Type = T;
     static constexpr int kDownCols = 8, kMaxUpLog = 0;
+    static constexpr bool kWhole = std::is_same<T, F16>::value;  // the activation is fp32
 
     // The waves share the contraction; each has the gate and up rows of all columns, so that a row of x is read for up to 32 of them.
     template <bool ONE>
@@ -466,7 +497,7 @@ struct Wide {
                 xo[2 * j] = (uint32_t)pair[j] * 2u * (uint32_t)a.act_pitch;
                 xo[2 * j + 1] = xo[2 * j] + a.act_pitch;
             }
-            row_dots<T, 2, 2 * N, (N == 1 ? 6 : N == 2 ? 4 : 2), (N == 1 ? 3 : N == 2 ? 2 : 1)>(acc, w, a.H * 2, a.act, (uint32_t)(a.T * a.top_k) * 2u * (uint32_t)a.act_pitch, xo, s0, s1, a.H, 2, 3, Arrival{&p.failed});
+            row_dots<T, 2, 2 * N, (N == 1 ? 6 : N == 2 ? 4 : 2), (N == 1 ? 3 : N == 2 ? 2 : 1), 2 * N, kWhole>(acc, w, a.H * 2, a.act, (uint32_t)(a.T * a.top_k) * 2u * (uint32_t)a.act_pitch, xo, s0, s1, a.H, 2, 3, Arrival{&p.failed});
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const float v0 = row_sum(acc[0][2 * j] + acc[0][2 * j + 1]), v1 = row_sum(acc[1][2 * j] + acc[1][2 * j + 1]);
@@ -483,6 +514,7 @@ template <class T, int GROUP>
 struct Narrow {
     using Type = T;
     static constexpr int kDownCols = 16, kMaxUpLog = 2;
+    static constexpr bool kWhole = false;
 
     // 8 >> up_log waves share the contraction of a strip of gate rows and the matching one of up rows.
     template <bool ONE>
@@ -503,7 +535,7 @@ struct Narrow {
         auto row = [&](int q) { return ONE ? 0u : (uint32_t)token_of(tokens, q) * (uint32_t)a.K * 2; };
         by_height<ONE>(last + 1, [&](auto m) {
             constexpr int M = decltype(m)::value, S = M == 4 || (M == 8 && GROUP > 32) ? 2 : 1;  // (what registers there are)
-            int4::dots<T, GROUP, 2, 1, S, M>(acc, w, s, a.x, row, last + 1, t0, t1, a.K, rows);
+            int4::dots<T, T, GROUP, 2, 1, S, M>(acc, w, s, a.x, row, last + 1, t0, t1, a.K, rows);
         });
 #pragma unroll
         for (int i = 0; i < 4; ++i) sums.part[wave][0][4 * c + i][r] = acc[0][0][i], sums.part[wave][1][4 * c + i][r] = acc[1][0][i];
@@ -537,7 +569,7 @@ struct Narrow {
             const int n = 2 * min(last + 1 - row0, 8);
             by_height<ONE>(n, [&](auto m) {
                 constexpr int M = decltype(m)::value, S = 16 / M;
-                int4::dots<T, GROUP, 1, 1, S, M>(acc, w, s, a.act, row, n, s0, s1, a.H, rows, Arrival{&p.failed});
+                int4::dots<Bf16, T, GROUP, 1, 1, S, M>(acc, w, s, a.act, row, n, s0, s1, a.H, rows, Arrival{&p.failed});
             });
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -672,9 +704,9 @@ __device__ __forceinline__ void up_jobs(const Args &a, Plan &p, Sums &sh, int ti
             W::template up<ONE>(a, p, sh, u, job - u * strips);
             __syncthreads();
             const int col0 = (job - u * strips) * a.up_cols;
-            if (W::kMaxUpLog == 0 || a.up_log == 0) finish_up<typename W::Type, ONE, 0>(a, p, sh.up, u, col0);
-            else if (a.up_log == 1) finish_up<typename W::Type, ONE, (W::kMaxUpLog > 0)>(a, p, sh.up, u, col0);
-            else finish_up<typename W::Type, ONE, W::kMaxUpLog>(a, p, sh.up, u, col0);
+            if (W::kMaxUpLog == 0 || a.up_log == 0) finish_up<W, ONE, 0>(a, p, sh.up, u, col0);
+            else if (a.up_log == 1) finish_up<W, ONE, (W::kMaxUpLog > 0)>(a, p, sh.up, u, col0);
+            else finish_up<W, ONE, W::kMaxUpLog>(a, p, sh.up, u, col0);
         } else if (own && down_too) {
             own = false;
             const int wave = gmm::uniform(tid >> 6), n = mine.to - mine.from, at = mine.from + (wave * n >> kWavesLog), end = mine.from + ((wave + 1) * n >> kWavesLog);
@@ -689,7 +721,7 @@ __device__ __forceinline__ void up_jobs(const Args &a, Plan &p, Sums &sh, int ti
     // (The last word of the last job: most others are there when it is, and lines that are not would be in the L2 for nothing.)
     if (tid == 0 && down_too) {
         const int u = p.n - 1, t = ONE ? 0 : __builtin_ctz(p.tokens[u]);
-        const int32_t *word = reinterpret_cast<const int32_t *>(a.act + (int64_t)pair_of<ONE>(a, p, u, t) * 2 * a.act_pitch + a.H * 2 - 4);
+        const int32_t *word = reinterpret_cast<const int32_t *>(a.act + ((int64_t)pair_of<ONE>(a, p, u, t) * 2 + 1) * a.act_pitch + a.H * 2 - 4);
 #pragma unroll 1
         for (int64_t tries = 0; (uint32_t)load_device(word) == kAbsent; ++tries) {
             if (tries >= kMostTries) {
