@@ -410,7 +410,10 @@ __device__ __forceinline__ void finish_up(const Args &a, const Plan &p, const Up
 #pragma unroll
             for (int i = 0; i < 2; ++i) gate[i] += s.part[strip * WAVES + k][0][j][c + i], up[i] += s.part[strip * WAVES + k][1][j][c + i];
         const int t = ONE ? 0 : token_of(tokens, j);
-        const float v[2] = {swiglu(gate[0], up[0]), swiglu(gate[1], up[1])};
+        // (the gate's curve first: gate * up may be beyond fp32 where what is left of it is not)
+        float v[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v[i] = gate[i] * __builtin_amdgcn_rcpf(1.0f + __expf(-gate[i])) * up[i];
         char *const row = a.act + (int64_t)pair_of<ONE>(a, p, u, t) * 2 * a.act_pitch;
         const int col = col0 + c;
         if constexpr (W::kWhole) {

@@ -125,6 +125,20 @@ def test_an_activation_between_the_largest_numbers_of_two_types(device):
     check(prime_moe.moe_layer(x, gate, w1, w2, 1, bias), x, w1, w2, bias, 2.0 ** -17)
 
 
+def test_gates_that_take_back_what_their_product_would_be(device):
+    """gate * up beyond fp32, the activation far inside."""
+    import prime_moe
+    K, H = 64, 32
+    x = torch.zeros((2, K), dtype=BF16, device=device)
+    x[0, 0], x[1, 0] = 1.0, 1.125
+    w1 = torch.zeros((1, 2 * H, K), dtype=BF16, device=device)
+    w1[0, :H, 0] = torch.arange(-64, -32)
+    w1[0, H:, 0] = 2.0 ** 125
+    w2 = torch.full((1, K, H), 2.0 ** -60, dtype=BF16, device=device)
+    bias = torch.zeros(1, device=device)
+    check(prime_moe.moe_layer(x, torch.zeros((1, K), dtype=BF16, device=device), w1, w2, 1, bias), x, w1, w2, bias, 2.0 ** -17)
+
+
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("kind", ["wide", "narrow"])
 def test_infinite_activations(device, dtype, kind):
