@@ -474,7 +474,8 @@ struct Wide {
     // Address of line `lane` of steps s0 .. s1 - 1 of a strip of out (null: there are fewer).
     static __device__ __forceinline__ const char *down_line(const Args &a, const Plan &p, int u, int strip, int s0, int s1, int lane) {
         const int row = lane % 8, line = lane / 8, at = s0 * 256 + line * 128;
-        return line < (s1 - s0) * 2 && at < a.H * 2 ? down_weights(a, p, u, strip) + (int64_t)row * a.H * 2 + at : nullptr;
+        const char *const first = down_weights(a, p, u, strip);
+        return line < (s1 - s0) * 2 && at < a.H * 2 ? first + (int64_t)row * a.H * 2 + at : nullptr;
     }
     static __device__ __forceinline__ const char *down_weights(const Args &a, const Plan &p, int u, int strip) {
         return a.w2 + ((int64_t)gmm::uniform(p.expert[u]) * a.K + strip * kDownCols) * a.H * 2;
@@ -546,7 +547,8 @@ struct Narrow {
 
     static __device__ __forceinline__ int down_steps(const Args &a) { return int4::tiles_of(a.H); }
     static __device__ __forceinline__ const char *down_line(const Args &a, const Plan &p, int u, int strip, int s0, int s1, int lane) {
-        return lane < (s1 - s0) * (int4::kTileBytes / 128) ? down_weights(a, p, u, strip) + (int64_t)s0 * int4::kTileBytes + lane * 128 : nullptr;
+        const char *const first = down_weights(a, p, u, strip);
+        return lane < (s1 - s0) * (int4::kTileBytes / 128) ? first + (int64_t)s0 * int4::kTileBytes + lane * 128 : nullptr;
     }
     static __device__ __forceinline__ const char *down_weights(const Args &a, const Plan &p, int u, int strip) {
         return a.w2 + ((int64_t)gmm::uniform(p.expert[u]) * (a.K / 16) + strip) * int4::tiles_of(a.H) * int4::kTileBytes;
