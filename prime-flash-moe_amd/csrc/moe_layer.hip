@@ -119,7 +119,8 @@ extern "C" int pmoe_moe_layer(const void *x, const void *gate, const float *bias
                               const void *w2_scale, int group, void *out, int32_t *topk_ids, float *topk_weights, int T, int K, int H,
                               int num_experts, int top_k, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
     PMOE_REQUIRE(dtype == PMOE_DTYPE_BF16 || dtype == PMOE_DTYPE_F16, "moe_layer: dtype must be bf16 or fp16");
-    PMOE_REQUIRE(T >= 0 && T <= kMaxTokens, "moe_layer takes up to %d tokens, got %d (more: route and fused_moe_bf16)", kMaxTokens, T);
+    PMOE_REQUIRE(T >= 0 && T <= kMaxTokens, "moe_layer takes up to %d tokens, got %d (more: %s)", kMaxTokens, T,
+                 group != 0 ? "route and grouped_mm_int4" : dtype == PMOE_DTYPE_F16 ? "route and grouped_mm" : "route and fused_moe_bf16");
     PMOE_REQUIRE(num_experts > 0 && num_experts <= kMaxExperts, "moe_layer supports 1..%d experts, got %d", kMaxExperts, num_experts);
     PMOE_REQUIRE(top_k > 0 && top_k <= kMaxTopK && top_k <= num_experts, "moe_layer: top_k must be in 1..min(%d, num_experts), got %d", kMaxTopK, top_k);
     PMOE_REQUIRE(group == 0 || group == 32 || group == 64 || group == 128, "moe_layer: group must be 0 (16-bit weights), 32, 64 or 128, got %d", group);

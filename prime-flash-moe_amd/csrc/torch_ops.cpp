@@ -614,7 +614,9 @@ LayerSizes check_layer(const char *op, const Layer &l, bool placement) {
     const int64_t T = l.x.size(0), K = l.x.size(1), E = l.gate.size(0);
     require_16bit(op, "x", l.x);
     REQUIRE(l.gate.scalar_type() == l.x.scalar_type(), op, ": x and gate must have the same dtype");
-    REQUIRE(T <= kMostTokens, op, " takes up to ", kMostTokens, " tokens, got ", T, " (more: route and fused_moe_bf16)");
+    REQUIRE(T <= kMostTokens, op, " takes up to ", kMostTokens, " tokens, got ", T, " (more: ",
+            l.w1_scale != nullptr ? "route, expert_offsets and grouped_mm_int4, or grouped_mm on what dequantize_int4 returns"
+            : l.x.scalar_type() == at::kHalf ? "route, expert_offsets and grouped_mm" : "route and fused_moe_bf16", ")");
     REQUIRE(E > 0 && E <= kMostExperts, op, " supports 1..", kMostExperts, " experts, got ", E);
     REQUIRE(l.top_k > 0 && l.top_k <= std::min(kMostTopK, E), op, ": top_k must be in 1..min(", kMostTopK, ", E), got ", l.top_k);
     LayerSizes z{0, 0};

@@ -378,7 +378,8 @@ def moe_layer(x: torch.Tensor, gate: torch.Tensor, w1: torch.Tensor, w2: torch.T
     softmax over the selected logits; ``out`` (T, K) the sum of ``weight * (w2[e] @ (silu(g) * u))`` with ``g`` and ``u`` the two
     halves of ``w1[e] @ x``.  ``x`` (T, K), ``gate`` (E, K), ``w1`` (E, 2H, K) with the gate rows first, ``w2`` (E, K, H): contiguous,
     all bfloat16 or all float16, K and H multiples of 8, at most 512 experts; ``bias`` (E,) float32.  Sums in fp32, one rounding at
-    the end; the same bits every time.  No gradients.  More than 16 tokens: :func:`route` and :func:`fused_moe_bf16`.
+    the end; the same bits every time.  No gradients.  More than 16 tokens: :func:`route` and :func:`fused_moe_bf16`, in
+    float16 :func:`route`, :func:`expert_offsets` and :func:`grouped_mm`.
     """
     return torch.ops.prime_moe.moe_layer(x, gate, w1, w2, top_k, bias)
 
@@ -387,7 +388,8 @@ def moe_layer_int4(x: torch.Tensor, gate: torch.Tensor, w1: torch.Tensor, w1_sca
                    w2_scale: torch.Tensor, top_k: int, bias: torch.Tensor = None):
     """:func:`moe_layer` with experts of 4 bits: ``w1``, ``w1_scale`` and ``w2``, ``w2_scale`` from :func:`quantize_int4` or
     :func:`pack_int4`, of (E, 2H, K) and (E, K, H) weights with one group size and scales of the type of ``x``.  K and H are
-    multiples of the group (and with it of 16)."""
+    multiples of the group (and with it of 16).  More than 16 tokens: :func:`route`, :func:`expert_offsets` and
+    :func:`grouped_mm_int4`, or :func:`grouped_mm` on what :func:`dequantize_int4` returns."""
     return torch.ops.prime_moe.moe_layer_int4(x, gate, w1, w1_scale, w2, w2_scale, top_k, bias)
 
 
