@@ -249,7 +249,8 @@ int pmoe_dequantize_int4(const void *q, const void *scales, void *out, int dtype
 /*
  * grouped_mm_int4 -- pmoe_grouped_mm with weights of 4 bits, made for few rows per group: x (M,K), out (M,N) and w_scale bf16 or
  *   fp16 (dtype), fp32 sums, rounded once; zero for rows behind the last group.  offsets == NULL: one matrix for all rows.
- *   A row of x that holds an infinity or a NaN comes out as NaN.  Every 32 rows of a group read its weights again.
+ *   A row of x that holds an infinity or a NaN comes out as NaN.  Every 16 rows of a group read its weights again, or, where there
+ *   are more than 14 on average of all groups (16 of a single matrix), every 32.
  */
 int pmoe_grouped_mm_int4(const void *x, const void *w, const void *w_scale, void *out, const int32_t *offsets, int n_groups,
                          int64_t M, int N, int K, int group, int64_t x_stride, int dtype, void *stream);
@@ -260,6 +261,8 @@ int pmoe_grouped_mm_int4(const void *x, const void *w, const void *w_scale, void
  *   x (T,K), gate (E,K), out (T,K); w1 (E,2H,K), gate rows first, and w2 (E,K,H); all of dtype (bf16 or fp16) and contiguous,
  *   or, with group != 0, w1 and w2 of 4 bits with their scales.  bias (E) fp32 or null.  topk_ids, topk_weights (T,top_k): what was
  *   chosen.  K and H are multiples of 8, with weights of 4 bits of 16 and of group.  num_experts <= 512, top_k <= min(32, E).
+ *   The activation keeps the range of fp32 and 16 bits of mantissa or more, in fp16 too.  With weights of 4 bits a token whose x or
+ *   activation holds an infinity or a NaN comes out as NaN.  16-bit weights of an expert are read again for every four of its tokens.
  *   The workspace, 256-byte aligned, is scratch of this one call.
  */
 size_t pmoe_moe_layer_workspace_bytes(int T, int H, int num_experts, int top_k);

@@ -85,7 +85,8 @@ __device__ __forceinline__ Buffer buffer(const char *p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(ring::uniform_ptr(p)), 0, (int)bytes, 0x00020000);  // (raw bytes, no stride)
 }
 __device__ __forceinline__ i32x4 load(Buffer b, uint32_t lane, uint32_t wave) { return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(b, lane, wave, 0)); }
-// The same with the non-temporal hint, for what no other workgroup reads.
+// The same with the non-temporal hint, for what no other workgroup reads.  (The workgroup itself does, of experts with more rows than it takes at
+// a time.)
 __device__ __forceinline__ i32x4 load_once(Buffer b, uint32_t lane, uint32_t wave) { return __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(b, lane, wave, 2)); }
 
 // The same, as it stands in memory now, whatever the caches of the XCD hold.

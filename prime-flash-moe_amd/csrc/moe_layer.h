@@ -3,7 +3,7 @@
 //   l[t][e] = x[t] . gate[e] (+ bias[e]);  S(t): the top_k largest, ties to the lower index;  a[t][.] = softmax over S(t)
 //   out[t]  = sum over e in S(t) of a[t][e] W2[e] (silu(G[e] x[t]) * (U[e] x[t])),  G: rows 0 .. H - 1 of W1[e], U: rows H .. 2H - 1
 //
-// With so few tokens every weight is used a few times at most: the stream of the touched experts' weights from HBM bounds the large
+// With so few tokens most experts have a row or two: the stream of the touched experts' weights from HBM bounds the large
 // layers (16 tokens on 128 experts of 2048 x 768, 778 MB: 138 us, 5.6 TB/s), a chain of latencies the small ones (one token on
 // them, 76 MB: 22.7 us, of which the logits take 2, the next kernel's start 1, the plan 2.5, the up jobs and the wait for the last 9,
 // the down projection 6).  Nothing is sorted or padded: a workgroup finds the touched experts and their tokens by itself, from the
@@ -12,8 +12,9 @@
 // first were idle, and the second began with its weights' latency.)
 //
 // Weights of 16 bits, rows of (E, 2H, K) and (E, K, H): sixteen lanes share a weight row, a step of theirs is 128 elements, 256
-// contiguous bytes, straight into registers, and a lane multiplies its eight with those of up to eight tokens by dot products
-// of two elements with fp32 sums.  (No matrix instruction wants its operands in whole lines of 128 bytes.)  Weights of 4 bits: int4_tile.h.
+// contiguous bytes, straight into registers, and a lane multiplies its eight with those of up to four tokens (eight in jobs of four columns) by
+// dot products of two elements with fp32 sums.  An expert with more rows has its weights loaded again for the next ones, which is what
+// bounds layers of few small experts (16 tokens, 4 of 8 experts of 4096 x 256: 44 us for 50 MB).  Weights of 4 bits: int4_tile.h.
 //
 // The activation keeps the range of fp32 and 16 bits of mantissa or more, so that the output is rounded once, in 32 bits a value.  With fp16
 // weights of 16 bits it is fp32: an instruction multiplies half of a register of fp16 with fp32, as many of them as dot products of two halves.

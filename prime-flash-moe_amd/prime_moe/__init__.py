@@ -328,7 +328,8 @@ def quantize_int4(w: torch.Tensor, group: int = 128, scale_dtype: torch.dtype = 
 
 def pack_int4(values: torch.Tensor, scale: torch.Tensor):
     """``(q, scale)`` as :func:`quantize_int4` lays them out, from integers ``values`` (..., N, K) int8, -8 to 7, and their scales
-    (..., N, K / group), bfloat16 or float16.  Load-time work, plain torch, on the device of ``values``."""
+    (..., N, K / group), bfloat16 or float16.  Load-time work, plain torch, on the device of ``values``, with about 2.5 bytes a
+    weight beside its arguments at the peak and two waits for the device (a large stack may be packed matrix by matrix)."""
     if values.dtype != torch.int8 or values.dim() < 2:
         raise RuntimeError("pack_int4: values must be int8 (..., N, K)")
     if scale.dtype not in (torch.bfloat16, torch.float16):
@@ -362,8 +363,8 @@ def grouped_mm_int4(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, off
     """:func:`grouped_mm` with weights of 4 bits: ``w``, ``w_scale`` from :func:`quantize_int4` or :func:`pack_int4`, of (E, N, K)
     weights, or of an (N, K) matrix without ``offsets`` (a dense product).
 
-    Made for few rows per expert, as in decoding: every 32 rows of an expert read its weights again (for many rows:
-    :func:`dequantize_int4`).  ``x`` (M, K) bfloat16 or float16 with a contiguous last dimension, rows a multiple of 8 elements
+    Made for few rows per expert, as in decoding: every 16 rows of an expert read its weights again, or, where the experts have more
+    than 14 on average (a single matrix more than 16), every 32 (for many rows: :func:`dequantize_int4`).  ``x`` (M, K) bfloat16 or float16 with a contiguous last dimension, rows a multiple of 8 elements
     apart, 16-byte aligned; ``w_scale`` of the same type.  Sums in fp32, rounded once; a row of ``x`` that holds an infinity or a
     NaN comes out as NaN.  No gradients.
     """
@@ -377,8 +378,9 @@ def moe_layer(x: torch.Tensor, gate: torch.Tensor, w1: torch.Tensor, w2: torch.T
     the ``top_k`` largest of ``x @ gate.T + bias``, largest first, ties to the lower index; ``topk_weights`` (T, top_k) float32,
     softmax over the selected logits; ``out`` (T, K) the sum of ``weight * (w2[e] @ (silu(g) * u))`` with ``g`` and ``u`` the two
     halves of ``w1[e] @ x``.  ``x`` (T, K), ``gate`` (E, K), ``w1`` (E, 2H, K) with the gate rows first, ``w2`` (E, K, H): contiguous,
-    all bfloat16 or all float16, K and H multiples of 8, at most 512 experts; ``bias`` (E,) float32.  Sums in fp32, one rounding at
-    the end; the same bits every time.  No gradients.  More than 16 tokens: :func:`route` and :func:`fused_moe_bf16`, in
+    all bfloat16 or all float16, K and H multiples of 8, at most 512 experts; ``bias`` (E,) float32.  Sums in fp32, the activation
+    in its range and with 16 bits of mantissa or more in both types, one rounding to 16 bits at the end; the same bits every time.
+    Made for few tokens per expert: every four of them read its weights again.  No gradients.  More than 16 tokens: :func:`route` and :func:`fused_moe_bf16`, in
     float16 :func:`route`, :func:`expert_offsets` and :func:`grouped_mm`.
     """
     return torch.ops.prime_moe.moe_layer(x, gate, w1, w2, top_k, bias)
@@ -388,7 +390,7 @@ def moe_layer_int4(x: torch.Tensor, gate: torch.Tensor, w1: torch.Tensor, w1_sca
                    w2_scale: torch.Tensor, top_k: int, bias: torch.Tensor = None):
     """:func:`moe_layer` with experts of 4 bits: ``w1``, ``w1_scale`` and ``w2``, ``w2_scale`` from :func:`quantize_int4` or
     :func:`pack_int4`, of (E, 2H, K) and (E, K, H) weights with one group size and scales of the type of ``x``.  K and H are
-    multiples of the group (and with it of 16).  More than 16 tokens: :func:`route`, :func:`expert_offsets` and
+    multiples of the group (and with it of 16).  A token whose ``x`` or activation holds an infinity or a NaN comes out as NaN.  More than 16 tokens: :func:`route`, :func:`expert_offsets` and
     :func:`grouped_mm_int4`, or :func:`grouped_mm` on what :func:`dequantize_int4` returns."""
     return torch.ops.prime_moe.moe_layer_int4(x, gate, w1, w1_scale, w2, w2_scale, top_k, bias)
 
