@@ -18,7 +18,8 @@
 // bf16 reaches as far as fp32, and 24 times a sum of 128 of it further.  So bf16 weights are 2^-12 (24 + q), from 2^-8 in place of 16.0: no
 // sum of a group passes 24 x 128 x 2^-12 = 0.75 of the largest |x|, and the 2^12 come back in the wave's sum, where all rows of weights
 // have been scaled.  Powers of two change no bit of what stays above 2^-126; the products of the least numbers are subnormal, which
-// the matrix instructions keep.
+// the matrix instructions keep.  (What is left of it: scaled sums have steps of 2^-149, so that those of outputs below 2^-114 are
+// rounded to multiples of 2^-137.)
 //
 // Sums of a group are scaled in fp32, by four multiply-adds per 128 / group tiles.
 #pragma once

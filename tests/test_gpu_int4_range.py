@@ -90,6 +90,22 @@ def test_rows_of_the_smallest_numbers(device, group):
         assert torch.equal(y, R.mm(x, values[None], scale[None], [M])[0].to(BF16))
 
 
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("size", [-124, -118, -112, -104])
+def test_outputs_of_the_smallest_numbers(device, size, group):
+    """Each of the K / group + 8 sums that make an output may be rounded by half of 2^-137, beside what int4_ref.check allows."""
+    import prime_moe
+    gen = torch.Generator().manual_seed(group - size)
+    M, N, K = 5, 64, 1024
+    values = torch.randint(-8, 8, (N, K), generator=gen, dtype=torch.int8).to(device)
+    scale = ((torch.rand((N, K // group), generator=gen) + 0.5) * 2.0 ** (size // 2)).to(BF16).to(device)
+    x = (torch.randn((M, K), generator=gen).double() * 2.0 ** (size - size // 2 - 7)).to(BF16).to(device)
+    y = prime_moe.grouped_mm_int4(x, *prime_moe.pack_int4(values, scale))
+    ref, m = R.mm(x, values[None], scale[None], [M])
+    sums = R.sums_bound(m, K, group) + (K / group + 8) * 2.0 ** -138
+    assert ((y.double() - ref).abs() <= sums + 2.0 ** -8 * (ref.abs() + sums) + 2.0 ** -134).all() and (y != 0).any()
+
+
 @pytest.mark.parametrize("T", [1, 2, 5, 16])
 @pytest.mark.parametrize("group", [32, 128])
 def test_layer_of_4_bits_with_large_rows(device, T, group):
