@@ -333,13 +333,13 @@ __device__ __forceinline__ void store_tile(const typename T::Acc (&acc)[4][FM], 
     unrolled<PARTS>([&](auto part) {
         constexpr int t = part.value / (4 / FRAGS), h = part.value % (4 / FRAGS);
         i32x4 v[READS];
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
 #pragma unroll
         for (int it = 0; it < READS; ++it) {
             const int row = it * PER_READ + sub;
             v[it] = *reinterpret_cast<const i32x4 *>(scratch + row * ROW + ((chunk ^ (row % CHUNKS)) << 4));
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_lds_order();
         if constexpr (part.value + 1 < PARTS) put(std::integral_constant<int, part.value + 1>());
         PMOE_GMM_FENCE();
         char *to = out + t * 32 * pitch + h * ROW;  // wave-uniform

@@ -7,7 +7,7 @@ import subprocess
 import pytest
 
 VECTOR = r"<\d+ x \w+>"
-EVENT = re.compile(rf"(?P<store>store {VECTOR} .*ptr addrspace\(3\))|(?P<load>load {VECTOR}, ptr addrspace\(3\))|(?P<fence>\bfence |\.s\.barrier)")
+EVENT = re.compile(rf"(?P<store>store {VECTOR} .*ptr addrspace\(3\))|(?P<load>load {VECTOR}, ptr addrspace\(3\))|(?P<fence>\bfence |\.s\.barrier|asm sideeffect .*~\{{memory\}})")
 
 
 def kernels(ir):
@@ -48,9 +48,10 @@ def unordered(blocks):
     return False
 
 
-@pytest.mark.parametrize("source", ["quantize_int4.hip", "grouped_int4.hip", "moe_layer.hip"])
+@pytest.mark.parametrize("source", ["quantize_int4.hip", "grouped_int4.hip", "moe_layer.hip", "grouped_mm.hip"])
 def test_a_fence_between_stores_and_reads_of_other_lanes_chunks(source, tmp_path):
-    """In the optimised code of every kernel: a fence (or the workgroup's barrier) stands between vectors stored to LDS and vectors
+    """In the optimised code of every kernel: a fence (the workgroup's barrier, assembly that
+    touches memory) stands between vectors stored to LDS and vectors
     read from it, in both orders, on every way through the kernel."""
     from prime_moe import build
     out = tmp_path / "kernels.ll"
